@@ -19,6 +19,11 @@ SOURCES = (
     ("dsa_inst.hip", ("-DDSA_T=bf16", "-DDSA_D=32")),
     ("dsa_inst.hip", ("-DDSA_T=float", "-DDSA_D=32")),
     ("dsa_capi.hip", ()),
+    ("dsa_hidden.hip", ()),
+    ("dsa_rms_inst.hip", ("-DDSA_TX=bf16", "-DDSA_TR=bf16")),
+    ("dsa_rms_inst.hip", ("-DDSA_TX=bf16", "-DDSA_TR=float")),
+    ("dsa_rms_inst.hip", ("-DDSA_TX=float", "-DDSA_TR=bf16")),
+    ("dsa_rms_inst.hip", ("-DDSA_TX=float", "-DDSA_TR=float")),
 )
 # bench.py's MFMA throughput probe (include/dsa_probe.h), a library of its own
 PROBE_PATH = PKG_DIR / "libdsa_probe.so"

@@ -24,7 +24,7 @@ DSA_STAGE_FOLD = 8
 DSA_STAGE_TABLE = 16  # the first half of FOLD: per-offset sums (workspace)
 DSA_STAGE_SUM = 32  # the second half: their fold onto dkr / dqr
 
-EXPECTED_VERSION = 13
+EXPECTED_VERSION = 14
 
 _i64x3 = ctypes.c_int64 * 3
 _i64x2 = ctypes.c_int64 * 2
@@ -102,6 +102,8 @@ class DsaBwdArgs(ctypes.Structure):
 DSA_BLOCK_LN = 0
 DSA_BLOCK_GELU = 1
 DSA_BLOCK_RTD = 2
+DSA_BLOCK_DROPOUT = 3
+DSA_BLOCK_RMS = 4
 
 
 class DsaLnArgs(ctypes.Structure):
@@ -195,6 +197,108 @@ class DsaRtdArgs(ctypes.Structure):
     ]
 
 
+class DsaDropoutArgs(ctypes.Structure):
+    """dsa_dropout_args (include/dsa_block.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("res", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("res_strides", _i64x2),
+        ("rows_per_group", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("dy", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dx_stride", ctypes.c_int64),
+        ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("seed", ctypes.c_uint64),
+        ("N", ctypes.c_int64),
+        ("C", ctypes.c_int32),
+        ("threshold", ctypes.c_uint32),
+        ("x_dtype", ctypes.c_int32),
+        ("res_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("dy_dtype", ctypes.c_int32),
+        ("dx_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+    ]
+
+
+class DsaRmsArgs(ctypes.Structure):
+    """dsa_rms_args (include/dsa_block.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("res", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("res_strides", _i64x2),
+        ("rows_per_group", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("z", ctypes.c_void_p),
+        ("z_stride", ctypes.c_int64),
+        ("rstd", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64),
+        ("dzu", ctypes.c_void_p),
+        ("dzu_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dx_stride", ctypes.c_int64),
+        ("dres", ctypes.c_void_p),
+        ("dres_stride", ctypes.c_int64),
+        ("dweight", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("seed", ctypes.c_uint64),
+        ("N", ctypes.c_int64),
+        ("C", ctypes.c_int32),
+        ("threshold", ctypes.c_uint32),
+        ("x_dtype", ctypes.c_int32),
+        ("res_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("dy_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class DsaEmbedArgs(ctypes.Structure):
+    """dsa_embed_args (include/dsa_block.h)."""
+
+    _fields_ = [
+        ("ids", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("dy", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64),
+        ("dweight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("N", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("padding", ctypes.c_int64),
+        ("C", ctypes.c_int32),
+        ("ids_bytes", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("dy_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 # Entry points of include/dsa_block.h (the fused row kernels).
 BLOCK_EXPORTS = (
     "dsa_block_workspace_bytes",
@@ -204,6 +308,14 @@ BLOCK_EXPORTS = (
     "dsa_bias_gelu_bwd",
     "dsa_rtd_loss_fwd",
     "dsa_rtd_loss_bwd",
+    "dsa_dropout_fwd",
+    "dsa_dropout_bwd",
+    "dsa_add_rms_fwd",
+    "dsa_add_rms_quant",
+    "dsa_add_rms_bwd",
+    "dsa_embed_workspace_bytes",
+    "dsa_embed_fwd",
+    "dsa_embed_bwd",
 )
 
 # Every entry point include/dsa.h declares.
@@ -264,6 +376,8 @@ def load() -> ctypes.CDLL:
         lib.dsa_version.restype = ctypes.c_int
         lib.dsa_block_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int64, ctypes.c_int32]
         lib.dsa_block_workspace_bytes.restype = ctypes.c_size_t
+        lib.dsa_embed_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int64]
+        lib.dsa_embed_workspace_bytes.restype = ctypes.c_size_t
         for name, st in (
             ("dsa_add_ln_fwd", DsaLnArgs),
             ("dsa_add_ln_bwd", DsaLnArgs),
@@ -271,6 +385,13 @@ def load() -> ctypes.CDLL:
             ("dsa_bias_gelu_bwd", DsaGeluArgs),
             ("dsa_rtd_loss_fwd", DsaRtdArgs),
             ("dsa_rtd_loss_bwd", DsaRtdArgs),
+            ("dsa_dropout_fwd", DsaDropoutArgs),
+            ("dsa_dropout_bwd", DsaDropoutArgs),
+            ("dsa_add_rms_fwd", DsaRmsArgs),
+            ("dsa_add_rms_quant", DsaRmsArgs),
+            ("dsa_add_rms_bwd", DsaRmsArgs),
+            ("dsa_embed_fwd", DsaEmbedArgs),
+            ("dsa_embed_bwd", DsaEmbedArgs),
         ):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]

@@ -23,7 +23,8 @@ the HIP kernels through the ``torch.library`` ops below, which have fake
 implementations for ``torch.compile`` and autograd registrations.  Hidden
 dropout p > 0 in training runs torch's dropout on the dense output (bias
 included, as the reference's ``dropout(dense(x))``) and then the residual
-LayerNorm kernel.  CPU tensors run the reference's blocks in torch
+LayerNorm kernel, or, with ``config.fused_hidden_dropout``, the dropout kernel
+of deberta_amd/hidden.py.  CPU tensors run the reference's blocks in torch
 operations (the kernels run on the GPU only).
 """
 
@@ -38,6 +39,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from deberta_amd import _eager, _lib
+from deberta_amd.hidden import FusedRMSNorm, _threshold, fused_add_rms_norm, fused_dropout, norm_out_dtype
 
 # As the attention ops (deberta_amd/ops.py): under torch.compile's CUDA-graph
 # modes these run between the captured graph partitions, not inside them
@@ -231,14 +233,6 @@ def call_add_ln(x, bias, res, gamma, beta, eps: float, out_dtype: torch.dtype):
     return torch.ops.deberta_amd.add_ln(x, bias, res, gamma, beta, eps, out_dtype)
 
 
-def _ln_out_dtype(x: Tensor, res: Optional[Tensor]) -> torch.dtype:
-    """torch's result dtype for LayerNorm(x + res): float32 under CUDA
-    autocast (layer_norm runs in float32 there), else the promoted dtype."""
-    if torch.is_autocast_enabled("cuda"):
-        return torch.float32
-    return x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
-
-
 def fused_add_layer_norm(
     x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], ln: nn.LayerNorm
 ) -> Tensor:
@@ -246,7 +240,7 @@ def fused_add_layer_norm(
     the last dim, with affine parameters)."""
     if ln.weight is None or ln.bias is None:
         raise ValueError("fused_add_layer_norm needs an affine LayerNorm")
-    y, _, _ = call_add_ln(x, bias, res, ln.weight, ln.bias, float(ln.eps), _ln_out_dtype(x, res))
+    y, _, _ = call_add_ln(x, bias, res, ln.weight, ln.bias, float(ln.eps), norm_out_dtype(x, res))
     return y
 
 
@@ -472,7 +466,10 @@ def _bce_loss(logits: Tensor, labels: Tensor, active: Optional[Tensor]) -> Tenso
 class FusedSelfOutput(nn.Module):
     """DebertaV2SelfOutput (deberta_v2_native.py:115-165): ``LayerNorm(
     dense(hidden) + input)``, the dense GEMM without its bias and the bias,
-    residual and LayerNorm in one kernel."""
+    residual and LayerNorm in one kernel.  With ``config.fused_hidden_dropout``
+    hidden dropout in training is :func:`deberta_amd.fused_dropout` (bias,
+    dropout and residual in one kernel, its keep bits drawn from torch's CPU
+    generator) in place of torch's."""
 
     def __init__(self, config: Any, in_features: Optional[int] = None) -> None:
         super().__init__()
@@ -480,8 +477,16 @@ class FusedSelfOutput(nn.Module):
         self.dense = nn.Linear(int(in_features or hidden), hidden)
         self.LayerNorm = nn.LayerNorm(hidden, eps=float(getattr(config, "layer_norm_eps", 1e-7)))
         self.dropout = nn.Dropout(float(getattr(config, "hidden_dropout_prob", 0.0)))
+        self.fused_dropout = bool(getattr(config, "fused_hidden_dropout", False))
+        if self.fused_dropout:
+            _threshold(self.dropout.p)
 
     def forward(self, hidden_states: Tensor, input_tensor: Tensor) -> Tensor:
+        if self.fused_dropout and self.training and self.dropout.p > 0.0:
+            # bias, dropout and residual in one kernel that stores no mask
+            x = F.linear(hidden_states, self.dense.weight)
+            x = fused_dropout(x, self.dropout.p, bias=self.dense.bias, res=input_tensor)
+            return fused_add_layer_norm(x, None, None, self.LayerNorm) if _on_gpu(x) else self.LayerNorm(x)
         if not _on_gpu(hidden_states):  # the reference's block in torch operations
             return self.LayerNorm(self.dropout(self.dense(hidden_states)) + input_tensor)
         if self.training and self.dropout.p > 0.0:
@@ -529,7 +534,8 @@ class FusedRTDHead(nn.Module):
     hidden[:, 0]))))``, with the LayerNorm of the CLS-conditioned states in
     one kernel (the CLS row read in place) and dense + bias + GELU in
     another; ``forward_loss`` also fuses the classifier with the
-    discriminator's BCE loss (rtd.py:1134-1139)."""
+    discriminator's BCE loss (rtd.py:1134-1139).  ``use_rmsnorm_heads``: the
+    norm is an RMS norm (:class:`deberta_amd.FusedRMSNorm`)."""
 
     def __init__(self, config: Any) -> None:
         super().__init__()
@@ -537,12 +543,11 @@ class FusedRTDHead(nn.Module):
         act = getattr(config, "hidden_act", "gelu")
         if act != "gelu":
             raise NotImplementedError(f"FusedRTDHead supports hidden_act 'gelu', got {act!r}")
-        if bool(getattr(config, "use_rmsnorm_heads", False)):
-            raise NotImplementedError("FusedRTDHead supports the LayerNorm head (use_rmsnorm_heads=False)")
         self.dense = nn.Linear(hidden, hidden)
         self.act = nn.GELU()
         eps = float(getattr(config, "norm_eps", getattr(config, "layer_norm_eps", 1e-6)))
-        self.norm = nn.LayerNorm(hidden, eps=eps)
+        rms = bool(getattr(config, "use_rmsnorm_heads", False))
+        self.norm = FusedRMSNorm(hidden, eps=eps) if rms else nn.LayerNorm(hidden, eps=eps)
         self.classifier = nn.Linear(hidden, 1)
 
     @staticmethod
@@ -560,10 +565,14 @@ class FusedRTDHead(nn.Module):
         res = None
         if self._use_global_cls_context(attention_mask):
             res = hidden_states[:, 0:1, :].expand(hidden_states.shape)
-        if not _on_gpu(hidden_states):  # the reference's head in torch operations
+        if isinstance(self.norm, FusedRMSNorm):
+            x, _ = fused_add_rms_norm(hidden_states, self.norm.weight, self.norm.eps, res=res)
+        elif _on_gpu(hidden_states):
+            x = fused_add_layer_norm(hidden_states, None, res, self.norm)
+        else:
             x = self.norm(hidden_states + res if res is not None else hidden_states)
+        if not _on_gpu(x):  # the reference's head in torch operations
             return self.act(self.dense(x))
-        x = fused_add_layer_norm(hidden_states, None, res, self.norm)
         x = F.linear(x, self.dense.weight)
         bias = self.dense.bias
         if bias is not None:

@@ -41,6 +41,28 @@ DSA_EXTERN(bf16, 32)
 DSA_EXTERN(float, 64)
 DSA_EXTERN(float, 32)
 #undef DSA_EXTERN
+
+int reduce_cols(const float* part, int64_t nparts, int64_t stride, int K, int nout, const int64_t* off, void* const* out,
+                int dt, hipStream_t st) {
+  dsa::rows::ReduceCols rc;
+  rc.part = part;
+  rc.nparts = nparts;
+  rc.stride = stride;
+  rc.K = K;
+  rc.nout = nout;
+  for (int j = 0; j < 3; ++j) {
+    rc.off[j] = j < nout ? off[j] : 0;
+    rc.out[j] = j < nout ? out[j] : nullptr;
+  }
+  rc.dt = dt;
+  hipLaunchKernelGGL(dsa::rows::reduce_cols_kernel, dim3((unsigned)cdiv(K, 64), (unsigned)nout), dim3(64 * dsa::rows::RED_W), 0,
+                     st, rc);
+  return launch_check("reduce_cols_kernel");
+}
+
+// dsa_hidden.hip
+size_t drop_workspace(int64_t N, int C);
+size_t rms_workspace(int64_t N, int C);
 }  // namespace host
 }  // namespace dsa
 
@@ -153,21 +175,6 @@ void* static_scratch_locked(StaticState& s) {
   return s.done ? s.addr : nullptr;
 }
 
-// Refuses a stream that is being captured into a HIP graph: capturing the
-// library's launches ended in a host fault inside the runtime's capture end
-// whose cause is not known, so the library does not run under capture.
-int refuse_capture(hipStream_t st, const char* what) {
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(st, &cs) != hipSuccess) {
-    (void)hipGetLastError();
-    return 0;
-  }
-  if (cs != hipStreamCaptureStatusNone)
-    return fail("%s: the stream is capturing a HIP graph; the library's launches are not supported under graph capture",
-                what);
-  return 0;
-}
-
 // Bytes of the forward's k-step copy of one relative table (TableKs).
 size_t table_ks_bytes(const dsa_fwd_args* a) {
   return align_up((size_t)a->H * (2 * a->att_span) * a->D * elem_bytes(a->dtype), 256);
@@ -268,8 +275,6 @@ int run_fwd(const dsa_fwd_args* a, int* order_buf, void* tab_buf, uint32_t* drop
 }
 
 // ---- fused row kernels (include/dsa_block.h) ------------------------------------------------
-bool dtype_ok(int dt) { return dt == DSA_F32 || dt == DSA_BF16; }
-
 // a tensor read or written in 4-element vectors along rows: base aligned to
 // four elements, row stride a multiple of four
 bool rows_ok(const void* p, int64_t stride, int dt) {
@@ -277,26 +282,6 @@ bool rows_ok(const void* p, int64_t stride, int dt) {
   return p && (reinterpret_cast<uintptr_t>(p) % a) == 0 && stride % 4 == 0;
 }
 bool vec_ok(const void* p, int dt) { return !p || (reinterpret_cast<uintptr_t>(p) % (4u * (uintptr_t)elem_bytes(dt))) == 0; }
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-int reduce_cols(const float* part, int64_t nparts, int64_t stride, int K, int nout, const int64_t* off, void* const* out,
-                int dt, hipStream_t st) {
-  dsa::rows::ReduceCols rc;
-  rc.part = part;
-  rc.nparts = nparts;
-  rc.stride = stride;
-  rc.K = K;
-  rc.nout = nout;
-  for (int j = 0; j < 3; ++j) {
-    rc.off[j] = j < nout ? off[j] : 0;
-    rc.out[j] = j < nout ? out[j] : nullptr;
-  }
-  rc.dt = dt;
-  hipLaunchKernelGGL(dsa::rows::reduce_cols_kernel, dim3((unsigned)cdiv(K, 64), (unsigned)nout), dim3(64 * dsa::rows::RED_W), 0,
-                     st, rc);
-  return launch_check("reduce_cols_kernel");
-}
 
 int check_ln(const dsa_ln_args* a, bool bwd) {
   if (!a) return fail("dsa: null arguments");
@@ -441,7 +426,7 @@ dsa::rows::RtdParams rtd_params(const dsa_rtd_args* a) {
 
 extern "C" {
 
-int dsa_version(void) { return 13; }
+int dsa_version(void) { return 14; }
 
 const char* dsa_last_error(void) { return g_err.c_str(); }
 
@@ -688,6 +673,8 @@ size_t dsa_block_workspace_bytes(int kind, int64_t N, int32_t C) {
       const int64_t nb = cdiv(N, dsa::rows::RTD_RB);
       return align_up((size_t)nb * (size_t)std::max<int64_t>(2, C + 1) * sizeof(float), 256);
     }
+    case DSA_BLOCK_DROPOUT: return N < (1LL << 31) ? drop_workspace(N, C) : 0;
+    case DSA_BLOCK_RMS: return N < (1LL << 31) ? rms_workspace(N, C) : 0;
     default: return 0;
   }
 }

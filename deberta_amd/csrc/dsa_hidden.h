@@ -1,0 +1,145 @@
+// dsa_hidden.h — what the operators on hidden states share (gfx950): rows of
+// any width, stride and element alignment in chunks of eight columns, the
+// keep bits of hidden dropout and sums over a wave.  The operators
+// (dsa_drop.h, dsa_rms.h, dsa_embed.h) are bound by HBM traffic.
+//
+// A lane holds chunks of eight consecutive columns: one 16-byte access for
+// bf16, two for fp32, and one Philox call for dropout.  The accesses are
+// declared with the alignment of one element: gfx950's global memory
+// instructions take any address, so an odd width or an odd first column
+// needs no kernel of its own.  A row's last chunk may hold fewer than eight
+// columns.  It is still read in one access where the eight elements lie
+// inside the tensor (they are then the next row's), element by element
+// where they do not (the last row), and what lies past the row is zeroed
+// in registers.  It is written element by element.
+#pragma once
+
+#include "dsa_common.h"
+#include "dsa_dropout.h"
+
+namespace dsa {
+namespace hid {
+
+constexpr int kBF16 = 1;  // DSA_BF16 (DSA_F32 = 0)
+
+template <typename T>
+struct Raw8 {
+  typedef T v8 __attribute__((ext_vector_type(8)));
+  typedef v8 v8u __attribute__((aligned(sizeof(T))));
+};
+template <typename T>
+using raw8 = typename Raw8<T>::v8;
+
+// Elements off .. off + 7 of a tensor that ends at element `extent`; the
+// lane's n <= 0 columns load nothing.
+template <typename T>
+DSA_DEV raw8<T> ld8(const void* base, int64_t off, int64_t extent, int n) {
+  raw8<T> r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)0.f;
+  if (n > 0) {
+    const T* p = static_cast<const T*>(base) + off;
+    if (off + 8 <= extent) {
+      r = *reinterpret_cast<const typename Raw8<T>::v8u*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < n) r[e] = p[e];
+    }
+  }
+  return r;
+}
+
+// the n first values as fp32, zero behind them
+template <typename T>
+DSA_DEV void cvt8(const raw8<T>& r, int n, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)r[e];
+  if (n < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+  }
+}
+
+template <typename T>
+DSA_DEV void st8(void* base, int64_t off, int n, const float (&v)[8]) {
+  if (n <= 0) return;
+  T* p = static_cast<T*>(base) + off;
+  raw8<T> r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
+  if (n >= 8) {
+    *reinterpret_cast<typename Raw8<T>::v8u*>(p) = r;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = r[e];
+  }
+}
+
+// A parameter vector's chunk, its type known at run time (read once a block
+// or from the caches).
+DSA_DEV void ld_param8(const void* p, int dt, int c, int n, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (!p || n <= 0) return;
+  if (dt == kBF16) cvt8<bf16>(ld8<bf16>(p, c, (int64_t)c + n, n), n, v);
+  else cvt8<float>(ld8<float>(p, c, (int64_t)c + n, n), n, v);
+}
+
+// element offset of the residual's row r
+DSA_DEV int64_t res_row(uint32_t r, uint32_t rpg, uint32_t N, int64_t rs0, int64_t rs1) {
+  if (rpg >= N) return (int64_t)r * rs1;
+  const uint32_t g = r / rpg;
+  return (int64_t)g * rs0 + (int64_t)(r - g * rpg) * rs1;
+}
+
+// Hidden dropout's keep bits.  The value at row r (all leading dimensions
+// flattened) and column c of a call with threshold t is kept where
+//   x = Philox4x32-10(counter = (c / 8, r & 0xffffffff, r >> 32, kHiddenDomain),
+//                     key = (seed & 0xffffffff, seed >> 32))
+//   u = c % 8;  (x[u / 2] >> (16 * (u % 2))) & 0xffff >= t
+// so it depends on the position and the seed alone, not on strides, types or
+// the launch, and the backward draws the same bits again: nothing is stored.
+// A value is dropped with probability t / 65536 exactly.  Sixteen bits a
+// value make one call serve a lane's chunk: about 20 32-bit products and 60
+// other operations for eight values, which a bf16 stream hides behind its
+// 32 bytes of traffic; with 32 bits a value they would not hide.
+constexpr uint32_t kHiddenDomain = 0x68696464u;  // the attention's counters end in the batch row
+
+struct Drop {
+  uint32_t t;       // 0: no dropout; 65536: everything dropped
+  uint32_t k0, k1;  // the seed's low and high words
+  float scale;      // 65536 / (65536 - t); 0 where everything is dropped
+};
+
+DSA_DEV uint32_t hidden_keep8(const Drop& d, int64_t row, int chunk) {
+  return keep8(philox4x32_10((uint32_t)chunk, (uint32_t)row, (uint32_t)((uint64_t)row >> 32), kHiddenDomain, d.k0, d.k1), d.t);
+}
+
+// A dropped value is 0 whatever it was (NaN and infinities included).
+DSA_DEV void apply_keep(uint32_t bits, float scale, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (bits >> e) & 1 ? v[e] * scale : 0.f;
+}
+
+// One data-parallel step of a sum over the lanes of a row of 16 (the
+// instruction's own lane patterns: no trip through LDS).
+template <int CTRL>
+DSA_DEV float dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+DSA_DEV float lane_value(float x, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+// The sum of x over the wave, in a fixed order, in every lane.
+DSA_DEV float wave_sum(float x) {
+  x += dpp<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x += dpp<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x += dpp<0x141>(x);  // row_half_mirror: the other quad of eight lanes
+  x += dpp<0x140>(x);  // row_mirror: the other eight of sixteen
+  return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+}
+
+}  // namespace hid
+}  // namespace dsa

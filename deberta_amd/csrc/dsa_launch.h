@@ -26,32 +26,11 @@
 #include "dsa_bwd_table.h"
 #include "dsa_dropout.h"
 #include "dsa_fwd.h"
+#include "dsa_host.h"
 #include "dsa_order.h"
 
 namespace dsa {
 namespace host {
-
-// description of the calling thread's last error (dsa_last_error)
-inline thread_local std::string g_err;
-
-static int fail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
-static int fail(const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return 1;
-}
-
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-static size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-static int round_up(int x, int a) { return (x + a - 1) / a * a; }
-
-static int elem_bytes(int dtype) { return dtype == DSA_BF16 ? 2 : 4; }
 
 // Whether the call's kernels look for far blocks (FarSpan): where at least
 // `need` percent of its blocks lie past the saturation.  A far block saves its
@@ -167,12 +146,6 @@ static int pair_blocks(const dsa::PairBits& t) { return (int)((dsa::pair_tiles(t
 
 static int mask_mode(const dsa_fwd_args* a) {
   return a->pair_keep ? dsa::MASK_PAIR : a->key_keep ? dsa::MASK_KEY : a->seg ? dsa::MASK_SEG : dsa::MASK_NONE;
-}
-
-static int launch_check(const char* what) {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail("dsa: %s launch failed: %s", what, hipGetErrorString(e));
-  return 0;
 }
 
 // Heaviest-first order (dsa_order.h) of B * ntiles items: cost and order
