@@ -30,13 +30,13 @@ struct DropRows {
   Drop d;
 };
 
-template <typename TX, typename TR, typename TY>
+template <typename TX, typename TR, typename TY, bool TAIL>
 __global__ __launch_bounds__(DROP_T) void drop_fwd_kernel(DropRows p) {
   const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * DROP_T + (int)threadIdx.x - sub * p.cw;
   const int c = 8 * chunk, n = p.C - c;
-  if (sub >= p.subs || n <= 0) return;
+  if (sub >= p.subs || n <= 0) return;  // all others: eight columns, or the row's last
   float bias[8];
-  ld_param8(p.bias, p.bias_dt, c, n, bias);
+  ld_param8<TAIL>(p.bias, p.bias_dt, c, n, bias);
   const int64_t r0 = (int64_t)blockIdx.x * p.rows * p.subs + sub;
   for (int i = 0; i < p.rows; i += DROP_U) {
     raw8<TX> x[DROP_U];
@@ -44,32 +44,37 @@ __global__ __launch_bounds__(DROP_T) void drop_fwd_kernel(DropRows p) {
 #pragma unroll
     for (int u = 0; u < DROP_U; ++u) {
       const uint32_t r = (uint32_t)min(r0 + (int64_t)(i + u) * p.subs, (int64_t)p.N - 1);
-      x[u] = ld8<TX>(p.x, (int64_t)r * p.xs + c, p.xe, n);
-      if (p.res) res[u] = ld8<TR>(p.res, res_row(r, p.rpg, p.N, p.rs0, p.rs1) + c, p.re, n);
+      x[u] = ld8<TX, TAIL>(p.x, (int64_t)r * p.xs + c, p.xe, n);
+      if (p.res) res[u] = ld8<TR, TAIL>(p.res, res_row(r, p.rpg, p.N, p.rs0, p.rs1) + c, p.re, n);
+    }
+    uint4 words[DROP_U];
+    if (p.d.on) {
+#pragma unroll
+      for (int u = 0; u < DROP_U; ++u) words[u] = hidden_words(p.d, r0 + (int64_t)(i + u) * p.subs, chunk);
     }
 #pragma unroll
     for (int u = 0; u < DROP_U; ++u) {
       const int64_t r = r0 + (int64_t)(i + u) * p.subs;
       if (r >= p.N) return;
       float v[8];
-      cvt8<TX>(x[u], 8, v);
+      cvt8<TX, TAIL>(x[u], 8, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += bias[e];
-      if (p.d.t) apply_keep(hidden_keep8(p.d, r, chunk), p.d.scale, v);
+      if (p.d.on) drop8(p.d, words[u], v);
       if (p.res) {
         float w[8];
-        cvt8<TR>(res[u], 8, w);
+        cvt8<TR, TAIL>(res[u], 8, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += w[e];
       }
-      st8<TY>(p.y, r * p.ys + c, n, v);
+      st8<TY, TAIL>(p.y, r * p.ys + c, n, v);
     }
   }
 }
 
 // dx and, where part is given, the block's column sums of it: the sums of a
 // thread's rows, then of the block's row groups in their order.
-template <typename TDY, typename TX>
+template <typename TDY, typename TX, bool TAIL>
 __global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
   __shared__ float red[DROP_T * 8];
   const int sub = threadIdx.x / p.cw, in_row = (int)threadIdx.x - sub * p.cw, chunk = blockIdx.y * DROP_T + in_row;
@@ -82,16 +87,21 @@ __global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
 #pragma unroll
       for (int u = 0; u < DROP_U; ++u) {
         const int64_t r = min(r0 + (int64_t)(i + u) * p.subs, (int64_t)p.N - 1);
-        dy[u] = ld8<TDY>(p.dy, r * p.dys + c, p.dye, n);
+        dy[u] = ld8<TDY, TAIL>(p.dy, r * p.dys + c, p.dye, n);
+      }
+      uint4 words[DROP_U];
+      if (p.d.on) {
+#pragma unroll
+        for (int u = 0; u < DROP_U; ++u) words[u] = hidden_words(p.d, r0 + (int64_t)(i + u) * p.subs, chunk);
       }
 #pragma unroll
       for (int u = 0; u < DROP_U; ++u) {
         const int64_t r = r0 + (int64_t)(i + u) * p.subs;
-        if (r < p.N && i + u < p.rows) {
+        if (r < p.N) {
           float v[8];
-          cvt8<TDY>(dy[u], n, v);
-          if (p.d.t) apply_keep(hidden_keep8(p.d, r, chunk), p.d.scale, v);
-          if (p.dx) st8<TX>(p.dx, r * p.dxs + c, n, v);
+          cvt8<TDY, TAIL>(dy[u], n, v);
+          if (p.d.on) drop8(p.d, words[u], v);
+          if (p.dx) st8<TX, TAIL>(p.dx, r * p.dxs + c, n, v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum[e] += v[e];
         }

@@ -50,7 +50,7 @@ DSA_DEV int64_t ld_id(const void* ids, int64_t i, int ids64) {
 
 // Threads as in drop_fwd_kernel.  An id outside [0, V) reads nothing and
 // gives a row of NaN.
-template <typename TW, typename TY>
+template <typename TW, typename TY, bool TAIL>
 __global__ __launch_bounds__(EMB_T) void embed_fwd_kernel(EmbedRows p) {
   const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * EMB_T + (int)threadIdx.x - sub * p.cw;
   const int c = 8 * chunk, n = p.C - c;
@@ -66,18 +66,18 @@ __global__ __launch_bounds__(EMB_T) void embed_fwd_kernel(EmbedRows p) {
 #pragma unroll
     for (int u = 0; u < EMB_U; ++u) {
       const bool ok = (uint64_t)id[u] < (uint64_t)p.V;
-      w[u] = ld8<TW>(p.w, ok ? id[u] * p.ws + c : c, extent, ok ? n : 0);
+      w[u] = ld8<TW, TAIL>(p.w, ok ? id[u] * p.ws + c : c, extent, ok ? n : 0);
     }
 #pragma unroll
     for (int u = 0; u < EMB_U; ++u) {
       const int64_t r = r0 + (int64_t)(i + u) * p.subs;
       if (r >= p.N) return;
       float v[8];
-      cvt8<TW>(w[u], 8, v);
+      cvt8<TW, TAIL>(w[u], 8, v);
       const float s = (uint64_t)id[u] < (uint64_t)p.V ? p.scale : __builtin_nanf("");
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= s;
-      st8<TY>(p.y, r * p.ys + c, n, v);
+      st8<TY, TAIL>(p.y, r * p.ys + c, n, v);
     }
   }
 }
@@ -314,7 +314,7 @@ struct EmbedSums {
   float scale;
 };
 
-template <typename TDY, typename TW>
+template <typename TDY, typename TW, bool TAIL>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSums p) {
   const int lane = threadIdx.x & 63;
   const uint32_t item = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -337,25 +337,25 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSums p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t r = (uint32_t)__builtin_amdgcn_readlane(pos, min(j0 + u, m - 1));
-      dy[u] = ld8<TDY>(p.dy, (int64_t)r * p.dys + c, p.dye, n);
+      dy[u] = ld8<TDY, TAIL>(p.dy, (int64_t)r * p.dys + c, p.dye, n);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u;
       if (j < m) {
         float v[8];
-        cvt8<TDY>(dy[u], n, v);
+        cvt8<TDY, TAIL>(dy[u], n, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += v[e];
         const bool end = (ends >> j) & 1;
         if (end || j == m - 1) {
           if (carried || !end) {
             float* out = p.part + ((int64_t)ch * 2 + (carried ? 0 : 1)) * p.C;
-            st8<float>(out, c, n, acc);
+            st8<float, TAIL>(out, c, n, acc);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = acc[e] * p.scale;
-            st8<TW>(p.dw, (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j) * p.dws + c, n, v);
+            st8<TW, TAIL>(p.dw, (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j) * p.dws + c, n, v);
           }
           carried = false;
 #pragma unroll
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSums p) {
 
 // Block (chunk, slab): the token that begins in the chunk and goes on past
 // its end, from the chunk's own partial sum and those of the chunks behind.
-template <typename TW>
+template <typename TW, bool TAIL>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedSums p) {
   __shared__ float red[3][64][8];
   const int lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -390,12 +390,12 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedSums p) {
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int64_t extent = (int64_t)p.chunks * 2 * p.C;
   constexpr int U = 4;
-  if (q == 0) cvt8<float>(ld8<float>(p.part, ((int64_t)ch * 2 + 1) * p.C + c, extent, n), n, acc);
+  if (q == 0) cvt8<float, TAIL>(ld8<float, TAIL>(p.part, ((int64_t)ch * 2 + 1) * p.C + c, extent, n), n, acc);
   for (int64_t k0 = (int64_t)ch + 1 + q; k0 <= last; k0 += 4 * U) {
     raw8<float> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      v[u] = ld8<float>(p.part, min(k0 + 4 * u, (int64_t)last) * 2 * p.C + c, extent, n);
+      v[u] = ld8<float, TAIL>(p.part, min(k0 + 4 * u, (int64_t)last) * 2 * p.C + c, extent, n);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (k0 + 4 * u <= last) {
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedSums p) {
     for (int e = 0; e < 8; ++e) acc[e] += red[v][lane][e];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
-  st8<TW>(p.dw, (int64_t)key * p.dws + c, n, acc);
+  st8<TW, TAIL>(p.dw, (int64_t)key * p.dws + c, n, acc);
 }
 
 }  // namespace hid

@@ -6,12 +6,14 @@
 // A lane holds chunks of eight consecutive columns: one 16-byte access for
 // bf16, two for fp32, and one Philox call for dropout.  The accesses are
 // declared with the alignment of one element: gfx950's global memory
-// instructions take any address, so an odd width or an odd first column
-// needs no kernel of its own.  A row's last chunk may hold fewer than eight
-// columns.  It is still read in one access where the eight elements lie
-// inside the tensor (they are then the next row's), element by element
-// where they do not (the last row), and what lies past the row is zeroed
-// in registers.  It is written element by element.
+// instructions take any address, so an odd row stride or first column needs
+// no kernel of its own.  An odd width does (TAIL: C is no multiple of
+// eight): its rows end in a chunk of fewer columns, which is read in one
+// access where the eight elements lie inside the tensor (they are then the
+// next row's), element by element where they do not (the last row), zeroed
+// in registers past the row, and written element by element.  In one kernel
+// for both the lanes' conditions would take more scalar registers than
+// there are: their spills were a third of the RMS backward's instructions.
 #pragma once
 
 #include "dsa_common.h"
@@ -30,45 +32,43 @@ struct Raw8 {
 template <typename T>
 using raw8 = typename Raw8<T>::v8;
 
-// Elements off .. off + 7 of a tensor that ends at element `extent`; the
-// lane's n <= 0 columns load nothing.
-template <typename T>
+// The lane's n columns from element off of a tensor that ends at element
+// `extent` (n <= 0: nothing, zeros; without TAIL n >= 8 otherwise).
+template <typename T, bool TAIL>
 DSA_DEV raw8<T> ld8(const void* base, int64_t off, int64_t extent, int n) {
   raw8<T> r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = (T)0.f;
-  if (n > 0) {
-    const T* p = static_cast<const T*>(base) + off;
-    if (off + 8 <= extent) {
-      r = *reinterpret_cast<const typename Raw8<T>::v8u*>(p);
-    } else {
+  const T* p = static_cast<const T*>(base) + off;
+  if (TAIL ? n >= 8 || (n > 0 && off + 8 <= extent) : n > 0) {
+    r = *reinterpret_cast<const typename Raw8<T>::v8u*>(p);
+  } else if (TAIL && n > 0) {
 #pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (e < n) r[e] = p[e];
-    }
+    for (int e = 0; e < 7; ++e)
+      if (e < n) r[e] = p[e];
   }
   return r;
 }
 
-// the n first values as fp32, zero behind them
-template <typename T>
+// the n first values as fp32, zero behind them (what ld8 gave for n <= 0 is zero)
+template <typename T, bool TAIL>
 DSA_DEV void cvt8(const raw8<T>& r, int n, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (float)r[e];
-  if (n < 8) {
+  if (TAIL && n > 0 && n < 8) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+    for (int e = 1; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
   }
 }
 
-template <typename T>
+template <typename T, bool TAIL>
 DSA_DEV void st8(void* base, int64_t off, int n, const float (&v)[8]) {
   if (n <= 0) return;
   T* p = static_cast<T*>(base) + off;
   raw8<T> r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
-  if (n >= 8) {
+  if (!TAIL || n >= 8) {
     *reinterpret_cast<typename Raw8<T>::v8u*>(p) = r;
   } else {
 #pragma unroll
@@ -79,12 +79,13 @@ DSA_DEV void st8(void* base, int64_t off, int n, const float (&v)[8]) {
 
 // A parameter vector's chunk, its type known at run time (read once a block
 // or from the caches).
+template <bool TAIL>
 DSA_DEV void ld_param8(const void* p, int dt, int c, int n, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
   if (!p || n <= 0) return;
-  if (dt == kBF16) cvt8<bf16>(ld8<bf16>(p, c, (int64_t)c + n, n), n, v);
-  else cvt8<float>(ld8<float>(p, c, (int64_t)c + n, n), n, v);
+  if (dt == kBF16) cvt8<bf16, TAIL>(ld8<bf16, TAIL>(p, c, (int64_t)c + n, n), n, v);
+  else cvt8<float, TAIL>(ld8<float, TAIL>(p, c, (int64_t)c + n, n), n, v);
 }
 
 // element offset of the residual's row r
@@ -108,19 +109,28 @@ DSA_DEV int64_t res_row(uint32_t r, uint32_t rpg, uint32_t N, int64_t rs0, int64
 constexpr uint32_t kHiddenDomain = 0x68696464u;  // the attention's counters end in the batch row
 
 struct Drop {
-  uint32_t t;       // 0: no dropout; 65536: everything dropped
+  uint32_t on;      // 0: no dropout
+  uint32_t lim;     // (t << 16) - 1: a value is kept where its 16 bits, shifted up, are above
+                    // (t = 65536: none is)
   uint32_t k0, k1;  // the seed's low and high words
   float scale;      // 65536 / (65536 - t); 0 where everything is dropped
 };
 
-DSA_DEV uint32_t hidden_keep8(const Drop& d, int64_t row, int chunk) {
-  return keep8(philox4x32_10((uint32_t)chunk, (uint32_t)row, (uint32_t)((uint64_t)row >> 32), kHiddenDomain, d.k0, d.k1), d.t);
+// the random words of a chunk
+DSA_DEV uint4 hidden_words(const Drop& d, int64_t row, int chunk) {
+  return philox4x32_10((uint32_t)chunk, (uint32_t)row, (uint32_t)((uint64_t)row >> 32), kHiddenDomain, d.k0, d.k1);
 }
 
-// A dropped value is 0 whatever it was (NaN and infinities included).
-DSA_DEV void apply_keep(uint32_t bits, float scale, float (&v)[8]) {
+// A dropped value is 0 whatever it was (NaN and infinities included).  The
+// words are kept rather than a mask of bits: a compare a value either way,
+// and no bit to set and test.
+DSA_DEV void drop8(const Drop& d, uint4 x, float (&v)[8]) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (bits >> e) & 1 ? v[e] * scale : 0.f;
+  for (int u = 0; u < 4; ++u) {
+    v[2 * u] = (w[u] << 16) > d.lim ? v[2 * u] * d.scale : 0.f;
+    v[2 * u + 1] = w[u] > d.lim ? v[2 * u + 1] * d.scale : 0.f;
+  }
 }
 
 // One data-parallel step of a sum over the lanes of a row of 16 (the

@@ -69,7 +69,8 @@ int64_t res_extent(const int64_t* strides, int64_t per_group, int64_t N, int C) 
 // Keep bits of a call: threshold in [0, 65536].
 hid::Drop drop_params(uint32_t t, uint64_t seed) {
   hid::Drop d;
-  d.t = t;
+  d.on = t != 0;
+  d.lim = (uint32_t)((uint64_t)t << 16) - 1u;
   d.k0 = (uint32_t)seed;
   d.k1 = (uint32_t)(seed >> 32);
   d.scale = t < 65536u ? (float)(65536.0 / (65536.0 - (double)t)) : 0.f;
@@ -133,9 +134,9 @@ int check_dropout(const dsa_dropout_args* a, bool bwd) {
 
 // ---- RMS norm ---------------------------------------------------------------
 
-// rows a team takes in the backward, so that at most 1024 blocks leave
-// partial sums
-int rms_sum_rows(int64_t N, int C) { return (int)cdiv(N, (int64_t)1024 * rms_teams_of(C)); }
+// rows a team takes in the backward, so that at most 512 blocks leave partial
+// sums
+int rms_sum_rows(int64_t N, int C) { return (int)cdiv(N, (int64_t)512 * rms_teams_of(C)); }
 int64_t rms_sum_blocks(int64_t N, int C) { return cdiv(N, (int64_t)rms_sum_rows(N, C) * rms_teams_of(C)); }
 
 int check_rms(const dsa_rms_args* a, bool quant, bool bwd) {
@@ -306,8 +307,10 @@ int dsa_dropout_fwd(const dsa_dropout_args* a, void* stream) {
     by_type(a->res ? a->res_dtype : a->x_dtype, [&](auto tr) {
       typedef typename decltype(tx)::type TX;
       typedef typename decltype(tr)::type TR;
-      hipLaunchKernelGGL((hid::drop_fwd_kernel<TX, TR, stream_t<TX, TR>>), dim3((unsigned)nb, (unsigned)g.slabs),
-                         dim3((unsigned)g.threads), 0, st, p);
+      by_tail(a->C, [&](auto tail) {
+        hipLaunchKernelGGL((hid::drop_fwd_kernel<TX, TR, stream_t<TX, TR>, decltype(tail)::value>),
+                           dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
+      });
     });
   });
   return launch_check("drop_fwd_kernel");
@@ -331,8 +334,10 @@ int dsa_dropout_bwd(const dsa_dropout_args* a, void* stream) {
   if (!grid_ok(nb, g.slabs, g.threads)) return fail("dsa_dropout: too many rows or columns for one launch");
   by_type(a->dy_dtype, [&](auto tdy) {
     by_type(a->dx ? a->dx_dtype : a->dy_dtype, [&](auto tx) {
-      hipLaunchKernelGGL((hid::drop_bwd_kernel<typename decltype(tdy)::type, typename decltype(tx)::type>),
-                         dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
+      by_tail(a->C, [&](auto tail) {
+        hipLaunchKernelGGL((hid::drop_bwd_kernel<typename decltype(tdy)::type, typename decltype(tx)::type, decltype(tail)::value>),
+                           dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
+      });
     });
   });
   if (launch_check("drop_bwd_kernel")) return 1;
@@ -390,8 +395,10 @@ int dsa_embed_fwd(const dsa_embed_args* a, void* stream) {
   if (!grid_ok(nb, g.slabs, g.threads)) return fail("dsa_embed: too many rows or columns for one launch");
   by_type(a->weight_dtype, [&](auto tw) {
     by_type(a->y_dtype, [&](auto ty) {
-      hipLaunchKernelGGL((hid::embed_fwd_kernel<typename decltype(tw)::type, typename decltype(ty)::type>),
-                         dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
+      by_tail(a->C, [&](auto tail) {
+        hipLaunchKernelGGL((hid::embed_fwd_kernel<typename decltype(tw)::type, typename decltype(ty)::type, decltype(tail)::value>),
+                           dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
+      });
     });
   });
   return launch_check("embed_fwd_kernel");
@@ -457,15 +464,19 @@ int dsa_embed_bwd(const dsa_embed_args* a, void* stream) {
   p.C = a->C, p.slabs = e.slabs, p.K = e.K, p.scale = a->scale;
   by_type(a->dy_dtype, [&](auto tdy) {
     by_type(a->weight_dtype, [&](auto tw) {
-      hipLaunchKernelGGL((hid::embed_sum_kernel<typename decltype(tdy)::type, typename decltype(tw)::type>),
-                         dim3((unsigned)cdiv(e.chunks * e.slabs, 4)), dim3(256), 0, st, p);
+      by_tail(a->C, [&](auto tail) {
+        hipLaunchKernelGGL((hid::embed_sum_kernel<typename decltype(tdy)::type, typename decltype(tw)::type, decltype(tail)::value>),
+                           dim3((unsigned)cdiv(e.chunks * e.slabs, 4)), dim3(256), 0, st, p);
+      });
     });
   });
   if (launch_check("embed_sum_kernel")) return 1;
   if (e.chunks == 1) return 0;
   by_type(a->weight_dtype, [&](auto tw) {
-    hipLaunchKernelGGL((hid::embed_join_kernel<typename decltype(tw)::type>), dim3((unsigned)(e.chunks * e.slabs)), dim3(256), 0,
-                       st, p);
+    by_tail(a->C, [&](auto tail) {
+      hipLaunchKernelGGL((hid::embed_join_kernel<typename decltype(tw)::type, decltype(tail)::value>),
+                         dim3((unsigned)(e.chunks * e.slabs)), dim3(256), 0, st, p);
+    });
   });
   return launch_check("embed_join_kernel");
 }

@@ -35,6 +35,13 @@ struct RmsRows {
   Drop d;
 };
 
+// The columns of a lane's chunk k from column c on: only the last chunk may
+// lie past the row, or hold less than eight columns (TAIL).
+template <int NC, bool TAIL>
+DSA_DEV int rms_cols(int C, int c, int k) {
+  return k < NC - 1 ? 8 : TAIL ? C - c : c < C ? 8 : 0;
+}
+
 // rows a block takes at a time: one team of four waves or more, four teams of one
 template <int W>
 constexpr int rms_teams() { return W == 1 ? 4 : 1; }
@@ -58,40 +65,46 @@ DSA_DEV float team_sum(float x, float* buf, int wr, int& turn) {
   return x;
 }
 
-// z of the lane's chunks of row r, and their keep bits
-template <int NC, int W, typename TX, typename TR>
-DSA_DEV void rms_load_z(const RmsRows& p, uint32_t r, int first, float (&z)[NC][8], uint32_t (&keep)[NC]) {
+// The lane's chunks of a row of x and the residual as they lie in memory.
+template <int NC, int W, typename TX, typename TR, bool TAIL>
+struct RawZ {
   raw8<TX> x[NC];
   raw8<TR> res[NC];
-  const int64_t xo = (int64_t)r * p.xs;
-  const int64_t ro = p.res ? res_row(r, p.rpg, p.N, p.rs0, p.rs1) : 0;
+  DSA_DEV void load(const RmsRows& p, uint32_t r, int first) {
+    const int64_t xo = (int64_t)r * p.xs;
+    const int64_t ro = p.res ? res_row(r, p.rpg, p.N, p.rs0, p.rs1) : 0;
 #pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int c = 8 * (first + 64 * W * k);
-    x[k] = ld8<TX>(p.x, xo + c, p.xe, p.C - c);
-    if (p.res) res[k] = ld8<TR>(p.res, ro + c, p.re, p.C - c);
-  }
-  if (p.d.t) {
-#pragma unroll
-    for (int k = 0; k < NC; ++k) keep[k] = hidden_keep8(p.d, r, first + 64 * W * k);
-  }
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int c = 8 * (first + 64 * W * k), n = p.C - c;
-    cvt8<TX>(x[k], n, z[k]);
-    if (p.bias) {
-      float b[8];
-      ld_param8(p.bias, p.bias_dt, c, n, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[k][e] += b[e];
+    for (int k = 0; k < NC; ++k) {
+      const int c = 8 * (first + 64 * W * k);
+      x[k] = ld8<TX, TAIL>(p.x, xo + c, p.xe, rms_cols<NC, TAIL>(p.C, c, k));
+      if (p.res) res[k] = ld8<TR, TAIL>(p.res, ro + c, p.re, rms_cols<NC, TAIL>(p.C, c, k));
     }
-    if (p.d.t) apply_keep(keep[k], p.d.scale, z[k]);
-    if (p.res) {
-      float v[8];
-      cvt8<TR>(res[k], n, v);
+  }
+};
+
+// The random words of the lane's chunks of row r.
+template <int NC, int W>
+DSA_DEV void rms_words(const RmsRows& p, uint32_t r, int first, uint4 (&words)[NC]) {
+  if (!p.d.on) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[k][e] += v[e];
-    }
+  for (int k = 0; k < NC; ++k) words[k] = hidden_words(p.d, r, first + 64 * W * k);
+}
+
+// chunk k of z = dropout(x + bias) + res
+template <int NC, int W, typename TX, typename TR, bool TAIL>
+DSA_DEV void rms_z(const RmsRows& p, const RawZ<NC, W, TX, TR, TAIL>& raw, int k, int n, const float (&bias)[8], uint4 words,
+                   float (&z)[8]) {
+  cvt8<TX, TAIL>(raw.x[k], n, z);
+  if (p.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += bias[e];
+  }
+  if (p.d.on) drop8(p.d, words, z);
+  if (p.res) {
+    float v[8];
+    cvt8<TR, TAIL>(raw.res[k], n, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += v[e];
   }
 }
 
@@ -99,21 +112,28 @@ DSA_DEV void rms_load_z(const RmsRows& p, uint32_t r, int first, float (&z)[NC][
 // infinity is above every finite value and a NaN above both.
 DSA_DEV uint32_t mag(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-template <int NC, int W, typename TX, typename TR, typename TZ, typename TY>
+template <int NC, int W, typename TX, typename TR, typename TZ, typename TY, bool TAIL>
 __global__ __launch_bounds__(rms_threads<W>()) void rms_fwd_kernel(RmsRows p) {
   __shared__ float buf[2 * W];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wv % W, first = wr * 64 + lane;
   const uint32_t r = blockIdx.x * rms_teams<W>() + wv / W;
   if (r >= p.N) return;  // the whole team; a block has barriers only where it is one team
+  RawZ<NC, W, TX, TR, TAIL> raw;
+  raw.load(p, r, first);
+  uint4 words[NC];
+  rms_words<NC, W>(p, r, first, words);  // while the loads are in flight
   float z[NC][8];
-  uint32_t keep[NC];
-  rms_load_z<NC, W, TX, TR>(p, r, first, z, keep);
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < NC; ++k)
+  for (int k = 0; k < NC; ++k) {
+    const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
+    float bias[8];
+    ld_param8<TAIL>(p.bias, p.bias_dt, c, n, bias);
+    rms_z<NC, W, TX, TR, TAIL>(p, raw, k, n, bias, words[k], z[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += z[k][e] * z[k][e];
+  }
   int turn = 0;
   const float rstd = 1.f / sqrtf(team_sum<W>(s, buf, wr, turn) / (float)p.C + p.eps);
   if (p.rstd && wr == 0 && lane == 0) p.rstd[r] = rstd;
@@ -121,17 +141,17 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_fwd_kernel(RmsRows p) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int c = 8 * (first + 64 * W * k);
-      st8<TZ>(p.z, (int64_t)r * p.zs + c, p.C - c, z[k]);
+      st8<TZ, TAIL>(p.z, (int64_t)r * p.zs + c, rms_cols<NC, TAIL>(p.C, c, k), z[k]);
     }
   }
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
-    const int c = 8 * (first + 64 * W * k), n = p.C - c;
+    const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
     float w[8];
-    ld_param8(p.w, p.w_dt, c, n, w);
+    ld_param8<TAIL>(p.w, p.w_dt, c, n, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[k][e] = z[k][e] * rstd * w[e];
-    if constexpr (!std::is_same<TY, fp8>::value) st8<TY>(p.y, (int64_t)r * p.ys + c, n, z[k]);
+    if constexpr (!std::is_same<TY, fp8>::value) st8<TY, TAIL>(p.y, (int64_t)r * p.ys + c, n, z[k]);
   }
   if constexpr (std::is_same<TY, fp8>::value) {
     __shared__ uint32_t mbuf[W];
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_fwd_kernel(RmsRows p) {
     }
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int c = 8 * (first + 64 * W * k), n = p.C - c;
+      const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
       if (n <= 0) continue;
       const float a = __builtin_bit_cast(float, m[k]);
       // every value below the smallest normal scale's range: zeros
@@ -201,68 +221,99 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_fwd_kernel(RmsRows p) {
   }
 }
 
+// What the backward reads of a row.
+template <int NC, int W, typename TX, typename TR, typename TZ, typename TDY, bool TAIL>
+struct RawBwd {
+  RawZ<NC, W, TX, TR, TAIL> z;
+  raw8<TDY> dy[NC];
+  raw8<TZ> u[NC];
+  float rstd;
+  DSA_DEV void load(const RmsRows& p, uint32_t r, int first) {
+    z.load(p, r, first);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = 8 * (first + 64 * W * k);
+      dy[k] = ld8<TDY, TAIL>(p.dy, (int64_t)r * p.dys + c, p.dye, rms_cols<NC, TAIL>(p.C, c, k));
+      if (p.dzu) u[k] = ld8<TZ, TAIL>(p.dzu, (int64_t)r * p.dzus + c, p.dzue, rms_cols<NC, TAIL>(p.C, c, k));
+    }
+    rstd = p.rstd[r];
+  }
+};
+
 // Rows [rows * team, + rows), team counted over the grid.  dw's and dbias's
 // partial sums of the block go to part[block][1 or 2][C].
-template <int NC, int W, typename TX, typename TR, typename TZ, typename TDY>
+//
+// A block stays for many rows (the launch holds as many blocks as run at
+// once), so that the partial sums are few.  A row's own latency is then
+// what bounds it: the next row is loaded while the row is worked on, where
+// its registers allow (PRE), and w and the bias stay in registers (KEEP).
+template <int NC, int W, typename TX, typename TR, typename TZ, typename TDY, bool TAIL>
 __global__ __launch_bounds__(rms_threads<W>()) void rms_bwd_kernel(RmsRows p) {
+  typedef RawBwd<NC, W, TX, TR, TZ, TDY, TAIL> Raw;
+  constexpr bool KEEP = W < 16;  // sixteen waves have 128 registers each
+  constexpr bool PRE = KEEP && sizeof(Raw) <= 4 * 44;
   __shared__ float buf[2 * W];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wv % W, first = wr * 64 + lane;
   const int64_t r0 = ((int64_t)blockIdx.x * rms_teams<W>() + wv / W) * p.rows;
-  float sw[NC][8], sb[NC][8];
+  const int64_t left = (int64_t)p.N - r0;
+  const int rows = (int)(left < p.rows ? left : p.rows);  // of this team; none: at most 0
+  float sw[NC][8], sb[NC][8], w[NC][8], bias[NC][8];
 #pragma unroll
-  for (int k = 0; k < NC; ++k)
+  for (int k = 0; k < NC; ++k) {
+    const int c = 8 * (first + 64 * W * k);
+    if (KEEP) ld_param8<TAIL>(p.w, p.w_dt, c, rms_cols<NC, TAIL>(p.C, c, k), w[k]);
+    if (KEEP) ld_param8<TAIL>(p.bias, p.bias_dt, c, rms_cols<NC, TAIL>(p.C, c, k), bias[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sw[k][e] = sb[k][e] = 0.f;
+  }
   int turn = 0;
+  Raw next;
+  if (PRE && rows > 0) next.load(p, (uint32_t)r0, first);
 #pragma unroll 1
-  for (int i = 0; i < p.rows; ++i) {
-    const int64_t r64 = r0 + i;
-    if (r64 >= p.N) break;  // the whole team
-    const uint32_t r = (uint32_t)r64;
-    raw8<TDY> dyr[NC];
-    raw8<TZ> ur[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      const int c = 8 * (first + 64 * W * k);
-      dyr[k] = ld8<TDY>(p.dy, r64 * p.dys + c, p.dye, p.C - c);
-      if (p.dzu) ur[k] = ld8<TZ>(p.dzu, r64 * p.dzus + c, p.dzue, p.C - c);
+  for (int i = 0; i < rows; ++i) {
+    const uint32_t r = (uint32_t)(r0 + i);
+    Raw raw;
+    if (PRE) {
+      raw = next;
+      if (i + 1 < rows) next.load(p, r + 1, first);
+    } else {
+      raw.load(p, r, first);
     }
+    uint4 words[NC];
+    rms_words<NC, W>(p, r, first, words);
     float z[NC][8], g[NC][8];
-    uint32_t keep[NC];
-    rms_load_z<NC, W, TX, TR>(p, r, first, z, keep);
-    const float rstd = p.rstd[r];
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int c = 8 * (first + 64 * W * k), n = p.C - c;
-      float w[8];
-      cvt8<TDY>(dyr[k], n, g[k]);
-      ld_param8(p.w, p.w_dt, c, n, w);
+      const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
+      if (!KEEP) ld_param8<TAIL>(p.w, p.w_dt, c, n, w[k]);
+      if (!KEEP) ld_param8<TAIL>(p.bias, p.bias_dt, c, n, bias[k]);
+      rms_z<NC, W, TX, TR, TAIL>(p, raw.z, k, n, bias[k], words[k], z[k]);
+      cvt8<TDY, TAIL>(raw.dy[k], n, g[k]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        z[k][e] *= rstd;  // the normed value
+        z[k][e] *= raw.rstd;  // the normed value
         sw[k][e] += g[k][e] * z[k][e];
-        g[k][e] *= w[e];
+        g[k][e] *= w[k][e];
         s += g[k][e] * z[k][e];
       }
     }
     const float m = team_sum<W>(s, buf, wr, turn) / (float)p.C;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int c = 8 * (first + 64 * W * k), n = p.C - c;
-      float u[8];
+      const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[k][e] = raw.rstd * (g[k][e] - z[k][e] * m);
       if (p.dzu) {
-        cvt8<TZ>(ur[k], n, u);
-      } else {
+        float u[8];
+        cvt8<TZ, TAIL>(raw.u[k], n, u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = 0.f;
+        for (int e = 0; e < 8; ++e) g[k][e] += u[e];
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[k][e] = rstd * (g[k][e] - z[k][e] * m) + u[e];
-      if (p.dres) st8<TR>(p.dres, r64 * p.drs + c, n, g[k]);
-      if (p.d.t) apply_keep(keep[k], p.d.scale, g[k]);
-      if (p.dx) st8<TX>(p.dx, r64 * p.dxs + c, n, g[k]);
+      if (p.dres) st8<TR, TAIL>(p.dres, (int64_t)r * p.drs + c, n, g[k]);
+      if (p.d.on) drop8(p.d, words[k], g[k]);
+      if (p.dx) st8<TX, TAIL>(p.dx, (int64_t)r * p.dxs + c, n, g[k]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sb[k][e] += g[k][e];
     }
@@ -273,13 +324,9 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_bwd_kernel(RmsRows p) {
   if constexpr (W > 1) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int c = 8 * (first + 64 * W * k);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < p.C) {
-          out[c + e] = sw[k][e];
-          if (sums == 2) out[p.C + c + e] = sb[k][e];
-        }
+      const int c = 8 * (first + 64 * W * k), n = rms_cols<NC, TAIL>(p.C, c, k);
+      st8<float, TAIL>(out, c, n, sw[k]);
+      if (sums == 2) st8<float, TAIL>(out, p.C + c, n, sb[k]);
     }
   } else {
     // the four waves' sums, added in wave order
@@ -289,17 +336,21 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_bwd_kernel(RmsRows p) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
           const int c = 8 * (first + 64 * k);
+          if (c < p.C) {  // columns past the row lie inside red, and are not read
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c + e < p.C) {
+            for (int e = 0; e < 8; ++e) {
               red[c + e] = v == 0 ? sw[k][e] : red[c + e] + sw[k][e];
-              if (sums == 2) red[p.C + c + e] = v == 0 ? sb[k][e] : red[p.C + c + e] + sb[k][e];
+              red[512 * NC + c + e] = v == 0 ? sb[k][e] : red[512 * NC + c + e] + sb[k][e];
             }
+          }
         }
       }
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < sums * p.C; i += 256) out[i] = red[i];
+    for (int i = threadIdx.x; i < p.C; i += 256) {
+      out[i] = red[i];
+      if (sums == 2) out[p.C + i] = red[512 * NC + i];
+    }
   }
 }
 
