@@ -3,13 +3,17 @@
 // token v, by sorted tokens.
 //
 // The gradient:
-//   1. the positions are sorted by token, stably, with a radix sort whose
+//   1. the positions are sorted by token, stably: up to RANK_N positions by
+//      counting, for each, the positions before it (every pair is compared,
+//      on all compute units, in one launch); more with a radix sort whose
 //      digits cover the vocabulary's bits (two digits of nine bits up to
-//      262143 tokens).  The padding token and ids outside the table take the
-//      key V, behind every token;
+//      262143 tokens; two launches a digit).  The padding token and ids
+//      outside the table take the key V, behind every token;
 //   2. while it runs, other workgroups of the same launches clear dW (the
 //      largest part of the traffic where the batch is smaller than the
-//      vocabulary);
+//      vocabulary).  Of the radix sort's launches the first marks the tokens
+//      that occur and the others clear the rows of those that do not, so that
+//      no row is written twice; beside the counting sort every row is cleared;
 //   3. the sorted positions are cut in chunks of equal length, one wave a
 //      chunk and 512 columns, whatever the tokens' frequencies are: a wave
 //      sums its rows of dout token by token, in fp32, in the order of the
@@ -24,6 +28,13 @@
 namespace dsa {
 namespace hid {
 
+// A lane's eight columns of what it would take from column c on: where they
+// would pass the row's end, the row's last eight.  Two lanes then take the
+// same columns and write the same values, and no width of eight or more needs
+// a condition.  NARROW: rows of fewer than eight columns.
+template <bool NARROW>
+DSA_DEV int embed_col(int C, int c) { return NARROW ? c : min(c, C - 8); }
+
 constexpr int EMB_T = 256;      // chunks (threads) a lookup block takes at most
 constexpr int EMB_U = 4;        // rows whose loads are issued together
 constexpr int SORT_T = 512;     // threads of a sort workgroup
@@ -32,7 +43,9 @@ constexpr int SORT_TILE = SORT_T * SORT_R;
 constexpr int SORT_BITS = 9;    // a digit's bits at most: SORT_T >= 2^SORT_BITS
 constexpr int SORT_D = 1 << SORT_BITS;
 constexpr int SORT_W = SORT_T / 64;
-constexpr int FILL_IT = 8;      // 16-byte stores a thread of a fill workgroup makes
+constexpr int FILL_BYTES = 65536;  // of dW, about, a fill workgroup clears
+constexpr int RANK_BITS = 13;
+constexpr int RANK_N = 1 << RANK_BITS;  // positions the counting sort takes at most
 
 struct EmbedRows {
   const void *ids, *w;
@@ -50,11 +63,11 @@ DSA_DEV int64_t ld_id(const void* ids, int64_t i, int ids64) {
 
 // Threads as in drop_fwd_kernel.  An id outside [0, V) reads nothing and
 // gives a row of NaN.
-template <typename TW, typename TY, bool TAIL>
+template <typename TW, typename TY, bool NARROW>
 __global__ __launch_bounds__(EMB_T) void embed_fwd_kernel(EmbedRows p) {
   const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * EMB_T + (int)threadIdx.x - sub * p.cw;
-  const int c = 8 * chunk, n = p.C - c;
-  if (sub >= p.subs || n <= 0) return;
+  const int c = embed_col<NARROW>(p.C, 8 * chunk), n = p.C - c;
+  if (sub >= p.subs || 8 * chunk >= p.C) return;
   const int64_t extent = (p.V - 1) * p.ws + p.C;
   const int64_t r0 = (int64_t)blockIdx.x * p.rows * p.subs + sub;
   for (int i = 0; i < p.rows; i += EMB_U) {
@@ -66,18 +79,18 @@ __global__ __launch_bounds__(EMB_T) void embed_fwd_kernel(EmbedRows p) {
 #pragma unroll
     for (int u = 0; u < EMB_U; ++u) {
       const bool ok = (uint64_t)id[u] < (uint64_t)p.V;
-      w[u] = ld8<TW, TAIL>(p.w, ok ? id[u] * p.ws + c : c, extent, ok ? n : 0);
+      w[u] = ld8<TW, NARROW>(p.w, ok ? id[u] * p.ws + c : c, extent, ok ? n : 0);
     }
 #pragma unroll
     for (int u = 0; u < EMB_U; ++u) {
       const int64_t r = r0 + (int64_t)(i + u) * p.subs;
       if (r >= p.N) return;
       float v[8];
-      cvt8<TW, TAIL>(w[u], 8, v);
+      cvt8<TW, NARROW>(w[u], 8, v);
       const float s = (uint64_t)id[u] < (uint64_t)p.V ? p.scale : __builtin_nanf("");
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= s;
-      st8<TY, TAIL>(p.y, r * p.ys + c, n, v);
+      st8<TY, NARROW>(p.y, r * p.ys + c, n, v);
     }
   }
 }
@@ -91,12 +104,13 @@ struct SortParams {
   const uint32_t *kin, *pin;  // sorted so far (null: from ids)
   uint32_t *kout, *pout;
   uint32_t* counts;       // [tiles][SORT_D]
-  char* fill;             // the part of dW that this launch clears
-  int64_t fill_bytes;
+  uint8_t* occurs;        // [V] tokens that occur, or null
+  void* dw;               // [V, C]; this launch clears rows [fill0, fill1), fill_rows a workgroup
+  int64_t fill0, fill1;
+  int C, fill_rows;
   uint32_t N;
   int ids64, tiles, per_tile;  // per_tile: runs of SORT_TILE keys a workgroup takes
   int shift, bits;        // the digit: (key >> shift) & ((1 << bits) - 1)
-  int passes;             // embed_sort_one_kernel: digits, from the lowest
 };
 
 DSA_DEV uint32_t token_key(const SortParams& s, uint32_t i) {
@@ -104,17 +118,34 @@ DSA_DEV uint32_t token_key(const SortParams& s, uint32_t i) {
   return (uint64_t)id < (uint64_t)s.V && id != s.padding ? (uint32_t)id : (uint32_t)s.V;
 }
 
-// workgroup `b` of the launch's fill workgroups
-DSA_DEV void fill_zero(const SortParams& s, int64_t b) {
-  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-  const int64_t n16 = s.fill_bytes / 16, at = b * SORT_T * FILL_IT + threadIdx.x;
+// Workgroup `b` of the launch's fill workgroups: its rows of dW, but those of
+// tokens that occur, 16 bytes a thread at a time; consecutive threads write
+// consecutive bytes.
+template <typename TW, bool NARROW>
+DSA_DEV void fill_zero(const SortParams& s, int b) {
+  constexpr int E = NARROW ? 1 : 16 / (int)sizeof(TW);  // elements a store
+  typedef TW vec __attribute__((ext_vector_type(E)));
+  typedef vec vecu __attribute__((aligned(sizeof(TW))));
+  const int64_t v0 = s.fill0 + (int64_t)b * s.fill_rows;
+  const int64_t left = s.fill1 - v0;
+  const uint32_t rows = (uint32_t)(left < s.fill_rows ? left : s.fill_rows), units = (uint32_t)(s.C + E - 1) / E;
+  vec zero;
 #pragma unroll
-  for (int i = 0; i < FILL_IT; ++i) {
-    const int64_t k = at + (int64_t)i * SORT_T;
-    if (k < n16) reinterpret_cast<u4*>(s.fill)[k] = u4{0u, 0u, 0u, 0u};
+  for (int e = 0; e < E; ++e) zero[e] = (TW)0.f;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < rows * units; i += SORT_T) {
+    const uint32_t r = i / units;
+    const int c = min(E * (int)(i - r * units), s.C - E);
+    if (s.occurs && s.occurs[v0 + r]) continue;
+    *reinterpret_cast<vecu*>(static_cast<TW*>(s.dw) + (v0 + r) * s.C + c) = zero;
   }
-  if (b == 0 && threadIdx.x == 0)
-    for (int64_t k = 16 * n16; k < s.fill_bytes; k += 2) *reinterpret_cast<uint16_t*>(s.fill + k) = 0;
+}
+
+// Clears the marks of the tokens that occur.
+static __global__ __launch_bounds__(SORT_T) void embed_unmark_kernel(SortParams s) {
+  const int64_t v0 = ((int64_t)blockIdx.x * SORT_T + threadIdx.x) * 16;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  if (v0 < s.V) *reinterpret_cast<u4*>(s.occurs + v0) = u4{0u, 0u, 0u, 0u};  // [V] rounded up to 16
 }
 
 struct SortLds {
@@ -166,9 +197,10 @@ DSA_DEV uint32_t digit_scan(SortLds& l, uint32_t mine) {
 }
 
 // counts[tile][digit]: the tile's keys of each digit
-static __global__ __launch_bounds__(SORT_T) void embed_count_kernel(SortParams s) {
+template <typename TW, bool NARROW>
+__global__ __launch_bounds__(SORT_T) void embed_count_kernel(SortParams s) {
   if ((int)blockIdx.x >= s.tiles) {
-    fill_zero(s, (int)blockIdx.x - s.tiles);
+    fill_zero<TW, NARROW>(s, (int)blockIdx.x - s.tiles);
     return;
   }
   __shared__ uint32_t cnt[SORT_D];
@@ -179,6 +211,7 @@ static __global__ __launch_bounds__(SORT_T) void embed_count_kernel(SortParams s
   const uint32_t mask = (1u << s.bits) - 1;
   for (int64_t i = n0 + threadIdx.x; i < n1; i += SORT_T) {
     const uint32_t key = s.kin ? s.kin[i] : token_key(s, (uint32_t)i);
+    if (!s.kin && key < (uint32_t)s.V) s.occurs[key] = 1;
     atomicAdd(&cnt[(key >> s.shift) & mask], 1u);
   }
   __syncthreads();
@@ -186,9 +219,10 @@ static __global__ __launch_bounds__(SORT_T) void embed_count_kernel(SortParams s
 }
 
 // Moves the tile's keys and positions to their places by one digit.
-static __global__ __launch_bounds__(SORT_T) void embed_scatter_kernel(SortParams s) {
+template <typename TW, bool NARROW>
+__global__ __launch_bounds__(SORT_T) void embed_scatter_kernel(SortParams s) {
   if ((int)blockIdx.x >= s.tiles) {
-    fill_zero(s, (int)blockIdx.x - s.tiles);
+    fill_zero<TW, NARROW>(s, (int)blockIdx.x - s.tiles);
     return;
   }
   __shared__ SortLds l;
@@ -196,6 +230,7 @@ static __global__ __launch_bounds__(SORT_T) void embed_scatter_kernel(SortParams
   const uint32_t mask = (1u << s.bits) - 1;
   // thread d: where digit d of this tile begins in the sorted order
   uint32_t before = 0, total = 0;
+#pragma unroll 16
   for (int i = 0; i < s.tiles; ++i) {
     const uint32_t c = s.counts[(int64_t)i * SORT_D + t];
     total += c;
@@ -238,66 +273,41 @@ static __global__ __launch_bounds__(SORT_T) void embed_scatter_kernel(SortParams
   }
 }
 
-// At most SORT_TILE positions: one workgroup sorts them by every digit in LDS.
-static __global__ __launch_bounds__(SORT_T) void embed_sort_one_kernel(SortParams s) {
-  if (blockIdx.x > 0) {
-    fill_zero(s, (int64_t)blockIdx.x - 1);
+// At most RANK_N positions of a vocabulary below 2^(32 - RANK_BITS): the key
+// and the position in one 32-bit word, and a position's place is the number
+// of smaller words.  A workgroup places 64 positions, one a lane; its waves
+// share the comparisons.  All words lie in its LDS and are read four at a
+// time, the same four by all lanes.
+template <typename TW, bool NARROW>
+__global__ __launch_bounds__(SORT_T) void embed_rank_kernel(SortParams s) {
+  if ((int)blockIdx.x >= s.tiles) {
+    fill_zero<TW, NARROW>(s, (int)blockIdx.x - s.tiles);
     return;
   }
-  __shared__ SortLds l;
-  __shared__ uint32_t ks[SORT_TILE], ps[SORT_TILE];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = threadIdx.x;
-  const int n0 = w * 64 * SORT_R + lane;
-  const uint32_t mask = (1u << s.bits) - 1;
-  uint32_t key[SORT_R], pos[SORT_R], digit[SORT_R], rank[SORT_R];
-  bool ok[SORT_R];
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  __shared__ __align__(16) uint32_t words[RANK_N];
+  __shared__ uint32_t part[SORT_W][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int n4 = ((int)s.N + 3) / 4;
+  for (int i = threadIdx.x; i < 4 * n4; i += SORT_T)
+    words[i] = i < (int)s.N ? token_key(s, (uint32_t)i) << RANK_BITS | (uint32_t)i : 0xffffffffu;
+  __syncthreads();
+  const int i = (int)blockIdx.x * 64 + lane;
+  const uint32_t mine = i < (int)s.N ? words[i] : 0u;
+  uint32_t place = 0;
+#pragma unroll 4
+  for (int q = w; q < n4; q += SORT_W) {
+    const u4 v = reinterpret_cast<const u4*>(words)[q];
 #pragma unroll
-  for (int j = 0; j < SORT_R; ++j) {
-    const uint32_t i = (uint32_t)(n0 + 64 * j);
-    ok[j] = i < s.N;
-    key[j] = ok[j] ? token_key(s, i) : 0;
-    pos[j] = i;
+    for (int e = 0; e < 4; ++e) place += v[e] < mine ? 1u : 0u;
   }
-  for (int pass = 0; pass < s.passes; ++pass) {
+  part[w][lane] = place;
+  __syncthreads();
+  if (w > 0 || i >= (int)s.N) return;
 #pragma unroll
-    for (int j = 0; j < SORT_R; ++j) digit[j] = (key[j] >> (pass * s.bits)) & mask;
-    wave_ranks(l, digit, ok, s.bits, rank);
-    __syncthreads();
-    uint32_t total = 0;
-#pragma unroll
-    for (int i = 0; i < SORT_W; ++i) total += l.cnt[i][t];
-    uint32_t at = digit_scan(l, total);
-#pragma unroll
-    for (int i = 0; i < SORT_W; ++i) {
-      const uint32_t c = l.cnt[i][t];
-      l.cnt[i][t] = at;
-      at += c;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SORT_R; ++j) {
-      if (ok[j]) {
-        const uint32_t to = l.cnt[w][digit[j]] + rank[j];
-        ks[to] = key[j];
-        ps[to] = pos[j];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SORT_R; ++j) {
-      if (ok[j]) {
-        key[j] = ks[n0 + 64 * j];
-        pos[j] = ps[n0 + 64 * j];
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < SORT_R; ++j) {
-    if (ok[j]) {
-      s.kout[n0 + 64 * j] = key[j];
-      s.pout[n0 + 64 * j] = pos[j];
-    }
-  }
+  for (int v = 1; v < SORT_W; ++v) place += part[v][lane];
+  s.kout[place] = mine >> RANK_BITS;
+  s.pout[place] = (uint32_t)i;
 }
 
 // ---------------------------------------------------------------------------
@@ -314,48 +324,64 @@ struct EmbedSums {
   float scale;
 };
 
-template <typename TDY, typename TW, bool TAIL>
+// A wave: one chunk of positions, 512 columns.  A wave keeps two batches of
+// rows in flight: the next is loaded while one is summed.  Every batch is
+// loaded whole (past the chunk's end its last row again): a load behind a
+// condition would make the compiler wait for the newer batch with the older.
+// dout is read past the caches in bf16, where one instruction takes whole
+// lines: it is read once, and the lines of dW that the fill has just written
+// stay in the last-level cache instead.  Of 131072 x 1024 bf16 positions and
+// 128100 tokens that takes the sums from 107 to 70 us and the whole pass from
+// 246 to 228.
+template <typename TDY, typename TW, bool NARROW>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSums p) {
+  constexpr int U = sizeof(TDY) == 2 ? 8 : 4;  // rows a batch
   const int lane = threadIdx.x & 63;
   const uint32_t item = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t ch = item / (uint32_t)p.slabs;
   if (ch >= p.chunks) return;
-  const int c = (int)(item - ch * p.slabs) * 512 + lane * 8, n = p.C - c;
+  const int c0 = (int)(item - ch * p.slabs) * 512 + lane * 8, c = embed_col<NARROW>(p.C, c0);
+  const int n = c0 < p.C ? p.C - c : 0;  // lanes past the row load with the others, and write nothing
   const uint32_t i0 = ch * (uint32_t)p.K, i1 = min(i0 + (uint32_t)p.K, p.N);
   const uint32_t i = i0 + lane;
   const uint32_t key = i < i1 ? p.keys[i] : p.V, pos = i < i1 ? p.pos[i] : 0;
   const uint32_t next = i < i1 && i + 1 < p.N ? p.keys[i + 1] : p.V;
+  const uint32_t prev = i0 > 0 ? p.keys[i0 - 1] : p.V;
   const int m = __popcll(__ballot(key < p.V));  // the chunk's tokens: the keys V come last
   if (m == 0) return;
   const uint64_t ends = __ballot(lane < m && key != next);
   // the chunk's first token began before it
-  bool carried = i0 > 0 && p.keys[i0 - 1] == (uint32_t)__builtin_amdgcn_readlane(key, 0);
+  bool carried = __builtin_amdgcn_readfirstlane(prev) == __builtin_amdgcn_readfirstlane(key);
+  const uint32_t cb = (uint32_t)c * (uint32_t)sizeof(TDY);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 8;
-  for (int j0 = 0; j0 < m; j0 += U) {
-    raw8<TDY> dy[U];
+  auto load = [&](int j0, raw8<TDY>(&dy)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t r = (uint32_t)__builtin_amdgcn_readlane(pos, min(j0 + u, m - 1));
-      dy[u] = ld8<TDY, TAIL>(p.dy, (int64_t)r * p.dys + c, p.dye, n);
+      const char* row = static_cast<const char*>(p.dy) + (int64_t)r * p.dys * (int64_t)sizeof(TDY);  // uniform
+      typedef const typename Raw8<TDY>::v8u* ptr;
+      if constexpr (NARROW) dy[u] = ld8<TDY, true>(p.dy, (int64_t)r * p.dys + c, p.dye, n);
+      else if constexpr (sizeof(TDY) == 2) dy[u] = __builtin_nontemporal_load(reinterpret_cast<ptr>(row + cb));
+      else dy[u] = *reinterpret_cast<ptr>(row + cb);
     }
+  };
+  auto sum = [&](int j0, const raw8<TDY>(&dy)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u;
       if (j < m) {
         float v[8];
-        cvt8<TDY, TAIL>(dy[u], n, v);
+        cvt8<TDY, NARROW>(dy[u], n, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += v[e];
         const bool end = (ends >> j) & 1;
         if (end || j == m - 1) {
           if (carried || !end) {
-            float* out = p.part + ((int64_t)ch * 2 + (carried ? 0 : 1)) * p.C;
-            st8<float, TAIL>(out, c, n, acc);
+            st8<float, NARROW>(p.part + ((int64_t)ch * 2 + (carried ? 0 : 1)) * p.C, c, n, acc);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = acc[e] * p.scale;
-            st8<TW, TAIL>(p.dw, (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j) * p.dws + c, n, v);
+            st8<TW, NARROW>(p.dw, (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j) * p.dws + c, n, v);
           }
           carried = false;
 #pragma unroll
@@ -363,59 +389,103 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSums p) {
         }
       }
     }
+  };
+  raw8<TDY> a[U], b[U];
+  load(0, a);
+  for (int j0 = 0; j0 < m; j0 += 2 * U) {
+    load(j0 + U, b);
+    sum(j0, a);
+    load(j0 + 2 * U, a);
+    sum(j0 + U, b);
   }
 }
 
-// Block (chunk, slab): the token that begins in the chunk and goes on past
-// its end, from the chunk's own partial sum and those of the chunks behind.
-template <typename TW, bool TAIL>
-__global__ __launch_bounds__(256) void embed_join_kernel(EmbedSums p) {
-  __shared__ float red[3][64][8];
-  const int lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t ch = blockIdx.x / (uint32_t)p.slabs;
-  const int c = (int)(blockIdx.x - ch * p.slabs) * 512 + lane * 8, n = p.C - c;
-  const uint64_t i0 = (uint64_t)ch * p.K, i1 = i0 + p.K;
-  if (i1 >= p.N) return;
-  const uint32_t key = p.keys[i1];
-  if (key >= p.V || p.keys[i1 - 1] != key) return;
-  if (i0 > 0 && p.keys[i0 - 1] == key) return;  // it began before
-  // the chunks behind that begin with the token: the keys are sorted
-  uint32_t last = ch;
-  for (;;) {
-    const uint64_t at = ((uint64_t)last + 1 + lane) * p.K;
-    const int more = __popcll(__ballot(at < p.N && p.keys[at < p.N ? at : 0] == key));
-    last += more;
-    if (more < 64) break;
-  }
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+// The sum of the token that begins in chunk ch and goes on to chunk `last`:
+// the lane's columns of ch's partial sum, and by every `waves`-th chunk from
+// q on of those behind.
+template <bool NARROW>
+DSA_DEV void join_parts(const EmbedSums& p, uint32_t ch, uint32_t last, int q, int waves, int c, int n, float (&acc)[8]) {
+  constexpr int U = 8;
   const int64_t extent = (int64_t)p.chunks * 2 * p.C;
-  constexpr int U = 4;
-  if (q == 0) cvt8<float, TAIL>(ld8<float, TAIL>(p.part, ((int64_t)ch * 2 + 1) * p.C + c, extent, n), n, acc);
-  for (int64_t k0 = (int64_t)ch + 1 + q; k0 <= last; k0 += 4 * U) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  if (q == 0) cvt8<float, NARROW>(ld8<float, NARROW>(p.part, ((int64_t)ch * 2 + 1) * p.C + c, extent, n), n, acc);
+  for (int64_t k0 = (int64_t)ch + 1 + q; k0 <= last; k0 += waves * U) {
     raw8<float> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      v[u] = ld8<float, TAIL>(p.part, min(k0 + 4 * u, (int64_t)last) * 2 * p.C + c, extent, n);
+      v[u] = ld8<float, NARROW>(p.part, min(k0 + waves * u, (int64_t)last) * 2 * p.C + c, extent, n);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (k0 + 4 * u <= last) {
+      if (k0 + waves * u <= last) {
+        float w[8];
+        cvt8<float, NARROW>(v[u], n, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += e < n ? v[u][e] : 0.f;
+        for (int e = 0; e < 8; ++e) acc[e] += w[e];
       }
   }
-  if (q > 0) {
+}
+
+// A block: JOIN_W chunks and 512 columns; wave q looks whether a token begins in
+// its chunk and goes on past the chunk's end.  One that ends within JOIN_ONE
+// chunks is joined by the wave, a longer one by the whole block.
+constexpr uint32_t JOIN_ONE = 8;
+constexpr int JOIN_W = 8;
+
+template <typename TW, bool NARROW>
+__global__ __launch_bounds__(64 * JOIN_W) void embed_join_kernel(EmbedSums p) {
+  __shared__ float red[JOIN_W - 1][64][8];
+  __shared__ uint32_t far[JOIN_W][2];  // per wave: its chunk's last chunk (0: none to share), the token
+  const int lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t ch0 = blockIdx.x / (uint32_t)p.slabs * JOIN_W, ch = ch0 + q;
+  const int c0 = (int)(blockIdx.x % (uint32_t)p.slabs) * 512 + lane * 8, c = embed_col<NARROW>(p.C, c0);
+  const int n = c0 < p.C ? p.C - c : 0;
+  const uint64_t i0 = (uint64_t)ch * p.K, i1 = i0 + p.K;
+  float acc[8];
+  if (lane == 0) far[q][0] = 0;
+  if (i1 < p.N) {
+    const uint32_t key = p.keys[i1], own = p.keys[i1 - 1], prev = i0 > 0 ? p.keys[i0 - 1] : p.V;
+    if (key < p.V && own == key && prev != key) {  // with prev == key it began before
+      // the chunks behind that begin with the token: the keys are sorted
+      uint32_t last = ch;
+      for (;;) {
+        const uint64_t at = ((uint64_t)last + 1 + lane) * p.K;
+        const int more = __popcll(__ballot(at < p.N && p.keys[at < p.N ? at : 0] == key));
+        last += more;
+        if (more < 64) break;
+      }
+      if (last - ch <= JOIN_ONE) {
+        join_parts<NARROW>(p, ch, last, 0, 1, c, n, acc);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) red[q - 1][lane][e] = acc[e];
+        for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
+        st8<TW, NARROW>(p.dw, (int64_t)key * p.dws + c, n, acc);
+      } else if (lane == 0) {
+        far[q][0] = last;
+        far[q][1] = key;
+      }
+    }
   }
   __syncthreads();
-  if (q > 0) return;
+  for (int v = 0; v < JOIN_W; ++v) {
+    const uint32_t last = far[v][0], key = far[v][1];
+    if (last == 0) continue;  // uniform over the block
+    join_parts<NARROW>(p, ch0 + v, last, q, JOIN_W, c, n, acc);
+    if (q > 0) {
 #pragma unroll
-  for (int v = 0; v < 3; ++v)
+      for (int e = 0; e < 8; ++e) red[q - 1][lane][e] = acc[e];
+    }
+    __syncthreads();
+    if (q == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += red[v][lane][e];
+      for (int w = 0; w < JOIN_W - 1; ++w)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
-  st8<TW, TAIL>(p.dw, (int64_t)key * p.dws + c, n, acc);
+        for (int e = 0; e < 8; ++e) acc[e] += red[w][lane][e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
+      st8<TW, NARROW>(p.dw, (int64_t)key * p.dws + c, n, acc);
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace hid

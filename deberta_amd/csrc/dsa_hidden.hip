@@ -43,6 +43,13 @@ void by_type(int dt, F f) {
   else f(Tag<float>{});
 }
 
+// f(NARROW): whether rows hold fewer than the eight columns of a lane
+template <typename F>
+void by_narrow(int C, F f) {
+  if (C < 8) f(std::true_type{});
+  else f(std::false_type{});
+}
+
 bool elem_aligned(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(elem_bytes(dt) - 1)) == 0; }
 // a tensor of rows: given, its type known, aligned to its elements
 bool rows_given(const void* p, int64_t stride, int dt) { return p && dtype_ok(dt) && elem_aligned(p, dt) && stride >= 0; }
@@ -222,31 +229,34 @@ int bit_length(int64_t v) {
   while (v >> b) ++b;
   return b;
 }
-// positions a chunk of the sums: enough chunks for 4096 waves, at most 64
+// positions a chunk of the sums: enough chunks for 2048 waves, at most 64
 int embed_chunk(int64_t N, int slabs) {
   int k = 8;
-  while (k < 64 && N * slabs > (int64_t)4096 * k) k *= 2;
+  while (k < 64 && N * slabs > (int64_t)2048 * k) k *= 2;
   return k;
 }
 struct EmbedPlan {
+  bool rank;  // sorted by counting
   int bits, passes, tiles, per_tile, slabs, K;
   int64_t chunks;
-  size_t keys, counts, part, total;  // bytes of a key or position buffer, the counts, the partial sums
+  size_t keys, counts, marks, part, total;  // bytes: a key or position buffer, the counts, the marks, the partial sums
 };
 EmbedPlan embed_plan(int64_t N, int C, int64_t V) {
   EmbedPlan e;
   const int all = bit_length(V);
   e.passes = (int)cdiv(all, hid::SORT_BITS);
   e.bits = (int)cdiv(all, e.passes);
+  e.rank = N <= hid::RANK_N && all <= 32 - hid::RANK_BITS;
   e.per_tile = (int)cdiv(N, (int64_t)hid::SORT_TILE * 256);
-  e.tiles = (int)cdiv(N, (int64_t)hid::SORT_TILE * e.per_tile);
+  e.tiles = e.rank ? (int)cdiv(N, 64) : (int)cdiv(N, (int64_t)hid::SORT_TILE * e.per_tile);
   e.slabs = (int)cdiv(C, 512);
   e.K = embed_chunk(N, e.slabs);
   e.chunks = cdiv(N, e.K);
   e.keys = align_up((size_t)N * 4, 256);
-  e.counts = e.tiles > 1 ? align_up((size_t)e.tiles * hid::SORT_D * 4, 256) : 0;
+  e.counts = e.rank ? 0 : align_up((size_t)e.tiles * hid::SORT_D * 4, 256);
+  e.marks = e.rank ? 0 : align_up((size_t)V, 256);
   e.part = align_up((size_t)e.chunks * 2 * C * sizeof(float), 256);
-  e.total = e.keys * (e.tiles > 1 && e.passes > 1 ? 4 : 2) + e.counts + e.part;
+  e.total = e.keys * (!e.rank && e.passes > 1 ? 4 : 2) + e.counts + e.marks + e.part;
   return e;
 }
 
@@ -395,8 +405,8 @@ int dsa_embed_fwd(const dsa_embed_args* a, void* stream) {
   if (!grid_ok(nb, g.slabs, g.threads)) return fail("dsa_embed: too many rows or columns for one launch");
   by_type(a->weight_dtype, [&](auto tw) {
     by_type(a->y_dtype, [&](auto ty) {
-      by_tail(a->C, [&](auto tail) {
-        hipLaunchKernelGGL((hid::embed_fwd_kernel<typename decltype(tw)::type, typename decltype(ty)::type, decltype(tail)::value>),
+      by_narrow(a->C, [&](auto narrow) {
+        hipLaunchKernelGGL((hid::embed_fwd_kernel<typename decltype(tw)::type, typename decltype(ty)::type, decltype(narrow)::value>),
                            dim3((unsigned)nb, (unsigned)g.slabs), dim3((unsigned)g.threads), 0, st, p);
       });
     });
@@ -410,53 +420,58 @@ int dsa_embed_bwd(const dsa_embed_args* a, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (refuse_capture(st, "dsa_embed_bwd")) return 1;
   const EmbedPlan e = embed_plan(a->N, a->C, a->V);
-  if (!grid_ok(cdiv(e.chunks * e.slabs, 4), 1, 256) || !grid_ok(e.chunks * e.slabs, 1, 256))
+  if (!grid_ok(cdiv(e.chunks, hid::JOIN_W) * cdiv(a->C, 512), 1, 64 * hid::JOIN_W))
     return fail("dsa_embed: too many rows or columns for one launch");
   char* ws = static_cast<char*>(a->workspace);
-  const bool one = e.tiles == 1;
   uint32_t* buf[4];  // keys and positions, twice
   for (int i = 0; i < 4; ++i) buf[i] = reinterpret_cast<uint32_t*>(ws + i * e.keys);
-  ws += e.keys * (!one && e.passes > 1 ? 4 : 2);
+  ws += e.keys * (!e.rank && e.passes > 1 ? 4 : 2);
   hid::SortParams s{};
   s.ids = a->ids, s.V = a->V, s.padding = a->padding;
   s.counts = reinterpret_cast<uint32_t*>(ws);
-  float* part = reinterpret_cast<float*>(ws + e.counts);
+  s.occurs = e.rank ? nullptr : reinterpret_cast<uint8_t*>(ws + e.counts);
+  float* part = reinterpret_cast<float*>(ws + e.counts + e.marks);
   s.N = (uint32_t)a->N, s.ids64 = a->ids_bytes == 8;
-  s.tiles = e.tiles, s.per_tile = e.per_tile, s.bits = e.bits, s.passes = e.passes;
-  // each sort launch clears its share of dW
-  const int64_t bytes = (int64_t)a->V * a->C * elem_bytes(a->weight_dtype);
-  const int launches = one ? 1 : 2 * e.passes;
-  const int64_t share = cdiv(cdiv(bytes, 16), launches) * 16;
-  constexpr int64_t kFill = (int64_t)hid::SORT_T * hid::FILL_IT * 16;
-  char* at = static_cast<char*>(a->dweight);
-  int64_t left = bytes;
-  auto fill_blocks = [&]() {
-    s.fill = at, s.fill_bytes = std::min(share, left);
-    at += s.fill_bytes, left -= s.fill_bytes;
-    return cdiv(s.fill_bytes, kFill);
+  s.tiles = e.tiles, s.per_tile = e.per_tile, s.bits = e.bits;
+  s.dw = a->dweight, s.C = a->C;
+  s.fill_rows = (int)std::max<int64_t>(1, hid::FILL_BYTES / ((int64_t)a->C * elem_bytes(a->weight_dtype)));
+  // each launch of the sort but the first of several clears its share of dW
+  const int64_t share = cdiv(a->V, e.rank ? 1 : 2 * e.passes - 1);
+  if (!grid_ok(e.tiles + cdiv(share, s.fill_rows), 1, hid::SORT_T)) return fail("dsa_embed: the table is too large for one launch");
+  const dim3 block(hid::SORT_T);
+  auto grid = [&](bool fill) {
+    s.fill0 = s.fill1;
+    if (fill) s.fill1 = std::min(s.fill0 + share, a->V);
+    return dim3((unsigned)(e.tiles + cdiv(s.fill1 - s.fill0, s.fill_rows)));
   };
-  if (!grid_ok(e.tiles + cdiv(share, kFill), 1, hid::SORT_T)) return fail("dsa_embed: the table is too large for one launch");
-  const uint32_t *keys, *pos;
-  if (one) {
-    s.kout = buf[0], s.pout = buf[1];
-    const int64_t nf = fill_blocks();
-    hipLaunchKernelGGL(hid::embed_sort_one_kernel, dim3((unsigned)(1 + nf)), dim3(hid::SORT_T), 0, st, s);
-    if (launch_check("embed_sort_one_kernel")) return 1;
-    keys = buf[0], pos = buf[1];
-  } else {
-    for (int pass = 0; pass < e.passes; ++pass) {
-      s.shift = pass * e.bits;
-      int64_t nf = fill_blocks();
-      hipLaunchKernelGGL(hid::embed_count_kernel, dim3((unsigned)(e.tiles + nf)), dim3(hid::SORT_T), 0, st, s);
-      if (launch_check("embed_count_kernel")) return 1;
-      nf = fill_blocks();
-      s.kout = buf[2 * (pass & 1)], s.pout = buf[2 * (pass & 1) + 1];
-      hipLaunchKernelGGL(hid::embed_scatter_kernel, dim3((unsigned)(e.tiles + nf)), dim3(hid::SORT_T), 0, st, s);
-      if (launch_check("embed_scatter_kernel")) return 1;
-      s.kin = s.kout, s.pin = s.pout;
-    }
-    keys = s.kin, pos = s.pin;
+  int rc = 0;
+  if (!e.rank) {
+    hipLaunchKernelGGL(hid::embed_unmark_kernel, dim3((unsigned)cdiv(a->V, 16 * hid::SORT_T)), block, 0, st, s);
+    if (launch_check("embed_unmark_kernel")) return 1;
   }
+  by_type(a->weight_dtype, [&](auto tw) {
+    by_narrow(a->C, [&](auto narrow) {
+      typedef typename decltype(tw)::type TW;
+      constexpr bool T = decltype(narrow)::value;
+      if (e.rank) {
+        s.kout = buf[0], s.pout = buf[1];
+        hipLaunchKernelGGL((hid::embed_rank_kernel<TW, T>), grid(true), block, 0, st, s);
+        rc = launch_check("embed_rank_kernel");
+        return;
+      }
+      for (int pass = 0; pass < e.passes && !rc; ++pass) {
+        s.shift = pass * e.bits;
+        s.kout = buf[2 * (pass & 1)], s.pout = buf[2 * (pass & 1) + 1];
+        hipLaunchKernelGGL((hid::embed_count_kernel<TW, T>), grid(pass > 0), block, 0, st, s);
+        if ((rc = launch_check("embed_count_kernel"))) return;
+        hipLaunchKernelGGL((hid::embed_scatter_kernel<TW, T>), grid(true), block, 0, st, s);
+        rc = launch_check("embed_scatter_kernel");
+        s.kin = s.kout, s.pin = s.pout;
+      }
+    });
+  });
+  if (rc) return rc;
+  const uint32_t *keys = s.kout, *pos = s.pout;
   hid::EmbedSums p{};
   p.keys = keys, p.pos = pos, p.dy = a->dy, p.dw = a->dweight, p.part = part;
   p.dys = a->dy_stride, p.dye = (a->N - 1) * a->dy_stride + a->C, p.dws = a->C;
@@ -464,18 +479,21 @@ int dsa_embed_bwd(const dsa_embed_args* a, void* stream) {
   p.C = a->C, p.slabs = e.slabs, p.K = e.K, p.scale = a->scale;
   by_type(a->dy_dtype, [&](auto tdy) {
     by_type(a->weight_dtype, [&](auto tw) {
-      by_tail(a->C, [&](auto tail) {
-        hipLaunchKernelGGL((hid::embed_sum_kernel<typename decltype(tdy)::type, typename decltype(tw)::type, decltype(tail)::value>),
-                           dim3((unsigned)cdiv(e.chunks * e.slabs, 4)), dim3(256), 0, st, p);
+      by_narrow(a->C, [&](auto narrow) {
+        typedef typename decltype(tdy)::type TDY;
+        typedef typename decltype(tw)::type TW;
+        constexpr bool T = decltype(narrow)::value;
+        const dim3 grid((unsigned)cdiv(e.chunks * e.slabs, 4)), block(256);
+        hipLaunchKernelGGL((hid::embed_sum_kernel<TDY, TW, T>), grid, block, 0, st, p);
       });
     });
   });
   if (launch_check("embed_sum_kernel")) return 1;
   if (e.chunks == 1) return 0;
   by_type(a->weight_dtype, [&](auto tw) {
-    by_tail(a->C, [&](auto tail) {
-      hipLaunchKernelGGL((hid::embed_join_kernel<typename decltype(tw)::type, decltype(tail)::value>),
-                         dim3((unsigned)(e.chunks * e.slabs)), dim3(256), 0, st, p);
+    by_narrow(a->C, [&](auto narrow) {
+      hipLaunchKernelGGL((hid::embed_join_kernel<typename decltype(tw)::type, decltype(narrow)::value>),
+                         dim3((unsigned)(cdiv(e.chunks, hid::JOIN_W) * p.slabs)), dim3(64 * hid::JOIN_W), 0, st, p);
     });
   });
   return launch_check("embed_join_kernel");
