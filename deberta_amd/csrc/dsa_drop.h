@@ -22,6 +22,7 @@ struct DropRows {
   const void *x, *bias, *res, *dy;
   void *y, *dx;
   float* part;  // backward: [blocks][C] column sums, or null
+  void* dbias;  // backward of one block: the column sums themselves, or null
   int64_t xs, xe, rs0, rs1, re, ys, dys, dye, dxs;  // row strides and extents, elements
   uint32_t N, rpg;  // rows; rows of a residual group
   int C, bias_dt;
@@ -72,8 +73,8 @@ __global__ __launch_bounds__(DROP_T) void drop_fwd_kernel(DropRows p) {
   }
 }
 
-// dx and, where part is given, the block's column sums of it: the sums of a
-// thread's rows, then of the block's row groups in their order.
+// dx and, where part or dbias is given, the block's column sums of it: the sums
+// of a thread's rows, then of the block's row groups in their order.
 template <typename TDY, typename TX, bool TAIL>
 __global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
   __shared__ float red[DROP_T * 8];
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
       }
     }
   }
-  if (!p.part) return;  // uniform over the block
+  if (!p.part && !p.dbias) return;  // uniform over the block
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = sum[e];
   __syncthreads();
@@ -117,10 +118,9 @@ __global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] += red[(s * p.cw + in_row) * 8 + e];
   }
-  float* out = p.part + (int64_t)blockIdx.x * p.C + c;
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) out[e] = sum[e];
+  if (!p.dbias) st8<float, TAIL>(p.part, (int64_t)blockIdx.x * p.C + c, n, sum);
+  else if (p.bias_dt == kBF16) st8<bf16, TAIL>(p.dbias, c, n, sum);
+  else st8<float, TAIL>(p.dbias, c, n, sum);
 }
 
 }  // namespace hid

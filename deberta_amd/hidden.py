@@ -36,12 +36,11 @@ included).
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Union
+from typing import Any, Optional, Union
 
 import torch
 import torch.nn as nn
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from deberta_amd import _eager, _lib
 from deberta_amd.ops import draw_dropout_seed, dropout_threshold
@@ -54,15 +53,11 @@ FP8_MAX = 448.0  # the largest value of float8_e4m3fn
 MAX_RMS_WIDTH = 16384
 
 
-def _dt(t: Tensor, what: str) -> int:
+def _dt(t: Tensor, what: str, name: str) -> int:
     code = _DT.get(t.dtype)
     if code is None:
-        raise TypeError(f"{what}: dtype must be float32 or bfloat16, got {t.dtype}")
+        raise TypeError(f"{what} {name}: dtype must be float32 or bfloat16, got {t.dtype}")
     return code
-
-
-def _ptr(t: Optional[Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
@@ -85,21 +80,22 @@ def _res_layout(res: Tensor) -> tuple[Tensor, tuple[int, int], int]:
     return t, (0, stride), max(1, res.numel() // max(1, res.shape[-1]))
 
 
-def _vec(t: Optional[Tensor], C: int, what: str) -> Optional[Tensor]:
+def _vec(t: Optional[Tensor], C: int, what: str, name: str) -> Optional[Tensor]:
     if t is None:
         return None
-    if t.shape != (C,):
-        raise ValueError(f"{what} must have shape ({C},), got {tuple(t.shape)}")
+    if t.dim() != 1 or t.shape[0] != C:
+        raise ValueError(f"{what} {name} must have shape ({C},), got {tuple(t.shape)}")
     return t.contiguous()
 
 
-def _check(what: str, x: Tensor, **others: Optional[Tensor]) -> int:
+def _check(what: str, x: Tensor, *others: Optional[Tensor]) -> int:
     """x's width; the other tensors on x's device."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"{what}: x needs a last dimension of at least one column, got shape {tuple(x.shape)}")
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
+    device = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{what}: a tensor is on {t.device}, x is on {x.device}")
     return x.shape[-1]
 
 
@@ -109,23 +105,44 @@ def _same_shape(what: str, x: Tensor, res: Optional[Tensor]) -> None:
 
 
 def _stream_dtype(x: Tensor, res: Optional[Tensor]) -> torch.dtype:
-    return x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
+    if res is None or res.dtype is x.dtype:
+        return x.dtype
+    return torch.promote_types(x.dtype, res.dtype)
+
+
+_entries: dict[str, Any] = {}
 
 
 def _launch(entry: str, a: ctypes.Structure, t: Tensor) -> None:
-    """Calls a library entry point on the current stream of t's device."""
-    fn = getattr(_lib.load(), entry)
-    if t.device.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(a), ctypes.c_void_p(_eager.stream_ptr(t)))
+    """Calls a library entry point on the current stream of t's device (it
+    refuses a stream that is capturing a HIP graph)."""
+    fn = _entries.get(entry)
+    if fn is None:
+        fn = _entries[entry] = getattr(_lib.load(), entry)
+    if t.get_device() == torch.cuda.current_device():
+        rc = fn(a, _eager.stream_ptr(t))
     else:
         with torch.cuda.device(t.device):
-            rc = fn(ctypes.byref(a), ctypes.c_void_p(_eager.stream_ptr(t)))
-    _lib.check(rc, entry)
+            rc = fn(a, _eager.stream_ptr(t))
+    if rc:
+        _lib.check(rc, entry)
 
 
-def _workspace(kind: int, N: int, C: int, t: Tensor) -> Tensor:
+def _empty(like: Tensor, dtype: torch.dtype) -> Tensor:
+    """An uninitialised contiguous tensor of like's shape."""
+    if like.dtype is dtype and like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(like.shape, dtype=dtype, device=like.device)
+
+
+def _workspace(kind: int, N: int, C: int, t: Tensor) -> Optional[Tensor]:
     n = _lib.load().dsa_block_workspace_bytes(kind, N, C)
-    return torch.empty((n,), dtype=torch.uint8, device=t.device)
+    return torch.empty((n,), dtype=torch.uint8, device=t.device) if n else None
+
+
+def _needs_grad(*tensors: Optional[Tensor]) -> bool:
+    """Whether autograd records a call on these tensors."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # ---------------------------------------------------------------------------
@@ -202,23 +219,22 @@ def _hidden_dropout_impl(
     x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], dropout_t: int, dropout_seed: Optional[Tensor]
 ) -> Tensor:
     """``dropout(x + bias) + res`` in x's type promoted with res's."""
-    _eager.refuse_capture("deberta_amd::hidden_dropout")
     what = "hidden_dropout"
-    C = _check(what, x, bias=bias, res=res)
+    C = _check(what, x, bias, res)
     _same_shape(what, x, res)
-    x_dt, seed = _dt(x, f"{what} x"), _seed_value(dropout_seed, dropout_t)
+    x_dt, seed = _dt(x, what, "x"), _seed_value(dropout_seed, dropout_t)
     xr, xs = _rows(x)
-    bias = _vec(bias, C, f"{what} bias")
-    y = torch.empty(x.shape, dtype=_stream_dtype(x, res), device=x.device)
+    bias = _vec(bias, C, what, "bias")
+    y = _empty(x, _stream_dtype(x, res))
     N = x.numel() // C
     a = _lib.DsaDropoutArgs(
         x=xr.data_ptr(), x_stride=xs, x_dtype=x_dt, y=y.data_ptr(), y_stride=C, y_dtype=_DT.get(y.dtype, -1), N=N, C=C,
         threshold=dropout_t, seed=seed,
     )
     if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, f"{what} bias")
+        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, what, "bias")
     if res is not None:
-        a.res_dtype = _dt(res, f"{what} res")
+        a.res_dtype = _dt(res, what, "res")
         rr, a.res_strides, a.rows_per_group = _res_layout(res)
         a.res = rr.data_ptr()
     if N:
@@ -227,27 +243,26 @@ def _hidden_dropout_impl(
 
 
 def _hidden_dropout_bwd_impl(
-    dy: Tensor, dx_dtype: torch.dtype, bias: Optional[Tensor], dropout_t: int, dropout_seed: Optional[Tensor]
+    dy: Tensor, dx_dtype: torch.dtype, bias_dtype: Optional[torch.dtype], dropout_t: int, dropout_seed: Optional[Tensor]
 ) -> tuple[Tensor, Tensor]:
-    """(dx in ``dx_dtype``, dbias in the bias's type, empty without one)."""
-    _eager.refuse_capture("deberta_amd::hidden_dropout_bwd")
+    """(dx in ``dx_dtype``, dbias in ``bias_dtype``, empty where that is None)."""
     what = "hidden_dropout_bwd"
-    C = _check(what, dy, bias=bias)
+    C = _check(what, dy)
     dyr, dys = _rows(dy)
     N = dy.numel() // C
-    dx = torch.empty(dy.shape, dtype=dx_dtype, device=dy.device)
-    dbias = torch.empty_like(_vec(bias, C, f"{what} bias")) if bias is not None else dy.new_empty((0,))
+    dx = _empty(dy, dx_dtype)
+    dbias = torch.empty((0 if bias_dtype is None else C,), dtype=bias_dtype or dx_dtype, device=dy.device)
     a = _lib.DsaDropoutArgs(
-        dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, f"{what} dy"), dx=dx.data_ptr(), dx_stride=C,
-        dx_dtype=_dt(dx, f"{what} dx"), N=N, C=C, threshold=dropout_t, seed=_seed_value(dropout_seed, dropout_t),
+        dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, what, "dy"), dx=dx.data_ptr(), dx_stride=C,
+        dx_dtype=_dt(dx, what, "dx"), N=N, C=C, threshold=dropout_t, seed=_seed_value(dropout_seed, dropout_t),
     )
-    if bias is not None:
-        a.dbias, a.bias_dtype = dbias.data_ptr(), _dt(bias, f"{what} bias")
+    if bias_dtype is not None:
         if not N:
-            dbias.zero_()
-            return dx, dbias
+            return dx, dbias.zero_()
+        a.dbias, a.bias_dtype = dbias.data_ptr(), _dt(dbias, what, "bias")
         ws = _workspace(_lib.DSA_BLOCK_DROPOUT, N, C, dy)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        if ws is not None:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     if N:
         _launch("dsa_dropout_bwd", a, dy)
     return dx, dbias
@@ -267,33 +282,36 @@ def _hidden_dropout_fake(x, bias, res, dropout_t, dropout_seed):
 
 
 @hidden_dropout_bwd.register_fake
-def _hidden_dropout_bwd_fake(dy, dx_dtype, bias, dropout_t, dropout_seed):
-    return dy.new_empty(dy.shape, dtype=dx_dtype), bias.new_empty(bias.shape) if bias is not None else dy.new_empty((0,))
+def _hidden_dropout_bwd_fake(dy, dx_dtype, bias_dtype, dropout_t, dropout_seed):
+    dbias = dy.new_empty((0 if bias_dtype is None else dy.shape[-1],), dtype=bias_dtype or dx_dtype)
+    return dy.new_empty(dy.shape, dtype=dx_dtype), dbias
 
 
 def _hidden_dropout_setup(ctx, inputs, output):
     x, bias, res, dropout_t, seed = inputs
-    ctx.save_for_backward(bias, seed)
+    ctx.save_for_backward(seed)
     ctx.dropout_t, ctx.x_dtype = dropout_t, x.dtype
+    ctx.bias_dtype = None if bias is None else bias.dtype
     ctx.res_dtype = None if res is None else res.dtype
+    ctx.op_in_graph = True
 
 
 def _hidden_dropout_backward(ctx, dy):
-    bias, seed = ctx.saved_tensors
+    (seed,) = ctx.saved_tensors
     dx = dbias = dres = None
-    with_bias = bias is not None and ctx.needs_input_grad[1]
-    if ctx.needs_input_grad[0] or with_bias:
+    for_x, for_bias, for_res = ctx.needs_input_grad[:3]
+    if for_x or for_bias:
         dx, dbias = _eager.on_eager(ctx, hidden_dropout_bwd, _hidden_dropout_bwd_impl)(
-            dy, ctx.x_dtype, bias if with_bias else None, ctx.dropout_t, seed
+            dy, ctx.x_dtype, ctx.bias_dtype if for_bias else None, ctx.dropout_t, seed
         )
-    if ctx.res_dtype is not None and ctx.needs_input_grad[2]:
-        dres = dy.to(ctx.res_dtype)
-    return dx, (dbias if with_bias else None), dres, None, None
+    if for_res:
+        dres = dy if dy.dtype is ctx.res_dtype else dy.to(ctx.res_dtype)
+    return dx, (dbias if for_bias else None), dres, None, None
 
 
 torch.library.register_autograd("deberta_amd::hidden_dropout", _hidden_dropout_backward, setup_context=_hidden_dropout_setup)
 _HiddenDropoutFunction = _eager.function(
-    "_HiddenDropoutFunction", _hidden_dropout_impl, _hidden_dropout_setup, once_differentiable(_hidden_dropout_backward)
+    "_HiddenDropoutFunction", _hidden_dropout_impl, _hidden_dropout_setup, _hidden_dropout_backward
 )
 
 
@@ -319,11 +337,12 @@ def fused_dropout(
         return x
     s = _seed_tensor(seed) if t else None
     if x.device.type != "cuda":
-        C = _check("fused_dropout", x, bias=bias, res=res)
+        C = _check("fused_dropout", x, bias, res)
         _same_shape("fused_dropout", x, res)
-        return _cpu_sum(x, _vec(bias, C, "fused_dropout bias"), res, t, s).to(_stream_dtype(x, res))
+        return _cpu_sum(x, _vec(bias, C, "fused_dropout", "bias"), res, t, s).to(_stream_dtype(x, res))
     if _eager.eager(x):
-        return _HiddenDropoutFunction.apply(x, bias, res, t, s)
+        run = _HiddenDropoutFunction.apply if _needs_grad(x, bias, res) else _hidden_dropout_impl
+        return run(x, bias, res, t, s)
     return torch.ops.deberta_amd.hidden_dropout(x, bias, res, t, s)
 
 
@@ -335,22 +354,22 @@ def _fill_rms(
     what: str, x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], weight: Tensor, dropout_t: int, seed: Optional[Tensor]
 ) -> tuple[_lib.DsaRmsArgs, tuple]:
     """The arguments every form shares, and the tensors they point into."""
-    C = _check(what, x, bias=bias, res=res, weight=weight)
+    C = _check(what, x, bias, res, weight)
     if C > MAX_RMS_WIDTH:
         raise ValueError(f"{what}: rows of at most {MAX_RMS_WIDTH} columns, got {C}")
     _same_shape(what, x, res)
-    bias, weight = _vec(bias, C, f"{what} bias"), _vec(weight, C, f"{what} weight")
+    bias, weight = _vec(bias, C, what, "bias"), _vec(weight, C, what, "weight")
     xr, xs = _rows(x)
     a = _lib.DsaRmsArgs(
-        x=xr.data_ptr(), x_stride=xs, x_dtype=_dt(x, f"{what} x"), weight=weight.data_ptr(),
-        weight_dtype=_dt(weight, f"{what} weight"), N=x.numel() // C, C=C, threshold=dropout_t,
+        x=xr.data_ptr(), x_stride=xs, x_dtype=_dt(x, what, "x"), weight=weight.data_ptr(),
+        weight_dtype=_dt(weight, what, "weight"), N=x.numel() // C, C=C, threshold=dropout_t,
         seed=_seed_value(seed, dropout_t),
     )
     rr = None
     if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, f"{what} bias")
+        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, what, "bias")
     if res is not None:
-        a.res_dtype = _dt(res, f"{what} res")
+        a.res_dtype = _dt(res, what, "res")
         rr, a.res_strides, a.rows_per_group = _res_layout(res)
         a.res = rr.data_ptr()
     return a, (xr, bias, weight, rr)
@@ -373,14 +392,14 @@ def _add_rms_norm_impl(
 ) -> tuple[Tensor, Tensor, Tensor]:
     """(y in ``out_dtype``, z = dropout(x + bias) + res, 1 / rms per row); z is
     empty where it is x itself."""
-    _eager.refuse_capture("deberta_amd::add_rms_norm")
     a, keep = _fill_rms("add_rms_norm", x, bias, res, weight, dropout_t, dropout_seed)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    z = torch.empty((0,) if _plain(bias, res, dropout_t) else x.shape, dtype=_stream_dtype(x, res), device=x.device)
+    y, z_dtype = _empty(x, out_dtype), _stream_dtype(x, res)
+    plain = _plain(bias, res, dropout_t)
+    z = torch.empty((0,), dtype=z_dtype, device=x.device) if plain else _empty(x, z_dtype)
     rstd = torch.empty((a.N,), dtype=torch.float32, device=x.device)
-    a.y, a.y_stride, a.y_dtype, a.rstd, a.eps = y.data_ptr(), a.C, _dt(y, "add_rms_norm y"), rstd.data_ptr(), eps
+    a.y, a.y_stride, a.y_dtype, a.rstd, a.eps = y.data_ptr(), a.C, _dt(y, "add_rms_norm", "y"), rstd.data_ptr(), eps
     if a.N:
-        if z.numel():
+        if not plain:
             a.z, a.z_stride = z.data_ptr(), a.C
         _launch("dsa_add_rms_fwd", a, x)
     return y, z, rstd
@@ -400,20 +419,19 @@ def _add_rms_norm_bwd_impl(
     """(dx, dres, dweight, dbias) for the gradients of y and (optional) of z.
     dres is empty without a residual and where it equals dx (no dropout, one
     type); dbias is empty without a bias."""
-    _eager.refuse_capture("deberta_amd::add_rms_norm_bwd")
     what = "add_rms_norm_bwd"
     a, keep = _fill_rms(what, x, bias, res, weight, dropout_t, dropout_seed)
-    _check(what, x, dy=dy, dz=dz, rstd=rstd)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _check(what, x, dy, dz, rstd)
+    dx = _empty(x, x.dtype)
     apart = res is not None and (dropout_t or res.dtype != x.dtype)
-    dres = torch.empty(x.shape if apart else (0,), dtype=x.dtype if res is None else res.dtype, device=x.device)
+    dres = _empty(x, res.dtype) if apart else torch.empty((0,), dtype=x.dtype, device=x.device)
     dweight = torch.empty_like(keep[2])
     dbias = torch.empty_like(keep[1]) if bias is not None else weight.new_empty((0,))
     if not a.N:
         dweight.zero_(), dbias.zero_()
         return dx, dres, dweight, dbias
     dyr, a.dy_stride = _rows(dy)
-    a.dy, a.dy_dtype, a.rstd = dyr.data_ptr(), _dt(dy, f"{what} dy"), rstd.data_ptr()
+    a.dy, a.dy_dtype, a.rstd = dyr.data_ptr(), _dt(dy, what, "dy"), rstd.data_ptr()
     if dz is not None:
         dzr, a.dzu_stride = _rows(dz if dz.dtype == _stream_dtype(x, res) else dz.to(_stream_dtype(x, res)))
         a.dzu = dzr.data_ptr()
@@ -424,7 +442,8 @@ def _add_rms_norm_bwd_impl(
     if bias is not None:
         a.dbias = dbias.data_ptr()
     ws = _workspace(_lib.DSA_BLOCK_RMS, a.N, a.C, x)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _launch("dsa_add_rms_bwd", a, x)
     return dx, dres, dweight, dbias
 
@@ -434,16 +453,16 @@ def _add_rms_norm_quant_impl(
 ) -> tuple[Tensor, Tensor, Tensor]:
     """(y as float8_e4m3fn, its scales, z); z is empty where it is x itself.
     ``group_size`` 0: one scale a row."""
-    _eager.refuse_capture("deberta_amd::add_rms_norm_quant")
     a, keep = _fill_rms("add_rms_norm_quant", x, bias, res, weight, 0, None)
     _check_group(a.C, group_size)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     groups = a.C // group_size if group_size else 1
     scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device)
-    z = torch.empty((0,) if _plain(bias, res, 0) else x.shape, dtype=_stream_dtype(x, res), device=x.device)
+    plain, z_dtype = _plain(bias, res, 0), _stream_dtype(x, res)
+    z = torch.empty((0,), dtype=z_dtype, device=x.device) if plain else _empty(x, z_dtype)
     a.y, a.y_stride, a.scales, a.group_size, a.eps = q.data_ptr(), a.C, scales.data_ptr(), group_size, eps
     if a.N:
-        if z.numel():
+        if not plain:
             a.z, a.z_stride = z.data_ptr(), a.C
         _launch("dsa_add_rms_quant", a, x)
     return q, scales, z
@@ -471,7 +490,7 @@ def _add_rms_norm_bwd_fake(dy, dz, x, bias, res, weight, rstd, dropout_t, dropou
     apart = res is not None and (dropout_t or res.dtype != x.dtype)
     return (
         x.new_empty(x.shape),
-        x.new_empty(x.shape if apart else (0,), dtype=x.dtype if res is None else res.dtype),
+        x.new_empty(x.shape if apart else (0,), dtype=res.dtype if apart else x.dtype),
         weight.new_empty(weight.shape),
         bias.new_empty(bias.shape) if bias is not None else weight.new_empty((0,)),
     )
@@ -494,6 +513,7 @@ def _add_rms_norm_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(*((rstd, z) if _plain(bias, res, dropout_t) else (rstd,)))
     ctx.save_for_backward(x, bias, res, weight, rstd, seed)
     ctx.dropout_t, ctx.out_dtype = dropout_t, out_dtype
+    ctx.op_in_graph = True
     ctx.set_materialize_grads(False)
 
 
@@ -515,7 +535,7 @@ def _add_rms_norm_backward(ctx, dy, dz, drstd):
 
 torch.library.register_autograd("deberta_amd::add_rms_norm", _add_rms_norm_backward, setup_context=_add_rms_norm_setup)
 _AddRmsNormFunction = _eager.function(
-    "_AddRmsNormFunction", _add_rms_norm_impl, _add_rms_norm_setup, once_differentiable(_add_rms_norm_backward)
+    "_AddRmsNormFunction", _add_rms_norm_impl, _add_rms_norm_setup, _add_rms_norm_backward
 )
 
 
@@ -551,13 +571,14 @@ def fused_add_rms_norm(
     s = _seed_tensor(seed) if t else None
     out_dtype = norm_out_dtype(x, res) if out_dtype is None else out_dtype
     if x.device.type != "cuda":
-        C = _check("fused_add_rms_norm", x, bias=bias, res=res, weight=weight)
+        C = _check("fused_add_rms_norm", x, bias, res, weight)
         _same_shape("fused_add_rms_norm", x, res)
-        z = _cpu_sum(x, _vec(bias, C, "bias"), res, t, s)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "weight").float()
+        z = _cpu_sum(x, _vec(bias, C, "fused_add_rms_norm", "bias"), res, t, s)
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "fused_add_rms_norm", "weight").float()
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
-        y, z, _ = _AddRmsNormFunction.apply(x, bias, res, weight, float(eps), out_dtype, t, s)
+        run = _AddRmsNormFunction.apply if _needs_grad(x, bias, res, weight) else _add_rms_norm_impl
+        y, z, _ = run(x, bias, res, weight, float(eps), out_dtype, t, s)
     else:
         y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
     return y, (x if _plain(bias, res, t) else z)
@@ -593,16 +614,16 @@ def fused_add_rms_norm_fp8(
     infinity has the scale NaN and q NaN.  For serving: there is no gradient,
     and a call under autograd whose inputs need one raises."""
     g = 0 if group_size is None else int(group_size)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
+    if _needs_grad(x, weight, bias, res):
         raise RuntimeError("fused_add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if group_size is not None and g == 0:
         raise ValueError("group_size must be 32, 64, 128, 256 or 512, or None for one scale a row")
     if x.device.type != "cuda":
-        C = _check("fused_add_rms_norm_fp8", x, bias=bias, res=res, weight=weight)
+        C = _check("fused_add_rms_norm_fp8", x, bias, res, weight)
         _same_shape("fused_add_rms_norm_fp8", x, res)
         _check_group(C, g)
-        z = _cpu_sum(x, _vec(bias, C, "bias"), res, 0, None)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "weight").float()
+        z = _cpu_sum(x, _vec(bias, C, "fused_add_rms_norm", "bias"), res, 0, None)
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "fused_add_rms_norm", "weight").float()
         y = y.unflatten(-1, (C // (g or C), g or C))
         top = y.abs().amax(-1, keepdim=True)
         scale = torch.where(top < FP8_MAX * 2.0**-126, 1.0, top / FP8_MAX)
@@ -630,16 +651,15 @@ def _embed_impl(ids: Tensor, weight: Tensor, padding_idx: int, scale: float, out
     """``scale * weight[ids]`` in ``out_dtype``; a row of NaN where an id is
     outside the table.  ``padding_idx`` (-1: none) matters to the gradient
     only."""
-    _eager.refuse_capture("deberta_amd::embed")
     if weight.dim() != 2 or not weight.shape[0]:
         raise ValueError(f"embed: weight must be (V, C) with V >= 1, got shape {tuple(weight.shape)}")
-    C = _check("embed", weight, ids=ids)
+    C = _check("embed", weight, ids)
     idr, nb = _ids_rows(ids)
     wr, ws = _rows(weight)
     y = torch.empty((*ids.shape, C), dtype=out_dtype, device=ids.device)
     a = _lib.DsaEmbedArgs(
-        ids=idr.data_ptr(), ids_bytes=nb, weight=wr.data_ptr(), weight_stride=ws, weight_dtype=_dt(weight, "embed weight"),
-        y=y.data_ptr(), y_stride=C, y_dtype=_dt(y, "embed y"), N=ids.numel(), V=weight.shape[0], C=C, padding=padding_idx,
+        ids=idr.data_ptr(), ids_bytes=nb, weight=wr.data_ptr(), weight_stride=ws, weight_dtype=_dt(weight, "embed", "weight"),
+        y=y.data_ptr(), y_stride=C, y_dtype=_dt(y, "embed", "y"), N=ids.numel(), V=weight.shape[0], C=C, padding=padding_idx,
         scale=scale,
     )
     if a.N:
@@ -651,8 +671,7 @@ def _embed_bwd_impl(
     dy: Tensor, ids: Tensor, num_embeddings: int, weight_dtype: torch.dtype, padding_idx: int, scale: float
 ) -> Tensor:
     """The gradient of the whole table, in ``weight_dtype``."""
-    _eager.refuse_capture("deberta_amd::embed_bwd")
-    C = _check("embed_bwd", dy, ids=ids)
+    C = _check("embed_bwd", dy, ids)
     if dy.shape[:-1] != ids.shape:
         raise ValueError(f"embed_bwd: dy must have the shape {(*ids.shape, C)}, got {tuple(dy.shape)}")
     idr, nb = _ids_rows(ids)
@@ -665,8 +684,8 @@ def _embed_bwd_impl(
     nws = lib.dsa_embed_workspace_bytes(N, C, num_embeddings)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dy.device)
     a = _lib.DsaEmbedArgs(
-        ids=idr.data_ptr(), ids_bytes=nb, dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, "embed_bwd dy"),
-        dweight=dw.data_ptr(), weight_dtype=_dt(dw, "embed_bwd weight"), N=N, V=num_embeddings, C=C, padding=padding_idx,
+        ids=idr.data_ptr(), ids_bytes=nb, dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, "embed_bwd", "dy"),
+        dweight=dw.data_ptr(), weight_dtype=_dt(dw, "embed_bwd", "weight"), N=N, V=num_embeddings, C=C, padding=padding_idx,
         scale=scale, workspace=ws.data_ptr(), workspace_bytes=nws,
     )
     _launch("dsa_embed_bwd", a, dy)
@@ -690,6 +709,7 @@ def _embed_bwd_fake(dy, ids, num_embeddings, weight_dtype, padding_idx, scale):
 def _embed_setup(ctx, inputs, output):
     ids, weight, padding_idx, scale, _ = inputs
     ctx.save_for_backward(ids)
+    ctx.op_in_graph = True
     ctx.table = (weight.shape[0], weight.dtype, padding_idx, scale)
 
 
@@ -699,7 +719,7 @@ def _embed_backward(ctx, dy):
 
 
 torch.library.register_autograd("deberta_amd::embed", _embed_backward, setup_context=_embed_setup)
-_EmbedFunction = _eager.function("_EmbedFunction", _embed_impl, _embed_setup, once_differentiable(_embed_backward))
+_EmbedFunction = _eager.function("_EmbedFunction", _embed_impl, _embed_setup, _embed_backward)
 
 
 def fused_embedding(
@@ -732,7 +752,8 @@ def fused_embedding(
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
         return (y.float() * scale).to(out_dtype)
     if _eager.eager(weight):
-        return _EmbedFunction.apply(ids, weight, pad, float(scale), out_dtype)
+        run = _EmbedFunction.apply if _needs_grad(weight) else _embed_impl
+        return run(ids, weight, pad, float(scale), out_dtype)
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)
 
 

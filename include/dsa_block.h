@@ -145,7 +145,8 @@ typedef struct dsa_dropout_args {
   void* dx;                   /* backward: [N, C], row stride dx_stride, or NULL */
   int64_t dx_stride;
   void* dbias;                /* backward: [C] or NULL, written: the column sums of dx */
-  void* workspace;            /* backward with dbias: dsa_block_workspace_bytes(DSA_BLOCK_DROPOUT, N, C) bytes */
+  void* workspace;            /* backward with dbias: dsa_block_workspace_bytes(DSA_BLOCK_DROPOUT, N, C) bytes
+                                 (none for few rows) */
   size_t workspace_bytes;
   uint64_t seed;
   int64_t N;                  /* at most 2^31 - 1 */
