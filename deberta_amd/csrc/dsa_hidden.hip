@@ -158,7 +158,7 @@ int check_rms(const dsa_rms_args* a, bool quant, bool bwd) {
   if (!res_ok(a->res, a->res_strides, a->rows_per_group, a->res_dtype)) return fail("dsa_add_rms: bad res");
   if (a->bias && !vec_given(a->bias, a->bias_dtype)) return fail("dsa_add_rms: bad bias");
   if (!vec_given(a->weight, a->weight_dtype)) return fail("dsa_add_rms: bad weight");
-  if (!quant && !a->rstd) return fail("dsa_add_rms: rstd is required");
+  if (bwd && !a->rstd) return fail("dsa_add_rms: rstd is required");
   if (!bwd) {
     if (!a->y || a->y_stride < a->C) return fail("dsa_add_rms: bad y");
     if (!quant && !rows_given(a->y, a->y_stride, a->y_dtype)) return fail("dsa_add_rms: bad y");

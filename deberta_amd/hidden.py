@@ -142,7 +142,11 @@ def _workspace(kind: int, N: int, C: int, t: Tensor) -> Optional[Tensor]:
 
 def _needs_grad(*tensors: Optional[Tensor]) -> bool:
     """Whether autograd records a call on these tensors."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------
@@ -336,7 +340,7 @@ def fused_dropout(
     if not t and bias is None and res is None:
         return x
     s = _seed_tensor(seed) if t else None
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         C = _check("fused_dropout", x, bias, res)
         _same_shape("fused_dropout", x, res)
         return _cpu_sum(x, _vec(bias, C, "fused_dropout", "bias"), res, t, s).to(_stream_dtype(x, res))
@@ -380,6 +384,34 @@ def _plain(bias: Optional[Tensor], res: Optional[Tensor], dropout_t: int) -> boo
     return bias is None and res is None and not dropout_t
 
 
+def _rms_forward(
+    x: Tensor,
+    bias: Optional[Tensor],
+    res: Optional[Tensor],
+    weight: Tensor,
+    eps: float,
+    out_dtype: torch.dtype,
+    dropout_t: int,
+    dropout_seed: Optional[Tensor],
+    rstd: Optional[Tensor] = None,
+) -> tuple[Tensor, Tensor]:
+    """(y in ``out_dtype``, z = dropout(x + bias) + res); z is x where there is
+    nothing to add or drop.  1 / rms per row goes to ``rstd``."""
+    a, keep = _fill_rms("add_rms_norm", x, bias, res, weight, dropout_t, dropout_seed)
+    C = a.C
+    y = _empty(x, out_dtype)
+    a.y, a.y_stride, a.y_dtype, a.eps = y.data_ptr(), C, _dt(y, "add_rms_norm", "y"), eps
+    z = x
+    if not _plain(bias, res, dropout_t):
+        z = _empty(x, _stream_dtype(x, res))
+        a.z, a.z_stride = z.data_ptr(), C
+    if rstd is not None:
+        a.rstd = rstd.data_ptr()
+    if a.N:
+        _launch("dsa_add_rms_fwd", a, x)
+    return y, z
+
+
 def _add_rms_norm_impl(
     x: Tensor,
     bias: Optional[Tensor],
@@ -392,17 +424,10 @@ def _add_rms_norm_impl(
 ) -> tuple[Tensor, Tensor, Tensor]:
     """(y in ``out_dtype``, z = dropout(x + bias) + res, 1 / rms per row); z is
     empty where it is x itself."""
-    a, keep = _fill_rms("add_rms_norm", x, bias, res, weight, dropout_t, dropout_seed)
-    y, z_dtype = _empty(x, out_dtype), _stream_dtype(x, res)
-    plain = _plain(bias, res, dropout_t)
-    z = torch.empty((0,), dtype=z_dtype, device=x.device) if plain else _empty(x, z_dtype)
-    rstd = torch.empty((a.N,), dtype=torch.float32, device=x.device)
-    a.y, a.y_stride, a.y_dtype, a.rstd, a.eps = y.data_ptr(), a.C, _dt(y, "add_rms_norm", "y"), rstd.data_ptr(), eps
-    if a.N:
-        if not plain:
-            a.z, a.z_stride = z.data_ptr(), a.C
-        _launch("dsa_add_rms_fwd", a, x)
-    return y, z, rstd
+    rows = x.numel() // max(1, x.shape[-1]) if x.dim() else 0
+    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    y, z = _rms_forward(x, bias, res, weight, eps, out_dtype, dropout_t, dropout_seed, rstd)
+    return y, (x.new_empty((0,)) if z is x else z), rstd
 
 
 def _add_rms_norm_bwd_impl(
@@ -570,15 +595,16 @@ def fused_add_rms_norm(
     t = _threshold(dropout_p) if training else 0
     s = _seed_tensor(seed) if t else None
     out_dtype = norm_out_dtype(x, res) if out_dtype is None else out_dtype
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         C = _check("fused_add_rms_norm", x, bias, res, weight)
         _same_shape("fused_add_rms_norm", x, res)
         z = _cpu_sum(x, _vec(bias, C, "fused_add_rms_norm", "bias"), res, t, s)
         y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "fused_add_rms_norm", "weight").float()
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
-        run = _AddRmsNormFunction.apply if _needs_grad(x, bias, res, weight) else _add_rms_norm_impl
-        y, z, _ = run(x, bias, res, weight, float(eps), out_dtype, t, s)
+        if not _needs_grad(x, bias, res, weight):
+            return _rms_forward(x, bias, res, weight, float(eps), out_dtype, t, s)
+        y, z, _ = _AddRmsNormFunction.apply(x, bias, res, weight, float(eps), out_dtype, t, s)
     else:
         y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
     return y, (x if _plain(bias, res, t) else z)
@@ -618,7 +644,7 @@ def fused_add_rms_norm_fp8(
         raise RuntimeError("fused_add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if group_size is not None and g == 0:
         raise ValueError("group_size must be 32, 64, 128, 256 or 512, or None for one scale a row")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         C = _check("fused_add_rms_norm_fp8", x, bias, res, weight)
         _same_shape("fused_add_rms_norm_fp8", x, res)
         _check_group(C, g)
@@ -747,7 +773,7 @@ def fused_embedding(
             raise ValueError(f"fused_embedding: padding_idx {padding_idx} is outside the table of {V} rows")
         pad = padding_idx % V
     out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if weight.device.type != "cuda":
+    if not weight.is_cuda:
         _ids_rows(ids)
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
         return (y.float() * scale).to(out_dtype)

@@ -169,7 +169,7 @@ typedef struct dsa_rms_args {
   void* z;                    /* [N, C] dropout(x + bias) + res, row stride z_stride, or NULL: float32 unless x
                                  and res are both bf16 */
   int64_t z_stride;
-  float* rstd;                /* [N]: 1 / sqrt(mean(z^2) + eps); the quantized form may pass NULL */
+  float* rstd;                /* [N]: 1 / sqrt(mean(z^2) + eps); a forward may pass NULL */
   float* scales;              /* quantized form: [N, group_size ? C / group_size : 1] */
   const void* dy;             /* backward: [N, C], row stride dy_stride */
   int64_t dy_stride;

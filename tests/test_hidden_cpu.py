@@ -231,7 +231,7 @@ def test_rms_entry_refuses():
     for entry, change, match in (
         ("dsa_add_rms_fwd", dict(C=16385), r"C in \[1, 16384\]"),
         ("dsa_add_rms_fwd", dict(weight=None), "bad weight"),
-        ("dsa_add_rms_fwd", dict(rstd=None), "rstd"),
+        ("dsa_add_rms_bwd", dict(dy=at, dy_stride=64, rstd=None), "rstd"),
         ("dsa_add_rms_fwd", dict(y_stride=63), "bad y"),
         ("dsa_add_rms_fwd", dict(z_stride=63), "bad z"),
         ("dsa_add_rms_fwd", dict(threshold=70000), "threshold"),
