@@ -42,24 +42,6 @@ DSA_EXTERN(float, 64)
 DSA_EXTERN(float, 32)
 #undef DSA_EXTERN
 
-int reduce_cols(const float* part, int64_t nparts, int64_t stride, int K, int nout, const int64_t* off, void* const* out,
-                const int* dt, hipStream_t st) {
-  dsa::rows::ReduceCols rc;
-  rc.part = part;
-  rc.nparts = nparts;
-  rc.stride = stride;
-  rc.K = K;
-  rc.nout = nout;
-  for (int j = 0; j < 3; ++j) {
-    rc.off[j] = j < nout ? off[j] : 0;
-    rc.out[j] = j < nout ? out[j] : nullptr;
-    rc.dt[j] = j < nout ? dt[j] : 0;
-  }
-  hipLaunchKernelGGL(dsa::rows::reduce_cols_kernel, dim3((unsigned)cdiv(K, 64), (unsigned)nout), dim3(64 * dsa::rows::RED_W), 0,
-                     st, rc);
-  return launch_check("reduce_cols_kernel");
-}
-
 // dsa_hidden.hip
 size_t drop_workspace(int64_t N, int C);
 size_t rms_workspace(int64_t N, int C);
@@ -282,6 +264,24 @@ bool rows_ok(const void* p, int64_t stride, int dt) {
   return p && (reinterpret_cast<uintptr_t>(p) % a) == 0 && stride % 4 == 0;
 }
 bool vec_ok(const void* p, int dt) { return !p || (reinterpret_cast<uintptr_t>(p) % (4u * (uintptr_t)elem_bytes(dt))) == 0; }
+
+int reduce_cols(const float* part, int64_t nparts, int64_t stride, int K, int nout, const int64_t* off, void* const* out,
+                int dt, hipStream_t st) {
+  dsa::rows::ReduceCols rc;
+  rc.part = part;
+  rc.nparts = nparts;
+  rc.stride = stride;
+  rc.K = K;
+  rc.nout = nout;
+  for (int j = 0; j < 3; ++j) {
+    rc.off[j] = j < nout ? off[j] : 0;
+    rc.out[j] = j < nout ? out[j] : nullptr;
+  }
+  rc.dt = dt;
+  hipLaunchKernelGGL(dsa::rows::reduce_cols_kernel, dim3((unsigned)cdiv(K, 64), (unsigned)nout), dim3(64 * dsa::rows::RED_W), 0,
+                     st, rc);
+  return launch_check("reduce_cols_kernel");
+}
 
 int check_ln(const dsa_ln_args* a, bool bwd) {
   if (!a) return fail("dsa: null arguments");
@@ -719,8 +719,7 @@ int dsa_add_ln_bwd(const dsa_ln_args* a, void* stream) {
   if (launch_check("ln_bwd_kernel")) return 1;
   const int64_t off[3] = {0, a->C, 2 * (int64_t)a->C};
   void* const out[3] = {a->dgamma, a->dbeta, a->dbias};
-  const int dt[3] = {a->param_dtype, a->param_dtype, a->param_dtype};
-  return reduce_cols(p.part, nb, 3 * (int64_t)a->C, a->C, 3, off, out, dt, st);
+  return reduce_cols(p.part, nb, 3 * (int64_t)a->C, a->C, 3, off, out, a->param_dtype, st);
 }
 
 int dsa_bias_gelu_fwd(const dsa_gelu_args* a, void* stream) {
@@ -772,7 +771,7 @@ int dsa_bias_gelu_bwd(const dsa_gelu_args* a, void* stream) {
   if (!a->dbias) return 0;
   const int64_t off[1] = {0};
   void* const out[1] = {a->dbias};
-  return reduce_cols(p.part, nb, a->C, a->C, 1, off, out, &a->param_dtype, st);
+  return reduce_cols(p.part, nb, a->C, a->C, 1, off, out, a->param_dtype, st);
 }
 
 int dsa_rtd_loss_fwd(const dsa_rtd_args* a, void* stream) {
@@ -812,8 +811,8 @@ int dsa_rtd_loss_bwd(const dsa_rtd_args* a, void* stream) {
   const int64_t off_w[1] = {0}, off_b[1] = {a->C};
   void* const out_w[1] = {a->dw};
   void* const out_b[1] = {a->db};
-  if (reduce_cols(p.part, nb, a->C + 1, a->C, 1, off_w, out_w, &a->param_dtype, st)) return 1;
-  return a->db ? reduce_cols(p.part, nb, a->C + 1, 1, 1, off_b, out_b, &a->param_dtype, st) : 0;
+  if (reduce_cols(p.part, nb, a->C + 1, a->C, 1, off_w, out_w, a->param_dtype, st)) return 1;
+  return a->db ? reduce_cols(p.part, nb, a->C + 1, 1, 1, off_b, out_b, a->param_dtype, st) : 0;
 }
 
 }  // extern "C"

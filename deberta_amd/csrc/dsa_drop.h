@@ -16,6 +16,7 @@ namespace dsa {
 namespace hid {
 
 constexpr int DROP_T = 256;  // chunks (threads) a block takes at most
+constexpr int DROP_SUM_T = 512;  // the same of a backward with dbias: larger blocks leave fewer partial sums
 constexpr int DROP_U = 4;    // rows whose loads are issued together
 
 struct DropRows {
@@ -33,7 +34,7 @@ struct DropRows {
 
 template <typename TX, typename TR, typename TY, bool TAIL>
 __global__ __launch_bounds__(DROP_T) void drop_fwd_kernel(DropRows p) {
-  const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * DROP_T + (int)threadIdx.x - sub * p.cw;
+  const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * p.cw + (int)threadIdx.x - sub * p.cw;
   const int c = 8 * chunk, n = p.C - c;
   if (sub >= p.subs || n <= 0) return;  // all others: eight columns, or the row's last
   float bias[8];
@@ -76,9 +77,9 @@ __global__ __launch_bounds__(DROP_T) void drop_fwd_kernel(DropRows p) {
 // dx and, where part or dbias is given, the block's column sums of it: the sums
 // of a thread's rows, then of the block's row groups in their order.
 template <typename TDY, typename TX, bool TAIL>
-__global__ __launch_bounds__(DROP_T) void drop_bwd_kernel(DropRows p) {
-  __shared__ float red[DROP_T * 8];
-  const int sub = threadIdx.x / p.cw, in_row = (int)threadIdx.x - sub * p.cw, chunk = blockIdx.y * DROP_T + in_row;
+__global__ __launch_bounds__(DROP_SUM_T) void drop_bwd_kernel(DropRows p) {
+  __shared__ float red[DROP_SUM_T * 8];
+  const int sub = threadIdx.x / p.cw, in_row = (int)threadIdx.x - sub * p.cw, chunk = blockIdx.y * p.cw + in_row;
   const int c = 8 * chunk, n = sub < p.subs ? p.C - c : 0;
   const int64_t r0 = (int64_t)blockIdx.x * p.rows * p.subs + sub;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

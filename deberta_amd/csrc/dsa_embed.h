@@ -65,7 +65,7 @@ DSA_DEV int64_t ld_id(const void* ids, int64_t i, int ids64) {
 // gives a row of NaN.
 template <typename TW, typename TY, bool NARROW>
 __global__ __launch_bounds__(EMB_T) void embed_fwd_kernel(EmbedRows p) {
-  const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * EMB_T + (int)threadIdx.x - sub * p.cw;
+  const int sub = threadIdx.x / p.cw, chunk = blockIdx.y * p.cw + (int)threadIdx.x - sub * p.cw;
   const int c = embed_col<NARROW>(p.C, 8 * chunk), n = p.C - c;
   if (sub >= p.subs || 8 * chunk >= p.C) return;
   const int64_t extent = (p.V - 1) * p.ws + p.C;

@@ -61,20 +61,27 @@ DSA_DEV void cvt8(const raw8<T>& r, int n, float (&v)[8]) {
   }
 }
 
+// Stores the first n of eight values (n <= 0: none).  Where n is below eight
+// it is the same in every lane that has such a chunk: C % 8.
 template <typename T, bool TAIL>
 DSA_DEV void st8(void* base, int64_t off, int n, const float (&v)[8]) {
   if (n <= 0) return;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  typedef T v2 __attribute__((ext_vector_type(2)));
+  typedef v4 v4u __attribute__((aligned(sizeof(T))));
+  typedef v2 v2u __attribute__((aligned(sizeof(T))));
   T* p = static_cast<T*>(base) + off;
   raw8<T> r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
   if (!TAIL || n >= 8) {
     *reinterpret_cast<typename Raw8<T>::v8u*>(p) = r;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (e < n) p[e] = r[e];
+    return;
   }
+  const int u = __builtin_amdgcn_readfirstlane(n);
+  if (u & 4) *reinterpret_cast<v4u*>(p) = v4{r[0], r[1], r[2], r[3]};
+  if (u & 2) *reinterpret_cast<v2u*>(p + (u & 4)) = u & 4 ? v2{r[4], r[5]} : v2{r[0], r[1]};
+  if (u & 1) p[u - 1] = u & 4 ? (u & 2 ? r[6] : r[4]) : (u & 2 ? r[2] : r[0]);
 }
 
 // A parameter vector's chunk, its type known at run time (read once a block
@@ -142,13 +149,58 @@ DSA_DEV float dpp(float x) {
 DSA_DEV float lane_value(float x, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
-// The sum of x over the wave, in a fixed order, in every lane.
-DSA_DEV float wave_sum(float x) {
+// The sum of x over each L neighbouring lanes, in a fixed order, in every lane.
+template <int L>
+DSA_DEV float lanes_sum(float x) {
+  static_assert(L == 16 || L == 32 || L == 64, "");
   x += dpp<0xB1>(x);   // quad_perm [1, 0, 3, 2]
   x += dpp<0x4E>(x);   // quad_perm [2, 3, 0, 1]
   x += dpp<0x141>(x);  // row_half_mirror: the other quad of eight lanes
   x += dpp<0x140>(x);  // row_mirror: the other eight of sixteen
-  return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+  if constexpr (L == 32) x += __shfl_xor(x, 16);
+  if constexpr (L == 64) x = (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// out[j][c] = sum over i < nparts of part[i * stride + j * C + c].  A block
+// takes SUM_C columns (one line of each part) in SUM_G groups: group g sums
+// parts g, g + SUM_G, ... into eight independent sums (eight loads in
+// flight), then the groups' sums are added in their order, so the result
+// does not depend on scheduling.
+constexpr int SUM_C = 32, SUM_G = 32;
+
+struct SumParts {
+  const float* part;
+  int64_t nparts, stride;
+  int C;
+  void* out[2];
+  int dt[2];
+};
+
+static __global__ __launch_bounds__(SUM_C * SUM_G) void sum_parts_kernel(SumParts p) {
+  __shared__ float red[SUM_G][SUM_C + 1];
+  const int col = threadIdx.x % SUM_C, g = threadIdx.x / SUM_C, j = blockIdx.y;
+  if (!p.out[j]) return;  // uniform over the block
+  const int c = blockIdx.x * SUM_C + col;
+  const float* base = p.part + (int64_t)j * p.C + min(c, p.C - 1);
+  float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int64_t i = g; i < p.nparts; i += 8 * SUM_G) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t k = i + u * SUM_G;
+      const float v = base[min(k, p.nparts - 1) * p.stride];
+      a[u] += k < p.nparts ? v : 0.f;
+    }
+  }
+  red[g][col] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+  __syncthreads();
+  if (g != 0 || c >= p.C) return;
+  float s = red[0][col];
+#pragma unroll
+  for (int i = 1; i < SUM_G; ++i) s += red[i][col];
+  if (p.dt[j] == kBF16) static_cast<bf16*>(p.out[j])[c] = (bf16)s;
+  else static_cast<float*>(p.out[j])[c] = s;
 }
 
 }  // namespace hid

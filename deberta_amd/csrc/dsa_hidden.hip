@@ -85,16 +85,17 @@ hid::Drop drop_params(uint32_t t, uint64_t seed) {
 }
 
 // Threads of a block whose threads own a chunk of eight columns each: cw
-// chunks of a row, subs rows at a time, slabs blocks beside each other.
+// chunks of a row, subs rows at a time, slabs blocks beside each other that
+// share the row evenly.
 struct ChunkGrid {
   int cw, subs, slabs, threads;
 };
 ChunkGrid chunk_grid(int C, int most) {
   ChunkGrid g;
   const int chunks = (int)cdiv(C, 8);
-  g.cw = std::min(chunks, most);
-  g.subs = most / g.cw;
   g.slabs = (int)cdiv(chunks, most);
+  g.cw = (int)cdiv(chunks, g.slabs);
+  g.subs = most / g.cw;
   g.threads = round_up(g.cw * g.subs, 64);
   return g;
 }
@@ -102,18 +103,30 @@ bool grid_ok(int64_t blocks, int slabs, int threads) {
   return blocks * threads <= 0xffffffffLL && blocks <= kMaxRows && slabs <= 65535;
 }
 
+// Sums the blocks' partial sums part[nparts][sums][C] into out0 (the first of
+// the sums) and out1 (the second); a null one is left out.
+int sum_parts(const float* part, int64_t nparts, int sums, int C, void* out0, int dt0, void* out1, int dt1, hipStream_t st) {
+  hid::SumParts p{};
+  p.part = part, p.nparts = nparts, p.stride = (int64_t)sums * C, p.C = C;
+  p.out[0] = out0, p.out[1] = out1;
+  p.dt[0] = dt0, p.dt[1] = dt1;
+  hipLaunchKernelGGL(hid::sum_parts_kernel, dim3((unsigned)cdiv(C, hid::SUM_C), out1 ? 2 : 1),
+                     dim3(hid::SUM_C * hid::SUM_G), 0, st, p);
+  return launch_check("sum_parts_kernel");
+}
+
 // ---- dropout ----------------------------------------------------------------
 
-// rows a thread takes in the backward with dbias: at most about 1024 blocks
+// rows a thread takes in the backward with dbias: at most about 512 blocks
 // leave partial sums, and where a thread's rows are 16 at most one block takes
 // all (256 x 128: 6 us, against 4 and 2 more in a second launch) and writes
 // dbias itself
 int drop_sum_rows(int64_t N, int subs) {
   if (N <= 16 * subs) return (int)cdiv(cdiv(N, subs), hid::DROP_U) * hid::DROP_U;
-  return (int)std::max<int64_t>(hid::DROP_U, cdiv(cdiv(N, (int64_t)subs * 1024), hid::DROP_U) * hid::DROP_U);
+  return (int)std::max<int64_t>(hid::DROP_U, cdiv(cdiv(N, (int64_t)subs * 512), hid::DROP_U) * hid::DROP_U);
 }
 int64_t drop_sum_blocks(int64_t N, int C) {
-  const ChunkGrid g = chunk_grid(C, hid::DROP_T);
+  const ChunkGrid g = chunk_grid(C, hid::DROP_SUM_T);
   return cdiv(N, (int64_t)drop_sum_rows(N, g.subs) * g.subs);
 }
 
@@ -144,9 +157,8 @@ int check_dropout(const dsa_dropout_args* a, bool bwd) {
 
 // ---- RMS norm ---------------------------------------------------------------
 
-// rows a team takes in the backward, so that at most 512 blocks leave partial
-// sums
-int rms_sum_rows(int64_t N, int C) { return (int)cdiv(N, (int64_t)512 * rms_teams_of(C)); }
+// rows a team takes in the backward
+int rms_sum_rows(int64_t N, int C) { return (int)cdiv(N, (int64_t)rms_blocks_of(C) * rms_teams_of(C)); }
 int64_t rms_sum_blocks(int64_t N, int C) { return cdiv(N, (int64_t)rms_sum_rows(N, C) * rms_teams_of(C)); }
 
 int check_rms(const dsa_rms_args* a, bool quant, bool bwd) {
@@ -196,10 +208,18 @@ hid::RmsRows rms_params(const dsa_rms_args* a) {
   if (a->res) {
     p.rs0 = a->res_strides[0], p.rs1 = a->res_strides[1];
     p.re = res_extent(a->res_strides, a->rows_per_group, a->N, a->C);
+    p.has_res = 1;
+  } else {  // the first row of x, over and over
+    p.res = a->x, p.re = a->C;
   }
   p.ys = a->y_stride, p.zs = a->z_stride;
   p.dys = a->dy_stride, p.dye = (a->N - 1) * a->dy_stride + a->C;
   p.dzus = a->dzu_stride, p.dzue = (a->N - 1) * a->dzu_stride + a->C;
+  p.has_u = a->dzu != nullptr;
+  if (!p.has_u) {  // the first row of whichever of x and res has z's type
+    p.dzu = a->x_dtype == stream_dtype(a->x_dtype, a->res, a->res_dtype) ? a->x : a->res;
+    p.dzus = 0, p.dzue = a->C;
+  }
   p.dxs = a->dx_stride, p.drs = a->dres_stride;
   p.N = (uint32_t)a->N;
   p.rpg = (uint32_t)std::min<int64_t>(a->res ? a->rows_per_group : a->N, a->N);
@@ -337,7 +357,7 @@ int dsa_dropout_bwd(const dsa_dropout_args* a, void* stream) {
   if (check_dropout(a, true)) return 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (refuse_capture(st, "dsa_dropout_bwd")) return 1;
-  const ChunkGrid g = chunk_grid(a->C, hid::DROP_T);
+  const ChunkGrid g = chunk_grid(a->C, a->dbias ? hid::DROP_SUM_T : hid::DROP_T);
   hid::DropRows p{};
   p.dy = a->dy, p.dx = a->dx;
   p.dys = a->dy_stride, p.dye = (a->N - 1) * a->dy_stride + a->C, p.dxs = a->dx_stride;
@@ -362,9 +382,7 @@ int dsa_dropout_bwd(const dsa_dropout_args* a, void* stream) {
   });
   if (launch_check("drop_bwd_kernel")) return 1;
   if (!p.part) return 0;
-  const int64_t off[1] = {0};
-  void* const out[1] = {a->dbias};
-  return reduce_cols(p.part, nb, a->C, a->C, 1, off, out, &a->bias_dtype, st);
+  return sum_parts(p.part, nb, 1, a->C, a->dbias, a->bias_dtype, nullptr, 0, st);
 }
 
 int dsa_add_rms_fwd(const dsa_rms_args* a, void* stream) { return rms_fwd(a, false, "dsa_add_rms_fwd", stream); }
@@ -387,11 +405,7 @@ int dsa_add_rms_bwd(const dsa_rms_args* a, void* stream) {
     });
   });
   if (rc || !p.part) return rc;
-  const int64_t stride = (int64_t)(a->bias ? 2 : 1) * a->C;
-  const int64_t off[2] = {0, a->C};
-  void* const out[2] = {a->dweight, a->dbias};
-  const int dt[2] = {a->weight_dtype, a->bias_dtype};
-  return reduce_cols(p.part, nb, stride, a->C, a->dbias ? 2 : 1, off, out, dt, st);
+  return sum_parts(p.part, nb, a->bias ? 2 : 1, a->C, a->dweight, a->weight_dtype, a->dbias, a->bias_dtype, st);
 }
 
 size_t dsa_embed_workspace_bytes(int64_t N, int32_t C, int64_t V) {

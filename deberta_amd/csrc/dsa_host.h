@@ -60,11 +60,5 @@ inline thread_local std::string g_err;
   return 0;
 }
 
-// Column sums of a row kernel's per-block partials (dsa_capi.hip): out[j][k]
-// = sum over i < nparts of part[i * stride + off[j] + k] for the nout <= 3
-// outputs (one that is null is left out), in a fixed order, in type dt[j].
-int reduce_cols(const float* part, int64_t nparts, int64_t stride, int K, int nout, const int64_t* off, void* const* out,
-                const int* dt, hipStream_t st);
-
 }  // namespace host
 }  // namespace dsa

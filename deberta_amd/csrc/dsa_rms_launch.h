@@ -16,23 +16,44 @@ namespace host {
 constexpr int kFp8 = 2;  // y's type beside DSA_F32 and DSA_BF16
 constexpr int kMaxRmsC = 16384;
 
-// Rows a block takes at a time: four waves with a row each up to 1024 columns
-// (what a wave holds in registers), beyond that one row for the whole block.
-inline int rms_teams_of(int C) { return C <= 1024 ? 4 : 1; }
-
-// f(NC, W): chunks a lane and waves a row (its team).  Two chunks a lane at
-// most: the backward keeps four fp32 values a column (w, the bias and both
-// sums) beside the row itself.
-template <typename F>
+// f(L, NC, W): lanes a row where it takes less than a wave, chunks a lane,
+// waves a row; at most two chunks a lane.
+//
+// Past 2048 columns the backward takes one chunk a lane and twice the waves of
+// the forward.  It keeps four fp32 values a column (w, the bias and both sums)
+// beside the row itself, and with fewer, larger blocks it leaves fewer partial
+// sums: 8192 x 4096 bf16 4.56 TB/s against 4.18 with two chunks and 512 blocks
+// of four waves, 4096 x 8192 4.42 against 3.97.  The forward has no such sums
+// and loses on widths that fill the waves badly: 8176 x 4104 4.1 against 5.3.
+template <bool BWD, typename F>
 void by_width(int C, F f) {
   using std::integral_constant;
-  if (C <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else if (C <= 1024) f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  else if (C <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-  else if (C <= 4096) f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-  else if (C <= 8192) f(integral_constant<int, 2>{}, integral_constant<int, 8>{});
-  else f(integral_constant<int, 2>{}, integral_constant<int, 16>{});
+  integral_constant<int, 16> i16;
+  integral_constant<int, 32> i32;
+  integral_constant<int, 64> i64;
+  integral_constant<int, 1> i1;
+  integral_constant<int, 2> i2;
+  integral_constant<int, 4> i4;
+  integral_constant<int, 8> i8;
+  if (C <= 128) f(i16, i1, i1);
+  else if (C <= 256) f(i32, i1, i1);
+  else if (C <= 512) f(i64, i1, i1);
+  else if (C <= 1024) f(i64, i2, i1);
+  else if (C <= 2048) f(i64, i1, i4);
+  else if (C <= 4096 && BWD) f(i64, i1, i8);
+  else if (C <= 4096) f(i64, i2, i4);
+  else if (C <= 8192 && BWD) f(i64, i1, i16);
+  else if (C <= 8192) f(i64, i2, i8);
+  else f(i64, i2, i16);
 }
+// Teams a block of the backward, and the blocks that run at once: two a
+// compute unit of four waves, one of eight or sixteen.
+inline int rms_teams_of(int C) {
+  int n = 0;
+  by_width<true>(C, [&](auto l, auto, auto w) { n = hid::rms_teams<decltype(l)::value, decltype(w)::value>(); });
+  return n;
+}
+inline int rms_blocks_of(int C) { return C <= 2048 ? 512 : 256; }
 
 // f(TAIL): whether rows end in a chunk of fewer than eight columns
 template <typename F>
@@ -47,14 +68,14 @@ using stream_t = std::conditional_t<std::is_same<TX, TR>::value, TX, float>;
 template <typename TX, typename TR>
 int launch_rms_fwd(const hid::RmsRows& p, int y_dt, hipStream_t st) {
   typedef stream_t<TX, TR> TZ;
-  by_width(p.C, [&](auto nc, auto w) {
+  by_width<false>(p.C, [&](auto l, auto nc, auto w) {
     by_tail(p.C, [&](auto tail) {
-      constexpr int NC = decltype(nc)::value, W = decltype(w)::value;
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, W = decltype(w)::value;
       constexpr bool T = decltype(tail)::value;
-      const dim3 grid((unsigned)cdiv(p.N, hid::rms_teams<W>())), block(hid::rms_threads<W>());
-      if (y_dt == kFp8) hipLaunchKernelGGL((hid::rms_fwd_kernel<NC, W, TX, TR, TZ, hid::fp8, T>), grid, block, 0, st, p);
-      else if (y_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_fwd_kernel<NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
-      else hipLaunchKernelGGL((hid::rms_fwd_kernel<NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
+      const dim3 grid((unsigned)cdiv(p.N, hid::rms_teams<L, W>())), block(hid::rms_threads<W>());
+      if (y_dt == kFp8) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, hid::fp8, T>), grid, block, 0, st, p);
+      else if (y_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
+      else hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
     });
   });
   return launch_check("rms_fwd_kernel");
@@ -63,13 +84,13 @@ int launch_rms_fwd(const hid::RmsRows& p, int y_dt, hipStream_t st) {
 template <typename TX, typename TR>
 int launch_rms_bwd(const hid::RmsRows& p, int dy_dt, int64_t blocks, hipStream_t st) {
   typedef stream_t<TX, TR> TZ;
-  by_width(p.C, [&](auto nc, auto w) {
+  by_width<true>(p.C, [&](auto l, auto nc, auto w) {
     by_tail(p.C, [&](auto tail) {
-      constexpr int NC = decltype(nc)::value, W = decltype(w)::value;
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, W = decltype(w)::value;
       constexpr bool T = decltype(tail)::value;
       const dim3 grid((unsigned)blocks), block(hid::rms_threads<W>());
-      if (dy_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_bwd_kernel<NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
-      else hipLaunchKernelGGL((hid::rms_bwd_kernel<NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
+      if (dy_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_bwd_kernel<L, NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
+      else hipLaunchKernelGGL((hid::rms_bwd_kernel<L, NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
     });
   });
   return launch_check("rms_bwd_kernel");

@@ -561,7 +561,7 @@ struct ReduceCols {
   int nout;
   int64_t off[3];
   void* out[3];
-  int dt[3];
+  int dt;
 };
 __global__ __launch_bounds__(64 * RED_W) void reduce_cols_kernel(ReduceCols rc) {
   __shared__ float red[RED_W][64];
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(64 * RED_W) void reduce_cols_kernel(ReduceCols rc) 
     float t = red[0][lane];
 #pragma unroll
     for (int v = 1; v < RED_W; ++v) t += red[v][lane];
-    st1(rc.out[j], k, t, rc.dt[j]);
+    st1(rc.out[j], k, t, rc.dt);
   }
 }
 
