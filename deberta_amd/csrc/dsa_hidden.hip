@@ -210,15 +210,16 @@ hid::RmsRows rms_params(const dsa_rms_args* a) {
     p.re = res_extent(a->res_strides, a->rows_per_group, a->N, a->C);
     p.has_res = 1;
   } else {  // the first row of x, over and over
-    p.res = a->x, p.re = a->C;
+    p.res = a->x, p.re = p.xe;
   }
   p.ys = a->y_stride, p.zs = a->z_stride;
   p.dys = a->dy_stride, p.dye = (a->N - 1) * a->dy_stride + a->C;
   p.dzus = a->dzu_stride, p.dzue = (a->N - 1) * a->dzu_stride + a->C;
   p.has_u = a->dzu != nullptr;
   if (!p.has_u) {  // the first row of whichever of x and res has z's type
-    p.dzu = a->x_dtype == stream_dtype(a->x_dtype, a->res, a->res_dtype) ? a->x : a->res;
-    p.dzus = 0, p.dzue = a->C;
+    const bool as_x = a->x_dtype == stream_dtype(a->x_dtype, a->res, a->res_dtype);
+    p.dzu = as_x ? a->x : a->res;
+    p.dzus = 0, p.dzue = as_x ? p.xe : p.re;
   }
   p.dxs = a->dx_stride, p.drs = a->dres_stride;
   p.N = (uint32_t)a->N;

@@ -567,6 +567,73 @@ def test_a_run_of_them_together(gpu):
         assert err <= 1e-4 * b.abs().max().item(), (name, err)
 
 
+def test_eight_bit_rows_feed_a_scaled_product(gpu):
+    """Serving in 8 bits as it is used: the norm's rows and scales straight
+    into torch's row-scaled float8 product.  Against float64 on the values
+    that q and the weight's bytes stand for, the product loses its float32
+    sums (K u of the sum of magnitudes) and the bf16 of its result."""
+    M, K, N = 64, 512, 256
+    x, res = _rand(M, K, seed=1, dtype=BF).to(gpu), _rand(M, K, seed=2, dtype=BF).to(gpu)
+    with torch.no_grad():
+        q, scale, z = da.fused_add_rms_norm_fp8(x, torch.ones(K, device=gpu), res=res)
+        w = _rand(N, K, seed=3, dtype=FP, std=0.05)
+        ws = w.abs().amax(1, keepdim=True) / 448.0
+        wq = (w / ws).to(torch.float8_e4m3fn)
+        y = torch._scaled_mm(q, wq.to(gpu).t(), scale_a=scale, scale_b=ws.t().contiguous().to(gpu), out_dtype=BF)
+    a = q.float().cpu().double() * scale.cpu().double()
+    b = (wq.float().double() * ws.double()).t()
+    _within("product", y, a @ b, (K * U + 4 * U) * (a.abs() @ b.abs()) + _half(BF) * (a @ b).abs())
+    assert torch.equal(z, x + res)
+
+
+def test_one_tensor_in_two_places(gpu):
+    """x and the residual one leaf, a table looked up twice, a graph walked
+    twice: gradients add up."""
+    x = _rand(6, 200, seed=1, dtype=FP).to(gpu).requires_grad_()
+    w = torch.ones(200, device=gpu)
+    dy = _rand(6, 200, seed=2, dtype=FP).to(gpu)
+    for p in (0.0, 0.5):
+        y, z = da.fused_add_rms_norm(x, w, EPS, res=x, dropout_p=p, seed=SEED)
+        (g,) = torch.autograd.grad((y, z), x, (dy, dy), retain_graph=True)
+        (again,) = torch.autograd.grad((y, z), x, (dy, dy))
+        assert torch.equal(g, again)
+        u, v = x.detach().requires_grad_(), x.detach().requires_grad_()
+        y, z = da.fused_add_rms_norm(u, w, EPS, res=v, dropout_p=p, seed=SEED)
+        gu, gv = torch.autograd.grad((y, z), (u, v), (dy, dy))
+        assert torch.equal(g, gu + gv)
+        y = da.fused_dropout(x, p, res=x, seed=SEED)
+        (g,) = torch.autograd.grad(y, x, dy)
+        keep = oh.keep_mask(6, 200, round(p * 65536), SEED).to(gpu) / (1 - p)
+        assert torch.equal(g, dy * keep + dy)
+    table = _rand(30, 40, seed=3, dtype=FP).to(gpu).requires_grad_()
+    a = torch.arange(10, device=gpu)
+    y = da.fused_embedding(a, table) + da.fused_embedding(a.flip(0), table)
+    (g,) = torch.autograd.grad(y.sum(), table)
+    assert (g[:10] == 2).all() and (g[10:] == 0).all()
+    # ids with strides of their own
+    grid = torch.arange(24, device=gpu).view(4, 6)
+    assert torch.equal(da.fused_embedding(grid.t(), table), table[grid.t()])
+    assert torch.equal(da.fused_embedding(grid[:, ::2], table), table[grid[:, ::2]])
+
+
+def test_only_some_inputs_need_gradients(gpu):
+    x, r, b = (_rand(*s, seed=k, dtype=FP).to(gpu) for k, s in enumerate(((4, 60), (4, 60), (60,))))
+    w = torch.ones(60, device=gpu)
+    dy = _rand(4, 60, seed=5, dtype=FP).to(gpu)
+
+    def grads(*which):
+        t = [v.detach().requires_grad_(k in which) for k, v in zip("xrbw", (x, r, b, w))]
+        y, z = da.fused_add_rms_norm(t[0], t[3], EPS, bias=t[2], res=t[1], dropout_p=0.25, seed=SEED)
+        d = da.fused_dropout(t[0], 0.25, bias=t[2], res=t[1], seed=SEED)
+        need = [v for v in t if v.requires_grad]
+        out = [(y * dy).sum() + (z * dy).sum()] + ([(d * dy).sum()] if d.requires_grad else [])
+        return dict(zip(which, torch.autograd.grad(sum(out), need)))
+
+    full = grads("x", "r", "b", "w")
+    for one in "xrbw":
+        assert torch.equal(grads(one)[one], full[one])
+
+
 def test_checkpointing_draws_the_same_bits(gpu):
     from torch.utils.checkpoint import checkpoint
 

@@ -50,8 +50,9 @@ def test_dropped_share_and_the_ends_of_p():
     assert da.hidden_keep_mask(4, 9, 0.0, 7).all() and not da.hidden_keep_mask(4, 9, 1.0, 7).any()
 
 
-@pytest.mark.parametrize("p", [0.0, 0.3, 1.0])
-@pytest.mark.parametrize("with_bias,with_res", [(False, False), (True, True), (False, True)])
+# p = 1 without a residual leaves zeros, whose norm's gradient goes by 1 / sqrt(eps)
+@pytest.mark.parametrize("p,with_bias,with_res", [(p, b, r) for p in (0.0, 0.3, 1.0)
+                                                  for b, r in ((False, False), (True, True), (False, True)) if p < 1 or r])
 def test_cpu_path_matches_float64(p, with_bias, with_res):
     x, w = _rand(2, 5, 40, seed=1), 1 + 0.1 * _rand(40, seed=2)
     bias = _rand(40, seed=3) if with_bias else None
@@ -76,8 +77,6 @@ def test_cpu_path_matches_float64(p, with_bias, with_res):
         z = oh.dropout_add(x, b, r, t, SEED)
         return oh.rms_norm(z, w, 1e-6), z, z
 
-    if p == 1.0 and not with_res:
-        pytest.skip("every value is 0: the norm's gradient is 1 / sqrt(eps)")
     for tol, a, b in zip((3e-5, 1e-4), run(ours, torch.float32), run(ref, torch.float64)):
         for u, v in zip(a, b):
             assert (u.double() - v).abs().max().item() <= tol
