@@ -1,10 +1,13 @@
-"""Builds ``libdsa.so`` (the HIP kernels and their C ABI) in-tree with hipcc for gfx950."""
+"""Builds ``libdsa.so`` (the HIP kernels and their C ABI) in-tree with hipcc for
+gfx950, and ``_hidden_ext.so`` (the host side of the operators on hidden
+states: PyTorch tensors and autograd over that C ABI) with g++."""
 
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -28,6 +31,9 @@ SOURCES = (
 # bench.py's MFMA throughput probe (include/dsa_probe.h), a library of its own
 PROBE_PATH = PKG_DIR / "libdsa_probe.so"
 PROBE_SOURCES = (("dsa_probe.hip", ()),)
+# the operators on hidden states for PyTorch tensors: host code, linked to libdsa.so
+EXT_PATH = PKG_DIR / "_hidden_ext.so"
+EXT_SOURCE = CSRC_DIR / "hidden_ext.cpp"
 ARCH = "gfx950"
 
 # Packed fp32 VALU ops are kept out of the generated code: hipcc otherwise
@@ -77,22 +83,54 @@ def _compile(sources, out: Path, verbose: bool) -> Path:
     return out
 
 
+def _ext_commands(obj: Path, out: Path) -> tuple[list[str], list[str]]:
+    """(compile, link) of the extension.  It finds libdsa.so beside itself and
+    torch's libraries where the process has loaded them."""
+    import torch
+
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: _hidden_ext.so cannot be built")
+    root = Path(torch.__file__).resolve().parent
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+               Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    compile_cmd = [cxx, *flags, *(f"-isystem{p}" for p in include), "-c", str(EXT_SOURCE), "-o", str(obj)]
+    libs = ("torch", "torch_cpu", "torch_hip", "c10", "c10_hip", "torch_python")
+    link_cmd = [cxx, "-shared", str(obj), f"-L{root / 'lib'}", *(f"-l{n}" for n in libs), f"-L{PKG_DIR}", "-l:libdsa.so",
+                "-Wl,-rpath,$ORIGIN", "-o", str(out)]
+    return compile_cmd, link_cmd
+
+
 def _run(cmd) -> None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}):\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP source: ``deberta_amd/libdsa.so`` (the kernels and
-    their C ABI) and ``deberta_amd/libdsa_probe.so`` (the MFMA probe).
+    """Compile every source: ``deberta_amd/libdsa.so`` (the kernels and their
+    C ABI), ``deberta_amd/libdsa_probe.so`` (the MFMA probe) and
+    ``deberta_amd/_hidden_ext.so`` (the hidden-state operators' host side).
 
     Always recompiles.  Each library is written to a temporary name first and
     renamed into place, so a process that already loaded the old file keeps a
     consistent image.
     """
-    _compile(PROBE_SOURCES, PROBE_PATH, verbose)
-    return _compile(SOURCES, LIB_PATH, verbose)
+    with tempfile.TemporaryDirectory(dir=PKG_DIR, prefix="_build") as tmp_dir, ThreadPoolExecutor(1) as pool:
+        tmp = EXT_PATH.with_suffix(".so.tmp")
+        compile_cmd, link_cmd = _ext_commands(Path(tmp_dir) / "ext.o", tmp)
+        ext = pool.submit(_run, compile_cmd)
+        _compile(PROBE_SOURCES, PROBE_PATH, verbose)
+        lib = _compile(SOURCES, LIB_PATH, verbose)
+        ext.result()
+        _run(link_cmd)
+        os.replace(tmp, EXT_PATH)
+        if verbose:
+            print(" ".join(compile_cmd))
+            print(" ".join(link_cmd))
+    return lib
 
 
 if __name__ == "__main__":

@@ -15,7 +15,9 @@ and the modules FusedEmbedding, FusedDropout and FusedRMSNorm on them.
 
 The kernels take float32 and bfloat16 tensors of any width, row stride and
 element alignment; arithmetic, sums and statistics are float32, and every
-result is rounded once.  CPU tensors run the same operators in torch
+result is rounded once.  In plain eager mode the functions go through
+csrc/hidden_ext.cpp (checks, memory, launches and autograd nodes in C++: the
+host time of a call is what bounds these operators on small batches).  CPU tensors run the same operators in torch
 operations, dropout with the same keep bits.  The ops under the functions
 (``deberta_amd::hidden_dropout``, ``add_rms_norm``, ``add_rms_norm_quant``,
 ``embed`` and the backwards) take device tensors only; like the package's
@@ -35,7 +37,7 @@ included).
 
 from __future__ import annotations
 
-import ctypes
+import functools
 from typing import Any, Optional, Union
 
 import torch
@@ -43,110 +45,45 @@ import torch.nn as nn
 from torch import Tensor
 
 from deberta_amd import _eager, _lib
+from deberta_amd._build import EXT_PATH
 from deberta_amd.ops import draw_dropout_seed, dropout_threshold
 
 _TAGS = (torch.Tag.cudagraph_unsafe,)  # as the package's other ops
-_DT = {torch.float32: _lib.DSA_F32, torch.bfloat16: _lib.DSA_BF16}
 _MASK32 = 0xFFFFFFFF
 _DOMAIN = 0x68696464  # the last word of hidden dropout's counters
 FP8_MAX = 448.0  # the largest value of float8_e4m3fn
 MAX_RMS_WIDTH = 16384
 
 
-def _dt(t: Tensor, what: str, name: str) -> int:
-    code = _DT.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} {name}: dtype must be float32 or bfloat16, got {t.dtype}")
-    return code
+@functools.lru_cache(maxsize=None)
+def _ext() -> Any:
+    """The host side of the operators on the GPU (csrc/hidden_ext.cpp)."""
+    _lib.load()  # and checks its version
+    if not EXT_PATH.exists():
+        raise RuntimeError(
+            f"{EXT_PATH} is missing: the operators on hidden states are not built. Run `python -m deberta_amd._build` first."
+        )
+    from deberta_amd import _hidden_ext
+
+    return _hidden_ext
 
 
-def _rows(t: Tensor) -> tuple[Tensor, int]:
-    """``t`` as rows of its last dimension with unit stride, and their
-    stride (a copy only where the leading dimensions have no one stride)."""
-    if t.is_contiguous():
-        return t, t.shape[-1]
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t2.stride(-1) != 1 and t2.shape[-1] > 1:
-        t2 = t2.contiguous()
-    return t2, t2.stride(0)
-
-
-def _res_layout(res: Tensor) -> tuple[Tensor, tuple[int, int], int]:
-    """(tensor, group and row stride, rows per group) of a residual; one that
-    is broadcast along the second of three dimensions is read in place."""
-    if res.dim() == 3 and not res.is_contiguous() and (res.stride(-1) == 1 or res.shape[-1] == 1):
-        return res, (res.stride(0), res.stride(1)), res.shape[1]
-    t, stride = _rows(res)
-    return t, (0, stride), max(1, res.numel() // max(1, res.shape[-1]))
-
-
-def _vec(t: Optional[Tensor], C: int, what: str, name: str) -> Optional[Tensor]:
-    if t is None:
-        return None
-    if t.dim() != 1 or t.shape[0] != C:
-        raise ValueError(f"{what} {name} must have shape ({C},), got {tuple(t.shape)}")
-    return t.contiguous()
-
-
-def _check(what: str, x: Tensor, *others: Optional[Tensor]) -> int:
-    """x's width; the other tensors on x's device."""
+def _cpu_args(what: str, x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], weight: Optional[Tensor] = None) -> None:
+    """The checks of the torch path."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"{what}: x needs a last dimension of at least one column, got shape {tuple(x.shape)}")
-    device = x.get_device()
-    for t in others:
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"{what}: a tensor is on {t.device}, x is on {x.device}")
-    return x.shape[-1]
-
-
-def _same_shape(what: str, x: Tensor, res: Optional[Tensor]) -> None:
+    for name, t in (("bias", bias), ("weight", weight)):
+        if t is not None and tuple(t.shape) != (x.shape[-1],):
+            raise ValueError(f"{what} {name} must have shape ({x.shape[-1]},), got {tuple(t.shape)}")
     if res is not None and res.shape != x.shape:
         raise ValueError(f"{what}: res must have x's shape {tuple(x.shape)}, got {tuple(res.shape)}")
+    for name, t in (("bias", bias), ("res", res), ("weight", weight)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, x is on {x.device}")
 
 
 def _stream_dtype(x: Tensor, res: Optional[Tensor]) -> torch.dtype:
-    if res is None or res.dtype is x.dtype:
-        return x.dtype
-    return torch.promote_types(x.dtype, res.dtype)
-
-
-_entries: dict[str, Any] = {}
-
-
-def _launch(entry: str, a: ctypes.Structure, t: Tensor) -> None:
-    """Calls a library entry point on the current stream of t's device (it
-    refuses a stream that is capturing a HIP graph)."""
-    fn = _entries.get(entry)
-    if fn is None:
-        fn = _entries[entry] = getattr(_lib.load(), entry)
-    if t.get_device() == torch.cuda.current_device():
-        rc = fn(a, _eager.stream_ptr(t))
-    else:
-        with torch.cuda.device(t.device):
-            rc = fn(a, _eager.stream_ptr(t))
-    if rc:
-        _lib.check(rc, entry)
-
-
-def _empty(like: Tensor, dtype: torch.dtype) -> Tensor:
-    """An uninitialised contiguous tensor of like's shape."""
-    if like.dtype is dtype and like.is_contiguous():
-        return torch.empty_like(like)
-    return torch.empty(like.shape, dtype=dtype, device=like.device)
-
-
-def _workspace(kind: int, N: int, C: int, t: Tensor) -> Optional[Tensor]:
-    n = _lib.load().dsa_block_workspace_bytes(kind, N, C)
-    return torch.empty((n,), dtype=torch.uint8, device=t.device) if n else None
-
-
-def _needs_grad(*tensors: Optional[Tensor]) -> bool:
-    """Whether autograd records a call on these tensors."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
+    return x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -173,16 +110,6 @@ def _seed_tensor(seed: Union[None, int, Tensor]) -> Tensor:
     if not isinstance(seed, Tensor) or seed.numel() != 1 or seed.dtype != torch.int64 or seed.device.type != "cpu":
         raise ValueError("dropout seed must be an int or an int64 CPU tensor of one element")
     return seed
-
-
-def _seed_value(seed: Optional[Tensor], t: int) -> int:
-    if not t:
-        return 0
-    if not 0 < t <= 65536:
-        raise ValueError(f"dropout threshold must be in [0, 65536], got {t}")
-    if seed is None:
-        raise ValueError("dropout needs a seed")
-    return int(_seed_tensor(seed).item()) & 0xFFFFFFFFFFFFFFFF
 
 
 def hidden_keep_mask(rows: int, C: int, p: float, seed: Union[int, Tensor], device: Union[str, torch.device] = "cpu") -> Tensor:
@@ -223,53 +150,14 @@ def _hidden_dropout_impl(
     x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], dropout_t: int, dropout_seed: Optional[Tensor]
 ) -> Tensor:
     """``dropout(x + bias) + res`` in x's type promoted with res's."""
-    what = "hidden_dropout"
-    C = _check(what, x, bias, res)
-    _same_shape(what, x, res)
-    x_dt, seed = _dt(x, what, "x"), _seed_value(dropout_seed, dropout_t)
-    xr, xs = _rows(x)
-    bias = _vec(bias, C, what, "bias")
-    y = _empty(x, _stream_dtype(x, res))
-    N = x.numel() // C
-    a = _lib.DsaDropoutArgs(
-        x=xr.data_ptr(), x_stride=xs, x_dtype=x_dt, y=y.data_ptr(), y_stride=C, y_dtype=_DT.get(y.dtype, -1), N=N, C=C,
-        threshold=dropout_t, seed=seed,
-    )
-    if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, what, "bias")
-    if res is not None:
-        a.res_dtype = _dt(res, what, "res")
-        rr, a.res_strides, a.rows_per_group = _res_layout(res)
-        a.res = rr.data_ptr()
-    if N:
-        _launch("dsa_dropout_fwd", a, x)
-    return y
+    return _ext().dropout_fwd(x, bias, res, dropout_t, dropout_seed)
 
 
 def _hidden_dropout_bwd_impl(
     dy: Tensor, dx_dtype: torch.dtype, bias_dtype: Optional[torch.dtype], dropout_t: int, dropout_seed: Optional[Tensor]
 ) -> tuple[Tensor, Tensor]:
     """(dx in ``dx_dtype``, dbias in ``bias_dtype``, empty where that is None)."""
-    what = "hidden_dropout_bwd"
-    C = _check(what, dy)
-    dyr, dys = _rows(dy)
-    N = dy.numel() // C
-    dx = _empty(dy, dx_dtype)
-    dbias = torch.empty((0 if bias_dtype is None else C,), dtype=bias_dtype or dx_dtype, device=dy.device)
-    a = _lib.DsaDropoutArgs(
-        dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, what, "dy"), dx=dx.data_ptr(), dx_stride=C,
-        dx_dtype=_dt(dx, what, "dx"), N=N, C=C, threshold=dropout_t, seed=_seed_value(dropout_seed, dropout_t),
-    )
-    if bias_dtype is not None:
-        if not N:
-            return dx, dbias.zero_()
-        a.dbias, a.bias_dtype = dbias.data_ptr(), _dt(dbias, what, "bias")
-        ws = _workspace(_lib.DSA_BLOCK_DROPOUT, N, C, dy)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    if N:
-        _launch("dsa_dropout_bwd", a, dy)
-    return dx, dbias
+    return _ext().dropout_bwd(dy, dx_dtype, bias_dtype, dropout_t, dropout_seed)
 
 
 hidden_dropout = torch.library.custom_op(
@@ -297,7 +185,6 @@ def _hidden_dropout_setup(ctx, inputs, output):
     ctx.dropout_t, ctx.x_dtype = dropout_t, x.dtype
     ctx.bias_dtype = None if bias is None else bias.dtype
     ctx.res_dtype = None if res is None else res.dtype
-    ctx.op_in_graph = True
 
 
 def _hidden_dropout_backward(ctx, dy):
@@ -305,18 +192,13 @@ def _hidden_dropout_backward(ctx, dy):
     dx = dbias = dres = None
     for_x, for_bias, for_res = ctx.needs_input_grad[:3]
     if for_x or for_bias:
-        dx, dbias = _eager.on_eager(ctx, hidden_dropout_bwd, _hidden_dropout_bwd_impl)(
-            dy, ctx.x_dtype, ctx.bias_dtype if for_bias else None, ctx.dropout_t, seed
-        )
+        dx, dbias = hidden_dropout_bwd(dy, ctx.x_dtype, ctx.bias_dtype if for_bias else None, ctx.dropout_t, seed)
     if for_res:
         dres = dy if dy.dtype is ctx.res_dtype else dy.to(ctx.res_dtype)
     return dx, (dbias if for_bias else None), dres, None, None
 
 
 torch.library.register_autograd("deberta_amd::hidden_dropout", _hidden_dropout_backward, setup_context=_hidden_dropout_setup)
-_HiddenDropoutFunction = _eager.function(
-    "_HiddenDropoutFunction", _hidden_dropout_impl, _hidden_dropout_setup, _hidden_dropout_backward
-)
 
 
 def fused_dropout(
@@ -341,12 +223,10 @@ def fused_dropout(
         return x
     s = _seed_tensor(seed) if t else None
     if not x.is_cuda:
-        C = _check("fused_dropout", x, bias, res)
-        _same_shape("fused_dropout", x, res)
-        return _cpu_sum(x, _vec(bias, C, "fused_dropout", "bias"), res, t, s).to(_stream_dtype(x, res))
+        _cpu_args("fused_dropout", x, bias, res)
+        return _cpu_sum(x, bias, res, t, s).to(_stream_dtype(x, res))
     if _eager.eager(x):
-        run = _HiddenDropoutFunction.apply if _needs_grad(x, bias, res) else _hidden_dropout_impl
-        return run(x, bias, res, t, s)
+        return _ext().dropout(x, bias, res, t, s)
     return torch.ops.deberta_amd.hidden_dropout(x, bias, res, t, s)
 
 
@@ -354,62 +234,9 @@ def fused_dropout(
 # residual + RMS norm
 
 
-def _fill_rms(
-    what: str, x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], weight: Tensor, dropout_t: int, seed: Optional[Tensor]
-) -> tuple[_lib.DsaRmsArgs, tuple]:
-    """The arguments every form shares, and the tensors they point into."""
-    C = _check(what, x, bias, res, weight)
-    if C > MAX_RMS_WIDTH:
-        raise ValueError(f"{what}: rows of at most {MAX_RMS_WIDTH} columns, got {C}")
-    _same_shape(what, x, res)
-    bias, weight = _vec(bias, C, what, "bias"), _vec(weight, C, what, "weight")
-    xr, xs = _rows(x)
-    a = _lib.DsaRmsArgs(
-        x=xr.data_ptr(), x_stride=xs, x_dtype=_dt(x, what, "x"), weight=weight.data_ptr(),
-        weight_dtype=_dt(weight, what, "weight"), N=x.numel() // C, C=C, threshold=dropout_t,
-        seed=_seed_value(seed, dropout_t),
-    )
-    rr = None
-    if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _dt(bias, what, "bias")
-    if res is not None:
-        a.res_dtype = _dt(res, what, "res")
-        rr, a.res_strides, a.rows_per_group = _res_layout(res)
-        a.res = rr.data_ptr()
-    return a, (xr, bias, weight, rr)
-
-
 def _plain(bias: Optional[Tensor], res: Optional[Tensor], dropout_t: int) -> bool:
     """z is x itself."""
     return bias is None and res is None and not dropout_t
-
-
-def _rms_forward(
-    x: Tensor,
-    bias: Optional[Tensor],
-    res: Optional[Tensor],
-    weight: Tensor,
-    eps: float,
-    out_dtype: torch.dtype,
-    dropout_t: int,
-    dropout_seed: Optional[Tensor],
-    rstd: Optional[Tensor] = None,
-) -> tuple[Tensor, Tensor]:
-    """(y in ``out_dtype``, z = dropout(x + bias) + res); z is x where there is
-    nothing to add or drop.  1 / rms per row goes to ``rstd``."""
-    a, keep = _fill_rms("add_rms_norm", x, bias, res, weight, dropout_t, dropout_seed)
-    C = a.C
-    y = _empty(x, out_dtype)
-    a.y, a.y_stride, a.y_dtype, a.eps = y.data_ptr(), C, _dt(y, "add_rms_norm", "y"), eps
-    z = x
-    if not _plain(bias, res, dropout_t):
-        z = _empty(x, _stream_dtype(x, res))
-        a.z, a.z_stride = z.data_ptr(), C
-    if rstd is not None:
-        a.rstd = rstd.data_ptr()
-    if a.N:
-        _launch("dsa_add_rms_fwd", a, x)
-    return y, z
 
 
 def _add_rms_norm_impl(
@@ -424,10 +251,7 @@ def _add_rms_norm_impl(
 ) -> tuple[Tensor, Tensor, Tensor]:
     """(y in ``out_dtype``, z = dropout(x + bias) + res, 1 / rms per row); z is
     empty where it is x itself."""
-    rows = x.numel() // max(1, x.shape[-1]) if x.dim() else 0
-    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    y, z = _rms_forward(x, bias, res, weight, eps, out_dtype, dropout_t, dropout_seed, rstd)
-    return y, (x.new_empty((0,)) if z is x else z), rstd
+    return _ext().rms_fwd(x, bias, res, weight, eps, out_dtype, dropout_t, dropout_seed)
 
 
 def _add_rms_norm_bwd_impl(
@@ -444,33 +268,7 @@ def _add_rms_norm_bwd_impl(
     """(dx, dres, dweight, dbias) for the gradients of y and (optional) of z.
     dres is empty without a residual and where it equals dx (no dropout, one
     type); dbias is empty without a bias."""
-    what = "add_rms_norm_bwd"
-    a, keep = _fill_rms(what, x, bias, res, weight, dropout_t, dropout_seed)
-    _check(what, x, dy, dz, rstd)
-    dx = _empty(x, x.dtype)
-    apart = res is not None and (dropout_t or res.dtype != x.dtype)
-    dres = _empty(x, res.dtype) if apart else torch.empty((0,), dtype=x.dtype, device=x.device)
-    dweight = torch.empty_like(keep[2])
-    dbias = torch.empty_like(keep[1]) if bias is not None else weight.new_empty((0,))
-    if not a.N:
-        dweight.zero_(), dbias.zero_()
-        return dx, dres, dweight, dbias
-    dyr, a.dy_stride = _rows(dy)
-    a.dy, a.dy_dtype, a.rstd = dyr.data_ptr(), _dt(dy, what, "dy"), rstd.data_ptr()
-    if dz is not None:
-        dzr, a.dzu_stride = _rows(dz if dz.dtype == _stream_dtype(x, res) else dz.to(_stream_dtype(x, res)))
-        a.dzu = dzr.data_ptr()
-    a.dx, a.dx_stride = dx.data_ptr(), a.C
-    if apart:
-        a.dres, a.dres_stride = dres.data_ptr(), a.C
-    a.dweight = dweight.data_ptr()
-    if bias is not None:
-        a.dbias = dbias.data_ptr()
-    ws = _workspace(_lib.DSA_BLOCK_RMS, a.N, a.C, x)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _launch("dsa_add_rms_bwd", a, x)
-    return dx, dres, dweight, dbias
+    return _ext().rms_bwd(dy, dz, x, bias, res, weight, rstd, dropout_t, dropout_seed)
 
 
 def _add_rms_norm_quant_impl(
@@ -478,19 +276,7 @@ def _add_rms_norm_quant_impl(
 ) -> tuple[Tensor, Tensor, Tensor]:
     """(y as float8_e4m3fn, its scales, z); z is empty where it is x itself.
     ``group_size`` 0: one scale a row."""
-    a, keep = _fill_rms("add_rms_norm_quant", x, bias, res, weight, 0, None)
-    _check_group(a.C, group_size)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    groups = a.C // group_size if group_size else 1
-    scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device)
-    plain, z_dtype = _plain(bias, res, 0), _stream_dtype(x, res)
-    z = torch.empty((0,), dtype=z_dtype, device=x.device) if plain else _empty(x, z_dtype)
-    a.y, a.y_stride, a.scales, a.group_size, a.eps = q.data_ptr(), a.C, scales.data_ptr(), group_size, eps
-    if a.N:
-        if not plain:
-            a.z, a.z_stride = z.data_ptr(), a.C
-        _launch("dsa_add_rms_quant", a, x)
-    return q, scales, z
+    return _ext().quant_fwd(x, bias, res, weight, eps, group_size)
 
 
 add_rms_norm = torch.library.custom_op(
@@ -538,7 +324,6 @@ def _add_rms_norm_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(*((rstd, z) if _plain(bias, res, dropout_t) else (rstd,)))
     ctx.save_for_backward(x, bias, res, weight, rstd, seed)
     ctx.dropout_t, ctx.out_dtype = dropout_t, out_dtype
-    ctx.op_in_graph = True
     ctx.set_materialize_grads(False)
 
 
@@ -548,9 +333,7 @@ def _add_rms_norm_backward(ctx, dy, dz, drstd):
         return (None,) * 8
     if dy is None:  # only z was used
         dy = torch.zeros(x.shape, dtype=ctx.out_dtype, device=x.device)
-    dx, dres, dweight, dbias = _eager.on_eager(ctx, add_rms_norm_bwd, _add_rms_norm_bwd_impl)(
-        dy, dz, x, bias, res, weight, rstd, ctx.dropout_t, seed
-    )
+    dx, dres, dweight, dbias = add_rms_norm_bwd(dy, dz, x, bias, res, weight, rstd, ctx.dropout_t, seed)
     if res is None:
         dres = None
     elif not (ctx.dropout_t or res.dtype != x.dtype):
@@ -559,9 +342,6 @@ def _add_rms_norm_backward(ctx, dy, dz, drstd):
 
 
 torch.library.register_autograd("deberta_amd::add_rms_norm", _add_rms_norm_backward, setup_context=_add_rms_norm_setup)
-_AddRmsNormFunction = _eager.function(
-    "_AddRmsNormFunction", _add_rms_norm_impl, _add_rms_norm_setup, _add_rms_norm_backward
-)
 
 
 def norm_out_dtype(x: Tensor, res: Optional[Tensor]) -> torch.dtype:
@@ -596,17 +376,13 @@ def fused_add_rms_norm(
     s = _seed_tensor(seed) if t else None
     out_dtype = norm_out_dtype(x, res) if out_dtype is None else out_dtype
     if not x.is_cuda:
-        C = _check("fused_add_rms_norm", x, bias, res, weight)
-        _same_shape("fused_add_rms_norm", x, res)
-        z = _cpu_sum(x, _vec(bias, C, "fused_add_rms_norm", "bias"), res, t, s)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "fused_add_rms_norm", "weight").float()
+        _cpu_args("fused_add_rms_norm", x, bias, res, weight)
+        z = _cpu_sum(x, bias, res, t, s)
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.float()
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
-        if not _needs_grad(x, bias, res, weight):
-            return _rms_forward(x, bias, res, weight, float(eps), out_dtype, t, s)
-        y, z, _ = _AddRmsNormFunction.apply(x, bias, res, weight, float(eps), out_dtype, t, s)
-    else:
-        y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
+        return _ext().rms(x, bias, res, weight, float(eps), out_dtype, t, s)
+    y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
     return y, (x if _plain(bias, res, t) else z)
 
 
@@ -614,11 +390,6 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, out_dtype: Opti
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension (see
     :func:`fused_add_rms_norm`)."""
     return fused_add_rms_norm(x, weight, eps, out_dtype=out_dtype)[0]
-
-
-def _check_group(C: int, group_size: int) -> None:
-    if group_size and (group_size not in (32, 64, 128, 256, 512) or C % group_size):
-        raise ValueError(f"group_size must be 32, 64, 128, 256 or 512 and divide the width {C}, got {group_size}")
 
 
 def fused_add_rms_norm_fp8(
@@ -640,16 +411,17 @@ def fused_add_rms_norm_fp8(
     infinity has the scale NaN and q NaN.  For serving: there is no gradient,
     and a call under autograd whose inputs need one raises."""
     g = 0 if group_size is None else int(group_size)
-    if _needs_grad(x, weight, bias, res):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
         raise RuntimeError("fused_add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if group_size is not None and g == 0:
         raise ValueError("group_size must be 32, 64, 128, 256 or 512, or None for one scale a row")
     if not x.is_cuda:
-        C = _check("fused_add_rms_norm_fp8", x, bias, res, weight)
-        _same_shape("fused_add_rms_norm_fp8", x, res)
-        _check_group(C, g)
-        z = _cpu_sum(x, _vec(bias, C, "fused_add_rms_norm", "bias"), res, 0, None)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * _vec(weight, C, "fused_add_rms_norm", "weight").float()
+        _cpu_args("fused_add_rms_norm_fp8", x, bias, res, weight)
+        C = x.shape[-1]
+        if g and (g not in (32, 64, 128, 256, 512) or C % g):
+            raise ValueError(f"group_size must be 32, 64, 128, 256 or 512 and divide the width {C}, got {g}")
+        z = _cpu_sum(x, bias, res, 0, None)
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.float()
         y = y.unflatten(-1, (C // (g or C), g or C))
         top = y.abs().amax(-1, keepdim=True)
         scale = torch.where(top < FP8_MAX * 2.0**-126, 1.0, top / FP8_MAX)
@@ -657,9 +429,8 @@ def fused_add_rms_norm_fp8(
         q = (y / scale).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
         return q, scale.squeeze(-1), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
-        q, scale, z = _add_rms_norm_quant_impl(x, bias, res, weight, float(eps), g)
-    else:
-        q, scale, z = torch.ops.deberta_amd.add_rms_norm_quant(x, bias, res, weight, float(eps), g)
+        return _ext().quant(x, bias, res, weight, float(eps), g)
+    q, scale, z = torch.ops.deberta_amd.add_rms_norm_quant(x, bias, res, weight, float(eps), g)
     return q, scale, (x if _plain(bias, res, 0) else z)
 
 
@@ -667,55 +438,18 @@ def fused_add_rms_norm_fp8(
 # embedding
 
 
-def _ids_rows(ids: Tensor) -> tuple[Tensor, int]:
-    if ids.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"embed: ids must be int64 or int32, got {ids.dtype}")
-    return ids.contiguous(), ids.element_size()
-
-
 def _embed_impl(ids: Tensor, weight: Tensor, padding_idx: int, scale: float, out_dtype: torch.dtype) -> Tensor:
     """``scale * weight[ids]`` in ``out_dtype``; a row of NaN where an id is
     outside the table.  ``padding_idx`` (-1: none) matters to the gradient
     only."""
-    if weight.dim() != 2 or not weight.shape[0]:
-        raise ValueError(f"embed: weight must be (V, C) with V >= 1, got shape {tuple(weight.shape)}")
-    C = _check("embed", weight, ids)
-    idr, nb = _ids_rows(ids)
-    wr, ws = _rows(weight)
-    y = torch.empty((*ids.shape, C), dtype=out_dtype, device=ids.device)
-    a = _lib.DsaEmbedArgs(
-        ids=idr.data_ptr(), ids_bytes=nb, weight=wr.data_ptr(), weight_stride=ws, weight_dtype=_dt(weight, "embed", "weight"),
-        y=y.data_ptr(), y_stride=C, y_dtype=_dt(y, "embed", "y"), N=ids.numel(), V=weight.shape[0], C=C, padding=padding_idx,
-        scale=scale,
-    )
-    if a.N:
-        _launch("dsa_embed_fwd", a, ids)
-    return y
+    return _ext().embed_fwd(ids, weight, padding_idx, scale, out_dtype)
 
 
 def _embed_bwd_impl(
     dy: Tensor, ids: Tensor, num_embeddings: int, weight_dtype: torch.dtype, padding_idx: int, scale: float
 ) -> Tensor:
     """The gradient of the whole table, in ``weight_dtype``."""
-    C = _check("embed_bwd", dy, ids)
-    if dy.shape[:-1] != ids.shape:
-        raise ValueError(f"embed_bwd: dy must have the shape {(*ids.shape, C)}, got {tuple(dy.shape)}")
-    idr, nb = _ids_rows(ids)
-    dyr, dys = _rows(dy)
-    dw = torch.empty((num_embeddings, C), dtype=weight_dtype, device=dy.device)
-    N = ids.numel()
-    if not N:
-        return dw.zero_()
-    lib = _lib.load()
-    nws = lib.dsa_embed_workspace_bytes(N, C, num_embeddings)
-    ws = torch.empty((nws,), dtype=torch.uint8, device=dy.device)
-    a = _lib.DsaEmbedArgs(
-        ids=idr.data_ptr(), ids_bytes=nb, dy=dyr.data_ptr(), dy_stride=dys, dy_dtype=_dt(dy, "embed_bwd", "dy"),
-        dweight=dw.data_ptr(), weight_dtype=_dt(dw, "embed_bwd", "weight"), N=N, V=num_embeddings, C=C, padding=padding_idx,
-        scale=scale, workspace=ws.data_ptr(), workspace_bytes=nws,
-    )
-    _launch("dsa_embed_bwd", a, dy)
-    return dw
+    return _ext().embed_bwd(dy, ids, num_embeddings, weight_dtype, padding_idx, scale)
 
 
 embed = torch.library.custom_op("deberta_amd::embed", _embed_impl, mutates_args=(), device_types="cuda", tags=_TAGS)
@@ -735,17 +469,15 @@ def _embed_bwd_fake(dy, ids, num_embeddings, weight_dtype, padding_idx, scale):
 def _embed_setup(ctx, inputs, output):
     ids, weight, padding_idx, scale, _ = inputs
     ctx.save_for_backward(ids)
-    ctx.op_in_graph = True
     ctx.table = (weight.shape[0], weight.dtype, padding_idx, scale)
 
 
 def _embed_backward(ctx, dy):
     (ids,) = ctx.saved_tensors
-    return None, _eager.on_eager(ctx, embed_bwd, _embed_bwd_impl)(dy, ids, *ctx.table), None, None, None
+    return None, embed_bwd(dy, ids, *ctx.table), None, None, None
 
 
 torch.library.register_autograd("deberta_amd::embed", _embed_backward, setup_context=_embed_setup)
-_EmbedFunction = _eager.function("_EmbedFunction", _embed_impl, _embed_setup, _embed_backward)
 
 
 def fused_embedding(
@@ -774,12 +506,12 @@ def fused_embedding(
         pad = padding_idx % V
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     if not weight.is_cuda:
-        _ids_rows(ids)
+        if ids.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"fused_embedding: ids must be int64 or int32, got {ids.dtype}")
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
         return (y.float() * scale).to(out_dtype)
     if _eager.eager(weight):
-        run = _EmbedFunction.apply if _needs_grad(weight) else _embed_impl
-        return run(ids, weight, pad, float(scale), out_dtype)
+        return _ext().embed(ids, weight, pad, float(scale), out_dtype)
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)
 
 

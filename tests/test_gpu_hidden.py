@@ -725,6 +725,23 @@ def test_under_capture_and_twice_differentiated_they_raise(gpu):
             torch.autograd.grad(g.sum(), v)
 
 
+def test_other_transforms_raise(gpu):
+    """Forward-mode tangents and torch.func have no rule here: an error, not a
+    result without them."""
+    import torch.autograd.forward_ad as fwAD
+
+    x, w = torch.randn(4, 64, device=gpu), torch.ones(64, device=gpu)
+    for call in (lambda v: da.fused_dropout(v, 0.5, seed=1), lambda v: da.fused_rms_norm(v, w),
+                 lambda v: da.fused_embedding(torch.zeros(2, dtype=torch.int64, device=gpu), v)):
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError):
+                call(fwAD.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.expand(3, 4, 64))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v).sum())(x)
+
+
 def test_refusals_on_the_gpu(gpu):
     x, w = torch.randn(4, 64, device=gpu), torch.ones(64, device=gpu)
     with pytest.raises(TypeError, match="float32 or bfloat16"):

@@ -15,6 +15,7 @@ import ctypes
 import re
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 import pytest
@@ -200,9 +201,16 @@ def _buffers():
 
 
 def _refused(entry, a, match):
+    """The call fails with this message (in a thread of its own: the error text
+    is the thread's)."""
     lib = _lib_or_fail()
-    assert getattr(lib, entry)(ctypes.byref(a), None) != 0
-    assert re.search(match, _lib.last_error()), _lib.last_error()
+
+    def call():
+        return getattr(lib, entry)(None if a is None else ctypes.byref(a), None), _lib.last_error()
+
+    with ThreadPoolExecutor(1) as pool:
+        rc, text = pool.submit(call).result()
+    assert rc != 0 and re.search(match, text), (rc, text)
 
 
 def test_dropout_entry_refuses():
@@ -210,8 +218,7 @@ def test_dropout_entry_refuses():
     good = dict(x=at, x_stride=8, y=at, y_stride=8, N=2, C=8, threshold=100)
     for entry in ("dsa_dropout_fwd", "dsa_dropout_bwd", "dsa_add_rms_fwd", "dsa_add_rms_quant", "dsa_add_rms_bwd",
                   "dsa_embed_fwd", "dsa_embed_bwd"):
-        assert getattr(_lib_or_fail(), entry)(None, None) != 0
-        assert "null arguments" in _lib.last_error()
+        _refused(entry, None, "null arguments")
     for change, match in (
         (dict(N=0), "N in"), (dict(N=1 << 31), "N in"), (dict(C=0), "C >= 1"), (dict(threshold=65537), "threshold"),
         (dict(x=None), "bad x"), (dict(x=at + 2), "bad x"), (dict(x_stride=-1), "bad x"), (dict(x_dtype=2), "bad x"),
@@ -271,6 +278,17 @@ def test_workspaces_cover_the_partial_sums():
             # keys and positions, and two partial sums a chunk of at most 64 positions
             assert lib.dsa_embed_workspace_bytes(N, C, 1000) >= 8 * N + 2 * C * 4 * -(-N // 64)
     assert lib.dsa_embed_workspace_bytes(0, 8, 5) == 0
+
+
+# --- the host side for PyTorch tensors ---------------------------------------------------
+def test_extension_is_built_and_refuses_cpu_tensors():
+    ext = hidden._ext()
+    x, w = torch.randn(3, 8), torch.ones(8)
+    for call in (lambda: ext.dropout(x, None, None, 100, torch.tensor([1])), lambda: ext.rms(x, None, None, w, 1e-6, x.dtype, 0, None),
+                 lambda: ext.quant(x, None, None, w, 1e-6, 0), lambda: ext.embed(torch.tensor([1]), x, -1, 1.0, x.dtype),
+                 lambda: ext.embed_bwd(x, torch.tensor([0, 1, 2]), 4, x.dtype, -1, 1.0)):
+        with pytest.raises(ValueError, match="must be on the GPU"):
+            call()
 
 
 # --- the ops -----------------------------------------------------------------------------
