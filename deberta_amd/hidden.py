@@ -17,8 +17,9 @@ The kernels take float32 and bfloat16 tensors of any width, row stride and
 element alignment; arithmetic, sums and statistics are float32, and every
 result is rounded once.  In plain eager mode the functions go through
 csrc/hidden_ext.cpp (checks, memory, launches and autograd nodes in C++: the
-host time of a call is what bounds these operators on small batches).  CPU tensors run the same operators in torch
-operations, dropout with the same keep bits.  The ops under the functions
+host time of a call is what bounds these operators on small batches).  CPU
+tensors run the same operators in torch operations (float64 ones in float64),
+dropout with the same keep bits.  The ops under the functions
 (``deberta_amd::hidden_dropout``, ``add_rms_norm``, ``add_rms_norm_quant``,
 ``embed`` and the backwards) take device tensors only; like the package's
 other ops they have fake implementations and autograd, are not twice
@@ -86,6 +87,11 @@ def _stream_dtype(x: Tensor, res: Optional[Tensor]) -> torch.dtype:
     return x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
 
 
+def _wide_dtype(t: torch.dtype) -> torch.dtype:
+    """The type that the torch path computes results of type t in."""
+    return torch.promote_types(t, torch.float32)
+
+
 # ---------------------------------------------------------------------------
 # dropout's arguments
 
@@ -131,15 +137,16 @@ def hidden_keep_mask(rows: int, C: int, p: float, seed: Union[int, Tensor], devi
 
 
 def _cpu_sum(x: Tensor, bias: Optional[Tensor], res: Optional[Tensor], t: int, seed: Optional[Tensor]) -> Tensor:
-    """dropout(x + bias) + res in float32 torch operations."""
-    z = x.float()
+    """dropout(x + bias) + res in torch operations, not rounded."""
+    wide = _wide_dtype(_stream_dtype(x, res))
+    z = x.to(wide)
     if bias is not None:
-        z = z + bias.float()
+        z = z + bias.to(wide)
     if t:
         C = x.shape[-1]
         keep = hidden_keep_mask(x.numel() // C, C, t / 65536.0, seed, x.device).view(x.shape)
         z = torch.where(keep, z * (65536.0 / (65536 - t) if t < 65536 else 0.0), 0.0)
-    return z if res is None else z + res.float()
+    return z if res is None else z + res.to(wide)
 
 
 # ---------------------------------------------------------------------------
@@ -378,7 +385,7 @@ def fused_add_rms_norm(
     if not x.is_cuda:
         _cpu_args("fused_add_rms_norm", x, bias, res, weight)
         z = _cpu_sum(x, bias, res, t, s)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.float()
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.to(z.dtype)
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
         return _ext().rms(x, bias, res, weight, float(eps), out_dtype, t, s)
@@ -421,13 +428,13 @@ def fused_add_rms_norm_fp8(
         if g and (g not in (32, 64, 128, 256, 512) or C % g):
             raise ValueError(f"group_size must be 32, 64, 128, 256 or 512 and divide the width {C}, got {g}")
         z = _cpu_sum(x, bias, res, 0, None)
-        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.float()
+        y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.to(z.dtype)
         y = y.unflatten(-1, (C // (g or C), g or C))
         top = y.abs().amax(-1, keepdim=True)
         scale = torch.where(top < FP8_MAX * 2.0**-126, 1.0, top / FP8_MAX)
         scale = torch.where(top.isfinite(), scale, torch.nan)
         q = (y / scale).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
-        return q, scale.squeeze(-1), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
+        return q, scale.squeeze(-1).float(), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
     if _eager.eager(x):
         return _ext().quant(x, bias, res, weight, float(eps), g)
     q, scale, z = torch.ops.deberta_amd.add_rms_norm_quant(x, bias, res, weight, float(eps), g)
@@ -509,7 +516,7 @@ def fused_embedding(
         if ids.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"fused_embedding: ids must be int64 or int32, got {ids.dtype}")
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
-        return (y.float() * scale).to(out_dtype)
+        return (y.to(_wide_dtype(y.dtype)) * scale).to(out_dtype)
     if _eager.eager(weight):
         return _ext().embed(ids, weight, pad, float(scale), out_dtype)
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)

@@ -83,6 +83,22 @@ def test_cpu_path_matches_float64(p, with_bias, with_res):
             assert (u.double() - v).abs().max().item() <= tol
 
 
+def test_cpu_path_of_float64_tensors_computes_in_float64():
+    x, w, bias, res = _rand(3, 40, seed=1, dtype=torch.float64), _rand(40, seed=2), _rand(40, seed=3), _rand(3, 40, seed=4)
+    t = round(0.3 * 65536)
+    z = oh.dropout_add(x, bias.double(), res.double(), t, SEED)
+    y = oh.rms_norm(z, w.double(), 1e-6)
+    got_y, got_z = da.fused_add_rms_norm(x, w, 1e-6, bias=bias, res=res, dropout_p=0.3, seed=SEED)
+    # 48 half steps of 2^-53 on values below 32: 2e-13
+    for got, want in ((got_y, y), (got_z, z), (da.fused_dropout(x, 0.3, bias=bias, res=res, seed=SEED), z)):
+        assert got.dtype == torch.float64 and (got - want).abs().max().item() < 2e-13
+    ids, table = torch.tensor([2, 0]), _rand(3, 40, seed=5, dtype=torch.float64)
+    assert torch.equal(da.fused_embedding(ids, table, scale=0.3), table[ids] * 0.3)
+    leaves = [v.double().requires_grad_() for v in (x, w, bias, res)]
+    assert torch.autograd.gradcheck(
+        lambda x, w, b, r: da.fused_add_rms_norm(x, w, 1e-6, bias=b, res=r, dropout_p=0.3, seed=SEED), leaves)
+
+
 def test_cpu_embedding_and_its_gradient():
     w = _rand(11, 6, seed=1).requires_grad_()
     ids = torch.tensor([[3, 0, 3], [10, 2, 0]])
