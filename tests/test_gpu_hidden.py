@@ -27,6 +27,7 @@ type (bf16 2^-8, fp32 2^-24), element by element:
 from __future__ import annotations
 
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -693,6 +694,36 @@ def test_side_streams(gpu):
         assert all(torch.equal(u, v) for u, v in zip(want, got)) and torch.equal(wantd, gotd)
 
 
+def test_two_threads(gpu):
+    """Two threads, each on its own stream, forward and backward at once (the
+    calls release the interpreter's lock)."""
+    x, res = _rand(300, 520, seed=1, dtype=BF).to(gpu), _rand(300, 520, seed=2, dtype=FP).to(gpu)
+    ids = _zipf(5000, 700, 3).to(gpu)
+    dys = [_rand(300, 520, seed=4, dtype=FP).to(gpu), _rand(5000, 520, seed=5, dtype=FP).to(gpu)]
+
+    def norm():
+        v, w = x.detach().requires_grad_(), torch.ones(520, device=gpu, requires_grad=True)
+        y, z = da.fused_add_rms_norm(v, w, EPS, res=res, dropout_p=0.25, seed=SEED)
+        return [y, z, *torch.autograd.grad((y, z), (v, w), (dys[0], dys[0]))]
+
+    def table():
+        t = torch.ones(700, 520, device=gpu, requires_grad=True)
+        y = da.fused_dropout(da.fused_embedding(ids, t), 0.5, seed=SEED)
+        return [y, *torch.autograd.grad(y, t, dys[1])]
+
+    want = [norm(), table()]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [(norm, table)[k]() for _ in range(8)]
+            torch.cuda.current_stream().synchronize()
+            return all(torch.equal(a, b) for out in outs for a, b in zip(out, want[k]))
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(work, (0, 1))) == [True, True]
+
+
 def test_under_capture_and_twice_differentiated_they_raise(gpu):
     x = torch.randn(4, 64, device=gpu)
     w = torch.ones(64, device=gpu)
@@ -825,3 +856,31 @@ def test_far_rows(gpu):
     assert torch.equal(dw[N - 2], dy[4]) and torch.equal(dw[N // 2], dy[2]) and torch.equal(dw[3], dy[1])
     dw[[N - 1, N - 2, N // 2, 3]] = 0
     assert not dw.view(torch.int16).any()
+
+
+def test_far_rows_backward(gpu):
+    """The gradients' last rows of more than 2^31 elements, all other rows zero."""
+    C, N = 2056, (1 << 20) + 5
+    rows = [0, N // 2, N - 2, N - 1]
+    some = _rand(len(rows), C, seed=1, dtype=BF)
+    dy = torch.zeros(N, C, dtype=BF, device=gpu)
+    dy[rows] = some.to(gpu)
+    seed = torch.tensor([SEED])
+    keep = oh.keep_mask(rows, C, 32768, SEED)
+    dx, db = hidden._hidden_dropout_bwd_impl(dy, BF, FP, 32768, seed)
+    want = some.double() * keep * 2
+    assert torch.equal(dx[rows].cpu().double(), want)
+    # four values a column and zeros: three roundings
+    _within("dbias", db, want.sum(0), 4 * U * want.abs().sum(0))
+    del dx
+    w, x = torch.ones(C, device=gpu), dy
+    rstd = torch.ones(N, device=gpu)
+    z64 = some.double()
+    dx, _, dw, _ = hidden._add_rms_norm_bwd_impl(dy, None, x, None, None, w, rstd, 0, None)
+    # g = z = dy, r = 1: dx = z (1 - mean(z^2)), a mean by at most 8 (lane) + 6 (lanes) + 8 (waves)
+    # additions and a division, then a product and a difference
+    m = z64.square().mean(-1, keepdim=True)
+    wx = z64 * (1 - m)
+    _within("dx", dx[rows], wx, _half(BF) * wx.abs() + 32 * U * z64.abs() * (1 + m))
+    ww = z64.square().sum(0)
+    _within("dw", dw, ww, 8 * U * ww)
