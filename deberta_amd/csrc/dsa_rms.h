@@ -19,6 +19,12 @@
 // it waits for both): lanes past the row load its last chunk, a residual or
 // gradient that is not there is read from a tensor that is, always the same
 // row, and not used.
+//
+// HBM bounds all but the smallest: 16384 x 768 bf16 with bias, dropout and
+// residual 21.8 us forward (101 MB, 4.6 TB/s) and 30.0 backward (151 MB, 5.0),
+// 16384 x 4096 bf16 on a float32 stream 164 (940 MB, 5.7) and 270 (1342 MB,
+// 5.0); 9971 x 1024 in 8 bits 14.0 (71 MB, 5.1).  Odd bf16 widths run at 60 to
+// 85% of that: every other row then starts between two words.
 #pragma once
 
 #include <type_traits>
