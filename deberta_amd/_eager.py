@@ -14,7 +14,7 @@ the op and its fake implementation.  Both paths launch the same kernels.
 
 from __future__ import annotations
 
-from typing import Any, Callable
+from typing import Any, Callable, Optional
 
 import torch
 
@@ -36,6 +36,12 @@ def eager(t: torch.Tensor) -> bool:
         and _dispatch_depth() == 0
         and (type(t) is torch.Tensor or (type(t) is torch.nn.Parameter and not torch.jit.is_tracing()))
     )
+
+
+def plain(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether every tensor given is a plain one (or a module's parameter): a
+    subclass may hold its values elsewhere, and has to see the op."""
+    return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
 
 
 def refuse_capture(what: str) -> None:

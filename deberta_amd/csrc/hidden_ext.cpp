@@ -42,6 +42,17 @@ void check_device(const char* what, const char* name, const Tensor& t, const Ten
   TORCH_CHECK_VALUE(t.device() == x.device(), what, ": ", name, " is on ", t.device(), ", x is on ", x.device());
 }
 
+// The address of t's first element.  A tensor may have elements and no memory
+// behind them (a wrapper subclass, a parameter whose storage was freed); its
+// null pointer would read as "not given" further down.
+const void* data_of(const char* what, const char* name, const Tensor& t) {
+  if (t.numel() == 0) return nullptr;
+  const size_t need = at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(), t.storage_offset());
+  TORCH_CHECK_VALUE(t.storage().data() != nullptr && t.storage().nbytes() >= need, what, ": ", name,
+                    " has elements but no memory for them (a wrapper tensor, or its storage was freed)");
+  return t.const_data_ptr();
+}
+
 // x's width, x on the GPU
 int64_t width_of(const char* what, const Tensor& x) {
   TORCH_CHECK_VALUE(x.is_cuda(), what, ": x must be on the GPU, it is on ", x.device());
@@ -55,6 +66,7 @@ int64_t width_of(const char* what, const Tensor& x) {
 Tensor vector_of(const char* what, const char* name, const Tensor& t, int64_t C, const Tensor& x) {
   check_device(what, name, t, x);
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == C, what, " ", name, " must have shape (", C, ",), got ", t.sizes());
+  data_of(what, name, t);
   return t.contiguous();
 }
 
@@ -63,8 +75,9 @@ Tensor vector_of(const char* what, const char* name, const Tensor& t, int64_t C,
 struct Rows {
   Tensor t;
   int64_t stride;
-  explicit Rows(const Tensor& v) {
+  Rows(const char* what, const char* name, const Tensor& v) {
     const int64_t C = v.size(-1);
+    data_of(what, name, v);
     t = v.is_contiguous() || v.dim() == 2 ? v : v.reshape({-1, C});
     if (t.stride(-1) != 1 && C > 1) t = t.contiguous();
     stride = t.is_contiguous() ? C : t.stride(0);
@@ -79,11 +92,12 @@ struct Residual {
   Residual(const char* what, const Tensor& res, const Tensor& x) {
     check_device(what, "res", res, x);
     TORCH_CHECK_VALUE(res.sizes() == x.sizes(), what, ": res must have x's shape ", x.sizes(), ", got ", res.sizes());
+    data_of(what, "res", res);
     if (res.dim() == 3 && !res.is_contiguous() && (res.stride(2) == 1 || res.size(2) == 1)) {
       t = res;
       strides[0] = res.stride(0), strides[1] = res.stride(1), per_group = res.size(1);
     } else {
-      const Rows r(res);
+      const Rows r(what, "res", res);
       t = r.t;
       strides[1] = r.stride, per_group = std::max<int64_t>(1, res.numel() / res.size(-1));
     }
@@ -110,7 +124,7 @@ uint64_t seed_of(const char* what, const Maybe& seed, int64_t t) {
   if (t == 0) return 0;
   TORCH_CHECK_VALUE(has(seed) && seed->is_cpu() && seed->numel() == 1 && seed->scalar_type() == at::kLong, what,
                     ": dropout needs its seed, an int64 CPU tensor of one element");
-  return (uint64_t)*seed->const_data_ptr<int64_t>();
+  return (uint64_t)*static_cast<const int64_t*>(data_of(what, "the seed", *seed));
 }
 
 // Whether autograd has to see the call (a node refuses forward-mode tangents).
@@ -156,7 +170,7 @@ Tensor dropout_fwd(const Tensor& x, const Maybe& bias, const Maybe& res, int64_t
   }
   const Tensor y = empty(x, stream_type(x, res));
   if (a.N == 0) return y;
-  const Rows xr(x);
+  const Rows xr(what, "x", x);
   a.x = xr.t.const_data_ptr(), a.x_stride = xr.stride;
   a.y = y.data_ptr(), a.y_stride = C, a.y_dtype = type_of(y, what, "y");
   launch(dsa_dropout_fwd, "dsa_dropout_fwd", a, x);
@@ -176,7 +190,7 @@ std::tuple<Tensor, Tensor> dropout_bwd(const Tensor& dy, ScalarType x_t, std::op
   Tensor dbias = at::empty({bias_t ? C : 0}, dy.options().dtype(bias_t.value_or(x_t))), ws;
   a.dx = dx.data_ptr(), a.dx_stride = C, a.dx_dtype = type_of(dx, what, "dx");
   if (a.N == 0) return {dx, dbias.zero_()};
-  const Rows dyr(dy);
+  const Rows dyr(what, "dy", dy);
   a.dy = dyr.t.const_data_ptr(), a.dy_stride = dyr.stride;
   if (bias_t) {
     a.dbias = dbias.data_ptr(), a.bias_dtype = type_of(dbias, what, "bias");
@@ -253,7 +267,7 @@ struct Rms {
       a.res_strides[0] = res->strides[0], a.res_strides[1] = res->strides[1], a.rows_per_group = res->per_group;
     }
     if (a.N) {
-      x.emplace(xt);
+      x.emplace(what, "x", xt);
       a.x = x->t.const_data_ptr(), a.x_stride = x->stride;
     }
   }
@@ -301,20 +315,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_bwd(const Tensor& dy, const Maybe
   check_device(what, "rstd", rstd, x);
   TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), what, ": dy must have x's shape ", x.sizes(), ", got ", dy.sizes());
   TORCH_CHECK_VALUE(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == m.a.N, what, ": bad rstd");
+  data_of(what, "rstd", rstd);
   const Tensor dx = empty(x, x.scalar_type());
   const bool apart = has(res) && (t != 0 || res->scalar_type() != x.scalar_type());
   const Tensor dres = apart ? empty(x, res->scalar_type()) : at::empty({0}, x.options());
   Tensor dweight = at::empty_like(m.weight);
   Tensor dbias = has(bias) ? at::empty_like(m.bias) : at::empty({0}, weight.options());
   if (m.a.N == 0) return {dx, dres, dweight.zero_(), dbias.zero_()};
-  const Rows dyr(dy);
+  const Rows dyr(what, "dy", dy);
   std::optional<Rows> dzr;
   m.a.dy = dyr.t.const_data_ptr(), m.a.dy_stride = dyr.stride, m.a.dy_dtype = type_of(dy, what, "dy");
   m.a.rstd = rstd.data_ptr<float>();
   if (has(dz)) {
     check_device(what, "dz", *dz, x);
     TORCH_CHECK_VALUE(dz->sizes() == x.sizes(), what, ": dz must have x's shape ", x.sizes(), ", got ", dz->sizes());
-    dzr.emplace(dz->to(stream_type(x, res)));
+    dzr.emplace(what, "dz", dz->to(stream_type(x, res)));
     m.a.dzu = dzr->t.const_data_ptr(), m.a.dzu_stride = dzr->stride;
   }
   m.a.dx = dx.data_ptr(), m.a.dx_stride = m.a.C;
@@ -415,6 +430,7 @@ Tensor ids_of(const char* what, const Tensor& ids, const Tensor& x) {
   TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "embed: ids must be int64 or int32, got ",
                    ids.scalar_type());
   TORCH_CHECK_VALUE(ids.device() == x.device(), what, ": ids are on ", ids.device(), ", the weight or its gradient on ", x.device());
+  data_of(what, "ids", ids);
   return ids.contiguous();
 }
 
@@ -423,7 +439,7 @@ Tensor embed_fwd(const Tensor& ids, const Tensor& weight, int64_t padding, doubl
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) > 0, what, ": weight must be (V, C) with V >= 1, got shape ", weight.sizes());
   const int64_t C = width_of(what, weight);
   const Tensor idr = ids_of(what, ids, weight);
-  const Rows w(weight);
+  const Rows w(what, "weight", weight);
   auto shape = ids.sizes().vec();
   shape.push_back(C);
   const Tensor y = at::empty(shape, weight.options().dtype(out));
@@ -450,7 +466,7 @@ Tensor embed_bwd(const Tensor& dy, const Tensor& ids, int64_t V, ScalarType weig
   a.dy_dtype = type_of(dy, what, "dy");
   a.N = ids.numel(), a.V = V, a.C = (int32_t)C, a.padding = padding, a.scale = (float)scale;
   if (a.N == 0) return dw.zero_();
-  const Rows dyr(dy);
+  const Rows dyr(what, "dy", dy);
   a.ids = idr.const_data_ptr(), a.ids_bytes = (int32_t)idr.element_size();
   a.dy = dyr.t.const_data_ptr(), a.dy_stride = dyr.stride;
   const size_t n = dsa_embed_workspace_bytes(a.N, a.C, V);

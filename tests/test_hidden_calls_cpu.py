@@ -1,0 +1,79 @@
+"""How calls of the hidden-state operators are routed and checked, without a
+GPU: what goes past ``torch.ops`` into the extension and what must not, which
+extension is loaded, where seeds are drawn, what the build needs, and what the
+torch path of CPU tensors sums in.
+
+A call on device tensors is seen here by letting CPU tensors say that they are
+on the GPU, with a recorder in the extension's place: calls that reach the
+recorder went past ``torch.ops``, calls that reach the op find no CPU kernel.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import deberta_amd as da
+from deberta_amd import hidden
+from tests._hidden import Wrapper
+
+
+class _Recorder:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append(name)
+            return args[1] if name == "embed" else (args[0], args[0], args[0])
+
+        return call
+
+
+@pytest.fixture
+def as_on_gpu(monkeypatch):
+    """CPU tensors that say they are on the GPU; the extension's recorder."""
+    ext = _Recorder()
+    monkeypatch.setattr(hidden, "_ext", lambda: ext)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    return ext
+
+
+def _calls(x, bias, res, w, ids):
+    return {
+        "dropout": lambda: da.fused_dropout(x, 0.5, bias=bias, res=res, seed=1),
+        "rms": lambda: da.fused_add_rms_norm(x, w, bias=bias, res=res),
+        "quant": lambda: da.fused_add_rms_norm_fp8(x, w, bias=bias, res=res),
+        "embed": lambda: da.fused_embedding(ids, x),
+    }
+
+
+def test_plain_tensors_go_into_the_extension(as_on_gpu):
+    x, w = torch.randn(3, 8), torch.nn.Parameter(torch.ones(8), requires_grad=False)
+    for name, call in _calls(x, w, x, w, torch.tensor([1])).items():
+        call()
+        assert as_on_gpu.calls == [name]
+        as_on_gpu.calls.clear()
+
+
+@pytest.mark.parametrize("which", ["bias", "res", "weight", "ids"])
+def test_a_wrapper_in_any_argument_sees_the_op(which, as_on_gpu):
+    """The extension reads addresses, and a wrapper has none: a bias or a
+    residual of that kind would be left out of the result."""
+    x, b, r, w, ids = torch.randn(3, 8), torch.ones(8), torch.randn(3, 8), torch.ones(8), torch.tensor([1])
+    if which == "bias":
+        b = Wrapper(b)
+    elif which == "res":
+        r = Wrapper(r)
+    elif which == "weight":
+        w = Wrapper(w)
+    else:
+        ids = Wrapper(ids)
+    reached = {"bias": ("dropout", "rms", "quant"), "res": ("dropout", "rms", "quant"), "weight": ("rms", "quant"),
+               "ids": ("embed",)}[which]
+    calls = _calls(x, b, r, w, ids)
+    for name in reached:
+        Wrapper.seen.clear()
+        with pytest.raises(NotImplementedError):  # the op, on tensors that are on the CPU after all
+            calls[name]()
+        assert as_on_gpu.calls == [] and any("deberta_amd" in str(f) for f in Wrapper.seen), name
