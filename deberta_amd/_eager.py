@@ -38,10 +38,17 @@ def eager(t: torch.Tensor) -> bool:
     )
 
 
-def plain(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether every tensor given is a plain one (or a module's parameter): a
-    subclass may hold its values elsewhere, and has to see the op."""
-    return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+def eager_all(t: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """:func:`eager` for a call that goes into an extension, past Python
+    autograd functions too.  Every tensor given has to be a plain one or a
+    module's parameter: a subclass may hold its values elsewhere, and has to
+    see the op.  torch.jit.trace records the extension's empty results and not
+    its launches, so a traced call is the op's as well."""
+    return (
+        eager(t)
+        and not torch.jit.is_tracing()
+        and all(o is None or type(o) is torch.Tensor or type(o) is torch.nn.Parameter for o in others)
+    )
 
 
 def refuse_capture(what: str) -> None:

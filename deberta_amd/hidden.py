@@ -232,7 +232,7 @@ def fused_dropout(
     if not x.is_cuda:
         _cpu_args("fused_dropout", x, bias, res)
         return _cpu_sum(x, bias, res, t, s).to(_stream_dtype(x, res))
-    if _eager.eager(x) and _eager.plain(bias, res, s):
+    if _eager.eager_all(x, bias, res, s):
         return _ext().dropout(x, bias, res, t, s)
     return torch.ops.deberta_amd.hidden_dropout(x, bias, res, t, s)
 
@@ -387,7 +387,7 @@ def fused_add_rms_norm(
         z = _cpu_sum(x, bias, res, t, s)
         y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.to(z.dtype)
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
-    if _eager.eager(x) and _eager.plain(bias, res, weight, s):
+    if _eager.eager_all(x, bias, res, weight, s):
         return _ext().rms(x, bias, res, weight, float(eps), out_dtype, t, s)
     y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
     return y, (x if _plain(bias, res, t) else z)
@@ -435,7 +435,7 @@ def fused_add_rms_norm_fp8(
         scale = torch.where(top.isfinite(), scale, torch.nan)
         q = (y / scale).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
         return q, scale.squeeze(-1).float(), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
-    if _eager.eager(x) and _eager.plain(bias, res, weight):
+    if _eager.eager_all(x, bias, res, weight):
         return _ext().quant(x, bias, res, weight, float(eps), g)
     q, scale, z = torch.ops.deberta_amd.add_rms_norm_quant(x, bias, res, weight, float(eps), g)
     return q, scale, (x if _plain(bias, res, 0) else z)
@@ -517,7 +517,7 @@ def fused_embedding(
             raise TypeError(f"fused_embedding: ids must be int64 or int32, got {ids.dtype}")
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
         return (y.to(_wide_dtype(y.dtype)) * scale).to(out_dtype)
-    if _eager.eager(weight) and _eager.plain(ids):
+    if _eager.eager_all(weight, ids):
         return _ext().embed(ids, weight, pad, float(scale), out_dtype)
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)
 

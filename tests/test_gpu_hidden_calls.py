@@ -72,3 +72,62 @@ def test_tensors_without_memory_are_refused(gpu):
     ):
         with pytest.raises(ValueError, match="no memory"):
             call()
+
+
+class _Path(torch.nn.Module):
+    def __init__(self, grad):
+        super().__init__()
+        for k, (name, shape) in enumerate((("table", (40, 64)), ("w", (64,)), ("b", (64,)))):
+            setattr(self, name, torch.nn.Parameter(_rand(*shape, seed=k), requires_grad=grad))
+
+    def forward(self, ids, res):
+        e = da.fused_embedding(ids, self.table, padding_idx=0, scale=2.0)
+        e = da.fused_dropout(e, 0.25, seed=SEED)
+        return da.fused_add_rms_norm(e, self.w, bias=self.b, res=res, dropout_p=0.5, seed=SEED)
+
+
+class _Eight(_Path):
+    def forward(self, r):
+        return da.fused_add_rms_norm_fp8(r, self.w, res=r)
+
+
+def _traced(m, *inputs):
+    """m's trace; memory freed afterwards holds NaN, which a result that is
+    only allocated would return."""
+    t = torch.jit.trace(m, inputs, check_trace=False)
+    junk = [torch.full((3, 5, 64), float("nan"), device=inputs[0].device) for _ in range(8)]
+    del junk
+    return t
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls_compute(grad, gpu):
+    """A traced module runs the kernels again on new inputs: equal to the
+    eager calls, with gradients."""
+    m = _Path(grad).to(gpu)
+    ids, res = torch.randint(0, 40, (3, 5), generator=torch.Generator().manual_seed(1)).to(gpu), _rand(3, 5, 64, seed=5).to(gpu)
+    traced = _traced(m, ids, res)
+    ids, res = ids.flip(0), res * 2
+    got, want = traced(ids, res), m(ids, res)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if grad:
+        dy = _rand(3, 5, 64, seed=6).to(gpu)
+        g, h = (torch.autograd.grad(o, list(m.parameters()), (dy, dy)) for o in (got, want))
+        assert all(torch.equal(a, b) for a, b in zip(g, h))
+
+
+def test_traced_eight_bit_rows_compute(gpu):
+    m, res = _Eight(False).to(gpu), _rand(3, 5, 64, seed=5).to(gpu)
+    traced = _traced(m, res)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(traced(res * 3), m(res * 3)))
+
+
+def test_a_traced_rtd_head_computes(gpu):
+    from oracle import eager
+
+    cfg = eager.make_config(hidden_size=64, num_attention_heads=4, intermediate_size=128, layer_norm_eps=1e-7, use_rmsnorm_heads=True)
+    head = da.FusedRTDHead(cfg).to(gpu).eval()
+    with torch.no_grad():
+        h = _rand(2, 9, 64, seed=1).to(gpu)
+        traced = _traced(head, h)
+        assert torch.equal(traced(h * 2), head(h * 2))

@@ -77,3 +77,18 @@ def test_a_wrapper_in_any_argument_sees_the_op(which, as_on_gpu):
         with pytest.raises(NotImplementedError):  # the op, on tensors that are on the CPU after all
             calls[name]()
         assert as_on_gpu.calls == [] and any("deberta_amd" in str(f) for f in Wrapper.seen), name
+
+
+def test_a_traced_call_is_the_op(as_on_gpu):
+    """torch.jit.trace records what the extension allocates, not what it
+    launches: a trace of its calls would return memory that nothing wrote."""
+    x, w, ids = torch.randn(3, 8), torch.ones(8), torch.tensor([1])
+    for name, call in _calls(x, w, x, w, ids).items():
+
+        def traced(_):
+            with pytest.raises(NotImplementedError):
+                call()
+            return torch.zeros(1)
+
+        torch.jit.trace(traced, (torch.zeros(1),), check_trace=False)
+        assert as_on_gpu.calls == [], name
