@@ -515,8 +515,11 @@ def fused_embedding(
     if not weight.is_cuda:
         if ids.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"fused_embedding: ids must be int64 or int32, got {ids.dtype}")
+        wide = _wide_dtype(weight.dtype)
+        if torch.is_grad_enabled() and weight.requires_grad:
+            weight = weight.to(wide)  # before the lookup: its gradient sums a token's positions in this type
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
-        return (y.to(_wide_dtype(y.dtype)) * scale).to(out_dtype)
+        return (y.to(wide) * scale).to(out_dtype)
     if _eager.eager_all(weight, ids):
         return _ext().embed(ids, weight, pad, float(scale), out_dtype)
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)

@@ -15,6 +15,7 @@ import torch
 
 import deberta_amd as da
 from deberta_amd import hidden
+from oracle import hidden as oh
 from tests._hidden import Wrapper
 
 
@@ -94,3 +95,22 @@ def test_a_traced_call_is_the_op(as_on_gpu, monkeypatch):
 
     torch.jit.trace(f, (x,), check_trace=False)
     assert as_on_gpu.calls == [] and ops.calls == ["hidden_dropout", "add_rms_norm", "add_rms_norm_quant", "embed"]
+
+
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16, torch.float32])
+def test_cpu_embedding_gradient_sums_in_float32(wt):
+    """A token at 4000 positions: 4000 additions in float32 and one rounding,
+    on the sum of magnitudes (torch's own gradient of a bf16 table stops
+    growing at 256 times a position's)."""
+    u, h = 2.0**-24, torch.finfo(wt).eps / 2
+    table = torch.randn(5, 6, generator=torch.Generator().manual_seed(1)).to(wt).requires_grad_()
+    ids = torch.full((4000,), 3)
+    ids[::1000] = 1
+    for out, dy in ((wt, torch.ones(4000, 6, dtype=wt)),
+                    (torch.float32, torch.randn(4000, 6, generator=torch.Generator().manual_seed(2)))):
+        y = da.fused_embedding(ids, table, padding_idx=1, scale=0.5, out_dtype=out)
+        assert y.dtype == out and torch.equal(y, (table.detach().float()[ids] * 0.5).to(out))
+        (g,) = torch.autograd.grad(y, table, dy)
+        want = oh.embedding_grad(ids, dy.double(), 5, 1, 0.5)
+        most = oh.embedding_grad(ids, dy.double().abs(), 5, 1, 0.5)
+        assert g.dtype == wt and ((g.double() - want).abs() <= 4001 * u * most + h * want.abs()).all()
