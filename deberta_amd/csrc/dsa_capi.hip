@@ -426,7 +426,7 @@ dsa::rows::RtdParams rtd_params(const dsa_rtd_args* a) {
 
 extern "C" {
 
-int dsa_version(void) { return 14; }
+int dsa_version(void) { return DSA_VERSION; }
 
 const char* dsa_last_error(void) { return g_err.c_str(); }
 

@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/version.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -505,6 +506,8 @@ Tensor embed(const Tensor& ids, const Tensor& weight, int64_t padding, double sc
 // The functions named like an operator record autograd; _fwd and _bwd are what
 // the registered ops call.
 PYBIND11_MODULE(_hidden_ext, m) {
+  m.attr("abi_version") = DSA_VERSION;      // whose structs it passes
+  m.attr("torch_version") = TORCH_VERSION;  // whose classes it was compiled with
   m.def("dropout", torch::wrap_pybind_function_no_gil(dropout));
   m.def("dropout_fwd", torch::wrap_pybind_function_no_gil(dropout_fwd));
   m.def("dropout_bwd", torch::wrap_pybind_function_no_gil(dropout_bwd));

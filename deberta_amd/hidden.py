@@ -66,6 +66,11 @@ def _ext() -> Any:
         )
     from deberta_amd import _hidden_ext
 
+    # an extension left from an earlier build would pass its own structs to the library, or hold torch's older ones
+    built = (getattr(_hidden_ext, "abi_version", None), getattr(_hidden_ext, "torch_version", None))
+    need = (_lib.EXPECTED_VERSION, torch.__version__.split("+")[0])
+    if built != need:
+        raise RuntimeError(f"{EXT_PATH} was built for (ABI, torch) versions {built}, expected {need}; rebuild it")
     return _hidden_ext
 
 

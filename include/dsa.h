@@ -298,7 +298,10 @@ size_t dsa_fwd_workspace_bytes(const dsa_fwd_args* args);
 /* Thread-local description of the last error (empty string if none). */
 const char* dsa_last_error(void);
 
-/* Library version, for the loader's compatibility check. */
+/* Library version, for the loader's compatibility check: DSA_VERSION of the
+ * headers that the library was built from.  Code compiled against these headers
+ * compares the two before it passes a struct. */
+#define DSA_VERSION 14
 int dsa_version(void);
 
 #ifdef __cplusplus

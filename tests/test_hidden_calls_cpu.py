@@ -10,11 +10,15 @@ recorder went past ``torch.ops``, calls that reach the op find no CPU kernel.
 
 from __future__ import annotations
 
+import re
+import types
+from pathlib import Path
+
 import pytest
 import torch
 
 import deberta_amd as da
-from deberta_amd import hidden
+from deberta_amd import _lib, hidden
 from oracle import hidden as oh
 from tests._hidden import Wrapper
 
@@ -114,3 +118,29 @@ def test_cpu_embedding_gradient_sums_in_float32(wt):
         want = oh.embedding_grad(ids, dy.double(), 5, 1, 0.5)
         most = oh.embedding_grad(ids, dy.double().abs(), 5, 1, 0.5)
         assert g.dtype == wt and ((g.double() - want).abs() <= 4001 * u * most + h * want.abs()).all()
+
+
+@pytest.fixture
+def fresh_ext():
+    hidden._ext.cache_clear()
+    yield
+    hidden._ext.cache_clear()
+
+
+@pytest.mark.parametrize("change", [None, {"abi_version": -1}, {"torch_version": "1.0.0"}], ids=str)
+def test_an_extension_of_another_build_is_refused(change, fresh_ext, monkeypatch):
+    """It would pass structs of another layout to the library."""
+    own = hidden._ext()
+    old = types.ModuleType("_hidden_ext")  # change None: one from before the versions were kept
+    if change is not None:
+        vars(old).update({"abi_version": own.abi_version, "torch_version": own.torch_version, **change})
+    monkeypatch.setattr(da, "_hidden_ext", old)
+    hidden._ext.cache_clear()
+    with pytest.raises(RuntimeError, match="rebuild"):
+        hidden._ext()
+
+
+def test_the_headers_version_is_the_loaders():
+    header = (Path(__file__).resolve().parents[1] / "include" / "dsa.h").read_text()
+    (version,) = re.findall(r"#define DSA_VERSION (\d+)", header)
+    assert int(version) == _lib.EXPECTED_VERSION == _lib.load().dsa_version() == hidden._ext().abi_version
