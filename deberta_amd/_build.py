@@ -1,6 +1,7 @@
 """Builds ``libdsa.so`` (the HIP kernels and their C ABI) in-tree with hipcc for
 gfx950, and ``_hidden_ext.so`` (the host side of the operators on hidden
-states: PyTorch tensors and autograd over that C ABI) with g++."""
+states: PyTorch tensors and autograd over that C ABI) with g++, or the ROCm
+toolchain's own clang++ where there is no g++."""
 
 from __future__ import annotations
 
@@ -9,6 +10,7 @@ import shutil
 import subprocess
 import sysconfig
 import tempfile
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -83,17 +85,38 @@ def _compile(sources, out: Path, verbose: bool) -> Path:
     return out
 
 
+def _host_compiler() -> str:
+    """A C++ compiler for host code: hipcc brings one."""
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    for found in (shutil.which("g++"), shutil.which("c++"), rocm / "llvm" / "bin" / "clang++", shutil.which("clang++")):
+        if found and Path(found).exists():
+            return str(found)
+    raise RuntimeError("no C++ compiler found: _hidden_ext.so cannot be built")
+
+
+def _ext_include() -> list[Path]:
+    """The extension's header folders: torch's, Python's and ROCm's."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent / "include"
+    return [root, root / "torch" / "csrc" / "api" / "include", Path(sysconfig.get_paths()["include"]),
+            Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"]
+
+
+def _missing_headers() -> list[str]:
+    """What the extension includes and this machine does not have (an
+    installation of torch or Python without its C++ headers)."""
+    torch_include, _, python_include, _ = _ext_include()
+    need = (torch_include / "torch" / "csrc" / "autograd" / "custom_function.h", python_include / "Python.h")
+    return [str(p) for p in need if not p.exists()]
+
+
 def _ext_commands(obj: Path, out: Path) -> tuple[list[str], list[str]]:
     """(compile, link) of the extension.  It finds libdsa.so beside itself and
     torch's libraries where the process has loaded them."""
     import torch
 
-    cxx = shutil.which("g++") or shutil.which("c++")
-    if cxx is None:
-        raise RuntimeError("g++ not found: _hidden_ext.so cannot be built")
-    root = Path(torch.__file__).resolve().parent
-    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
-               Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"]
+    cxx, root, include = _host_compiler(), Path(torch.__file__).resolve().parent, _ext_include()
     flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     compile_cmd = [cxx, *flags, *(f"-isystem{p}" for p in include), "-c", str(EXT_SOURCE), "-o", str(obj)]
@@ -117,7 +140,17 @@ def build(verbose: bool = False) -> Path:
     Always recompiles.  Each library is written to a temporary name first and
     renamed into place, so a process that already loaded the old file keeps a
     consistent image.
+
+    Where torch's or Python's C++ headers are not installed the kernels are
+    built alone, with a warning: the operators on hidden states then raise on
+    device tensors, everything else runs.
     """
+    missing = _missing_headers()
+    if missing:
+        warnings.warn(f"{EXT_PATH.name} is not built, {', '.join(missing)} not found: the operators on hidden states will not run")
+        EXT_PATH.unlink(missing_ok=True)  # not to be taken for this build's
+        _compile(PROBE_SOURCES, PROBE_PATH, verbose)
+        return _compile(SOURCES, LIB_PATH, verbose)
     with tempfile.TemporaryDirectory(dir=PKG_DIR, prefix="_build") as tmp_dir, ThreadPoolExecutor(1) as pool:
         tmp = EXT_PATH.with_suffix(".so.tmp")
         compile_cmd, link_cmd = _ext_commands(Path(tmp_dir) / "ext.o", tmp)

@@ -11,6 +11,8 @@ recorder went past ``torch.ops``, calls that reach the op find no CPU kernel.
 from __future__ import annotations
 
 import re
+import shutil
+import subprocess
 import types
 from pathlib import Path
 
@@ -18,7 +20,7 @@ import pytest
 import torch
 
 import deberta_amd as da
-from deberta_amd import _lib, hidden
+from deberta_amd import _build, _lib, hidden
 from oracle import hidden as oh
 from tests._hidden import Wrapper
 
@@ -144,3 +146,23 @@ def test_the_headers_version_is_the_loaders():
     header = (Path(__file__).resolve().parents[1] / "include" / "dsa.h").read_text()
     (version,) = re.findall(r"#define DSA_VERSION (\d+)", header)
     assert int(version) == _lib.EXPECTED_VERSION == _lib.load().dsa_version() == hidden._ext().abi_version
+
+
+def test_the_build_without_gcc_takes_rocms_compiler(monkeypatch, tmp_path):
+    """hipcc needs no g++, and neither does the extension."""
+    which = shutil.which
+    monkeypatch.setattr(shutil, "which", lambda name: None if name in ("g++", "c++") else which(name))
+    compile_cmd, _ = _build._ext_commands(tmp_path / "ext.o", tmp_path / "ext.so")
+    assert Path(compile_cmd[0]).name == "clang++"
+    subprocess.run([*(a for a in compile_cmd if a != "-O2"), "-fsyntax-only"], check=True)
+
+
+def test_the_build_without_torchs_headers_builds_the_kernels(monkeypatch, tmp_path):
+    built = []
+    monkeypatch.setattr(_build, "_compile", lambda sources, out, verbose: built.append(out) or out)
+    monkeypatch.setattr(_build, "_ext_include", lambda: [tmp_path] * 4)
+    monkeypatch.setattr(_build, "EXT_PATH", tmp_path / "_hidden_ext.so")
+    _build.EXT_PATH.write_text("an earlier build's")
+    with pytest.warns(UserWarning, match="custom_function.h"):
+        assert _build.build() == _build.LIB_PATH
+    assert built == [_build.PROBE_PATH, _build.LIB_PATH] and not _build.EXT_PATH.exists()
