@@ -19,7 +19,7 @@ namespace hid = dsa::hid;
 namespace dsa {
 namespace host {
 #define DSA_EXTERN(TX, TR)                                                                  \
-  extern template int launch_rms_fwd<TX, TR>(const hid::RmsRows&, int, hipStream_t);        \
+  extern template int launch_rms_fwd<TX, TR>(hid::RmsRows, int, hipStream_t);               \
   extern template int launch_rms_bwd<TX, TR>(const hid::RmsRows&, int, int64_t, hipStream_t);
 DSA_EXTERN(bf16, bf16)
 DSA_EXTERN(bf16, float)

@@ -42,6 +42,7 @@ struct RmsRows {
   float *rstd, *yscale, *part;
   int64_t xs, xe, rs0, rs1, re, ys, zs, dys, dye, dzus, dzue, dxs, drs;
   uint32_t N, rpg;
+  uint32_t r0;         // forward: the launch's first row
   int C, bias_dt, w_dt, group;
   int has_res, has_u;  // whether res and dzu are there
   int rows;            // backward: rows a team takes
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(rms_threads<W>()) void rms_fwd_kernel(RmsRows p) {
   __shared__ float buf[2 * W];
   const Place<L, NC, W, TAIL> at(p.C);
   const int lane = at.lane, wr = at.wr;
-  const uint32_t r = blockIdx.x * (uint32_t)rms_teams<L, W>() + at.wv / W * (64 / L) + (L < 64 ? lane / L : 0);
+  const uint32_t r = p.r0 + blockIdx.x * (uint32_t)rms_teams<L, W>() + at.wv / W * (64 / L) + (L < 64 ? lane / L : 0);
   if (r >= p.N) return;  // the whole team; a block has barriers only where it is one team
   RawZ<NC, TX, TR, TAIL> raw;
   raw.load(p, r, at);

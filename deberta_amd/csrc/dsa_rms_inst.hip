@@ -4,7 +4,7 @@
 
 namespace dsa {
 namespace host {
-template int launch_rms_fwd<DSA_TX, DSA_TR>(const hid::RmsRows&, int, hipStream_t);
+template int launch_rms_fwd<DSA_TX, DSA_TR>(hid::RmsRows, int, hipStream_t);
 template int launch_rms_bwd<DSA_TX, DSA_TR>(const hid::RmsRows&, int, int64_t, hipStream_t);
 }  // namespace host
 }  // namespace dsa

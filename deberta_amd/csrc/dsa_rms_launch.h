@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "dsa_host.h"
@@ -65,17 +66,24 @@ void by_tail(int C, F f) {
 template <typename TX, typename TR>
 using stream_t = std::conditional_t<std::is_same<TX, TR>::value, TX, float>;
 
+// One launch for all rows, or for as many as its 2^32 - 1 threads hold (2^28
+// rows of at most 128 columns).
 template <typename TX, typename TR>
-int launch_rms_fwd(const hid::RmsRows& p, int y_dt, hipStream_t st) {
+int launch_rms_fwd(hid::RmsRows p, int y_dt, hipStream_t st) {
   typedef stream_t<TX, TR> TZ;
   by_width<false>(p.C, [&](auto l, auto nc, auto w) {
     by_tail(p.C, [&](auto tail) {
       constexpr int L = decltype(l)::value, NC = decltype(nc)::value, W = decltype(w)::value;
       constexpr bool T = decltype(tail)::value;
-      const dim3 grid((unsigned)cdiv(p.N, hid::rms_teams<L, W>())), block(hid::rms_threads<W>());
-      if (y_dt == kFp8) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, hid::fp8, T>), grid, block, 0, st, p);
-      else if (y_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
-      else hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
+      const dim3 block(hid::rms_threads<W>());
+      const int64_t most = 0xffffffffLL / block.x;  // blocks
+      for (int64_t b = 0, all = cdiv(p.N, hid::rms_teams<L, W>()); b < all; b += most) {
+        const dim3 grid((unsigned)std::min(most, all - b));
+        p.r0 = (uint32_t)(b * hid::rms_teams<L, W>());
+        if (y_dt == kFp8) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, hid::fp8, T>), grid, block, 0, st, p);
+        else if (y_dt == DSA_BF16) hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, bf16, T>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((hid::rms_fwd_kernel<L, NC, W, TX, TR, TZ, float, T>), grid, block, 0, st, p);
+      }
     });
   });
   return launch_check("rms_fwd_kernel");

@@ -10,11 +10,14 @@ import torch
 
 import deberta_amd as da
 from deberta_amd import hidden
+from oracle import hidden as oh
 from tests._hidden import Wrapper
 
 pytestmark = pytest.mark.gpu
 
-FP = torch.float32
+BF, FP = torch.bfloat16, torch.float32
+U = 2.0**-24
+EPS = 1e-6
 SEED = 0x3_1234_5678_9ABC
 
 
@@ -131,3 +134,29 @@ def test_a_traced_rtd_head_computes(gpu):
         h = _rand(2, 9, 64, seed=1).to(gpu)
         traced = _traced(head, h)
         assert torch.equal(traced(h * 2), head(h * 2))
+
+
+def test_more_rows_than_one_launch_holds(gpu):
+    """2^28 rows of eight columns are one more than 2^32 - 1 threads; the keep
+    bits show that a row keeps its number.  A norm of eight values: 8 squares,
+    8 additions, a division, a root and two products, under 24 half steps."""
+    C, N = 8, (1 << 28) + 37
+    rows = [0, 17, (1 << 28) - 17, (1 << 28) - 16, (1 << 28) - 1, 1 << 28, N - 2, N - 1]
+    some, one = _rand(len(rows), C, seed=1, dtype=BF), torch.ones(C, dtype=torch.float64)
+    x, w = torch.zeros(N, C, dtype=BF, device=gpu), torch.ones(C, device=gpu)
+    x[rows] = some.to(gpu)
+    z64 = some.double() * oh.keep_mask(rows, C, 32768, SEED) * 2
+    y, z = da.fused_add_rms_norm(x, w, EPS, dropout_p=0.5, seed=SEED)
+    assert torch.equal(z[rows].cpu().double(), z64)
+    y64 = oh.rms_norm(z64, one, EPS)
+    assert ((y[rows].cpu().double() - y64).abs() <= (24 * U + 2.0**-8) * y64.abs()).all()
+    y[rows] = 0
+    assert not y.view(torch.int16).any()
+    del y, z
+    with torch.no_grad():
+        q, s, _ = da.fused_add_rms_norm_fp8(x, w, EPS)
+    got = q[rows].cpu().float() * s[rows].cpu()
+    y64 = oh.rms_norm(some.double(), one, EPS)
+    assert ((got.double() - y64).abs() <= (2.0**-4 + 32 * U) * y64.abs() + 2.0**-10 * s[rows].cpu().double()).all()
+    s[rows] = 1
+    assert (s == 1).all()
