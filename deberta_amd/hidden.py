@@ -117,7 +117,7 @@ def _seed_tensor(seed: Union[None, int, Tensor]) -> Tensor:
     if isinstance(seed, int) and not isinstance(seed, bool):
         if not 0 <= seed < 1 << 63:
             raise ValueError(f"dropout seed must be in [0, 2^63), got {seed}")
-        return torch.tensor([seed], dtype=torch.int64)
+        return torch.tensor([seed], dtype=torch.int64, device="cpu")
     if not isinstance(seed, Tensor) or seed.numel() != 1 or seed.dtype != torch.int64 or seed.device.type != "cpu":
         raise ValueError("dropout seed must be an int or an int64 CPU tensor of one element")
     return seed

@@ -114,7 +114,7 @@ def draw_dropout_seed() -> Tensor:
     """A fresh 62-bit seed for the keep bits, drawn from torch's default CPU
     generator (so ``torch.manual_seed`` reproduces it, and activation
     checkpointing, which restores the RNG states, redraws the same one)."""
-    return torch.randint(0, 1 << 62, (1,), dtype=torch.int64)
+    return torch.randint(0, 1 << 62, (1,), dtype=torch.int64, device="cpu")  # whatever the default device is
 
 
 def _seed_value(seed: Optional[Tensor], t: int) -> int:

@@ -166,3 +166,15 @@ def test_the_build_without_torchs_headers_builds_the_kernels(monkeypatch, tmp_pa
     with pytest.warns(UserWarning, match="custom_function.h"):
         assert _build.build() == _build.LIB_PATH
     assert built == [_build.PROBE_PATH, _build.LIB_PATH] and not _build.EXT_PATH.exists()
+
+
+def test_seeds_are_on_the_cpu_whatever_the_default_device():
+    """As under torch.set_default_device("cuda"): a seed of the default device
+    was refused, and would have been drawn from its generator."""
+    x = torch.ones(4, 100)
+    torch.manual_seed(3)
+    want = da.fused_dropout(x, 0.5), da.fused_dropout(x, 0.5, seed=9), da.hidden_keep_mask(4, 100, 0.5, 9)
+    torch.manual_seed(3)
+    with torch.device("meta"):
+        got = da.fused_dropout(x, 0.5), da.fused_dropout(x, 0.5, seed=9), da.hidden_keep_mask(4, 100, 0.5, 9)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
