@@ -43,15 +43,17 @@ void check_device(const char* what, const char* name, const Tensor& t, const Ten
   TORCH_CHECK_VALUE(t.device() == x.device(), what, ": ", name, " is on ", t.device(), ", x is on ", x.device());
 }
 
-// The address of t's first element.  A tensor may have elements and no memory
-// behind them (a wrapper subclass, a parameter whose storage was freed); its
-// null pointer would read as "not given" further down.
-const void* data_of(const char* what, const char* name, const Tensor& t) {
-  if (t.numel() == 0) return nullptr;
+// t with its values in memory as they count.  A tensor may have elements and no
+// memory behind them (a wrapper subclass, a parameter whose storage was freed);
+// its null pointer would read as "not given" further down.  And its sign may be
+// pending: the imaginary part of a conjugated tensor is a view of the values
+// before their negation, which is made here.
+Tensor held(const char* what, const char* name, const Tensor& t) {
+  if (t.numel() == 0) return t;
   const size_t need = at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(), t.storage_offset());
   TORCH_CHECK_VALUE(t.storage().data() != nullptr && t.storage().nbytes() >= need, what, ": ", name,
                     " has elements but no memory for them (a wrapper tensor, or its storage was freed)");
-  return t.const_data_ptr();
+  return t.resolve_neg();
 }
 
 // x's width, x on the GPU
@@ -67,8 +69,7 @@ int64_t width_of(const char* what, const Tensor& x) {
 Tensor vector_of(const char* what, const char* name, const Tensor& t, int64_t C, const Tensor& x) {
   check_device(what, name, t, x);
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == C, what, " ", name, " must have shape (", C, ",), got ", t.sizes());
-  data_of(what, name, t);
-  return t.contiguous();
+  return held(what, name, t).contiguous();
 }
 
 // A tensor as rows of its last dimension with unit stride (a copy only where
@@ -76,9 +77,9 @@ Tensor vector_of(const char* what, const char* name, const Tensor& t, int64_t C,
 struct Rows {
   Tensor t;
   int64_t stride;
-  Rows(const char* what, const char* name, const Tensor& v) {
-    const int64_t C = v.size(-1);
-    data_of(what, name, v);
+  Rows(const char* what, const char* name, const Tensor& given) {
+    const int64_t C = given.size(-1);
+    const Tensor v = held(what, name, given);
     t = v.is_contiguous() || v.dim() == 2 ? v : v.reshape({-1, C});
     if (t.stride(-1) != 1 && C > 1) t = t.contiguous();
     stride = t.is_contiguous() ? C : t.stride(0);
@@ -90,10 +91,10 @@ struct Rows {
 struct Residual {
   Tensor t;
   int64_t strides[2] = {0, 0}, per_group = 1;
-  Residual(const char* what, const Tensor& res, const Tensor& x) {
-    check_device(what, "res", res, x);
-    TORCH_CHECK_VALUE(res.sizes() == x.sizes(), what, ": res must have x's shape ", x.sizes(), ", got ", res.sizes());
-    data_of(what, "res", res);
+  Residual(const char* what, const Tensor& given, const Tensor& x) {
+    check_device(what, "res", given, x);
+    TORCH_CHECK_VALUE(given.sizes() == x.sizes(), what, ": res must have x's shape ", x.sizes(), ", got ", given.sizes());
+    const Tensor res = held(what, "res", given);
     if (res.dim() == 3 && !res.is_contiguous() && (res.stride(2) == 1 || res.size(2) == 1)) {
       t = res;
       strides[0] = res.stride(0), strides[1] = res.stride(1), per_group = res.size(1);
@@ -125,7 +126,7 @@ uint64_t seed_of(const char* what, const Maybe& seed, int64_t t) {
   if (t == 0) return 0;
   TORCH_CHECK_VALUE(has(seed) && seed->is_cpu() && seed->numel() == 1 && seed->scalar_type() == at::kLong, what,
                     ": dropout needs its seed, an int64 CPU tensor of one element");
-  return (uint64_t)*static_cast<const int64_t*>(data_of(what, "the seed", *seed));
+  return (uint64_t)*held(what, "the seed", *seed).const_data_ptr<int64_t>();
 }
 
 // Whether autograd has to see the call (a node refuses forward-mode tangents).
@@ -316,7 +317,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_bwd(const Tensor& dy, const Maybe
   check_device(what, "rstd", rstd, x);
   TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), what, ": dy must have x's shape ", x.sizes(), ", got ", dy.sizes());
   TORCH_CHECK_VALUE(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == m.a.N, what, ": bad rstd");
-  data_of(what, "rstd", rstd);
+  const Tensor stats = held(what, "rstd", rstd);
   const Tensor dx = empty(x, x.scalar_type());
   const bool apart = has(res) && (t != 0 || res->scalar_type() != x.scalar_type());
   const Tensor dres = apart ? empty(x, res->scalar_type()) : at::empty({0}, x.options());
@@ -326,7 +327,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_bwd(const Tensor& dy, const Maybe
   const Rows dyr(what, "dy", dy);
   std::optional<Rows> dzr;
   m.a.dy = dyr.t.const_data_ptr(), m.a.dy_stride = dyr.stride, m.a.dy_dtype = type_of(dy, what, "dy");
-  m.a.rstd = rstd.data_ptr<float>();
+  m.a.rstd = stats.data_ptr<float>();
   if (has(dz)) {
     check_device(what, "dz", *dz, x);
     TORCH_CHECK_VALUE(dz->sizes() == x.sizes(), what, ": dz must have x's shape ", x.sizes(), ", got ", dz->sizes());
@@ -431,8 +432,7 @@ Tensor ids_of(const char* what, const Tensor& ids, const Tensor& x) {
   TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "embed: ids must be int64 or int32, got ",
                    ids.scalar_type());
   TORCH_CHECK_VALUE(ids.device() == x.device(), what, ": ids are on ", ids.device(), ", the weight or its gradient on ", x.device());
-  data_of(what, "ids", ids);
-  return ids.contiguous();
+  return held(what, "ids", ids).contiguous();
 }
 
 Tensor embed_fwd(const Tensor& ids, const Tensor& weight, int64_t padding, double scale, ScalarType out) {

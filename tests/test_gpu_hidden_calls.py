@@ -136,6 +136,31 @@ def test_a_traced_rtd_head_computes(gpu):
         assert torch.equal(traced(h * 2), head(h * 2))
 
 
+def test_a_pending_sign_counts(gpu):
+    """The imaginary part of a conjugated tensor is a view whose values are to
+    be negated: equal to its copy in every argument and as a gradient."""
+    z = torch.complex(_rand(6, 1, seed=1), _rand(6, 1, seed=2)).to(gpu)
+    view = z.conj().imag  # one column: rows of stride 2 are read in place
+    assert view.is_neg()
+    zero = torch.zeros(1, device=gpu)
+    assert torch.equal(da.fused_dropout(view, 0.0, bias=zero), view.clone())
+    x, w, r = (_rand(*s, seed=k).to(gpu) for k, s in enumerate(((5, 24), (24,), (5, 24))))
+    ids, neg = torch.tensor([1, 3], device=gpu), torch._neg_view
+    seed = torch.tensor([SEED])
+    rstd = torch.ones(5, device=gpu)
+    for call in (
+        lambda f: da.fused_dropout(f(x), 0.5, bias=f(w), res=f(r), seed=SEED),
+        lambda f: da.fused_dropout(f(x.view(1, 5, 24)), 0.5, res=f(r[:1]).expand(1, 5, 24), seed=SEED),
+        lambda f: da.fused_add_rms_norm(f(x), f(w), bias=f(w), res=f(r))[0],
+        lambda f: da.fused_add_rms_norm_fp8(f(x), f(w), res=f(r))[0].view(torch.uint8),
+        lambda f: da.fused_embedding(ids, f(x)),
+        lambda f: hidden._hidden_dropout_bwd_impl(f(x), FP, FP, 100, seed)[1],
+        lambda f: hidden._add_rms_norm_bwd_impl(f(x), f(r), f(r), None, None, f(w), rstd, 0, None)[0],
+        lambda f: hidden._embed_bwd_impl(f(x[:2]), ids, 6, FP, -1, 1.0),
+    ):
+        assert torch.equal(call(neg), call(lambda t: -t))
+
+
 def test_more_rows_than_one_launch_holds(gpu):
     """2^28 rows of eight columns are one more than 2^32 - 1 threads; the keep
     bits show that a row keeps its number.  A norm of eight values: 8 squares,
