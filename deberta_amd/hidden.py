@@ -554,6 +554,23 @@ class FusedEmbedding(nn.Embedding):
         self.scale = float(scale)
         self.out_dtype = out_dtype
 
+    @classmethod
+    def from_pretrained(
+        cls,
+        embeddings: Tensor,
+        freeze: bool = True,
+        padding_idx: Optional[int] = None,
+        scale: float = 1.0,
+        out_dtype: Optional[torch.dtype] = None,
+    ) -> "FusedEmbedding":
+        """A module on the given ``(V, C)`` table (not a copy), as
+        ``nn.Embedding.from_pretrained``."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"FusedEmbedding: embeddings must be (V, C), got shape {tuple(embeddings.shape)}")
+        emb = cls(*embeddings.shape, padding_idx, scale, out_dtype, device="meta")
+        emb.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return emb
+
     def forward(self, ids: Tensor) -> Tensor:
         return fused_embedding(ids, self.weight, self.padding_idx, self.scale, self.out_dtype)
 

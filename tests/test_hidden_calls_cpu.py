@@ -178,3 +178,19 @@ def test_seeds_are_on_the_cpu_whatever_the_default_device():
     with torch.device("meta"):
         got = da.fused_dropout(x, 0.5), da.fused_dropout(x, 0.5, seed=9), da.hidden_keep_mask(4, 100, 0.5, 9)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_embedding_from_a_given_table():
+    """nn.Embedding's constructor for a given table, which passes arguments
+    that FusedEmbedding's own does not take."""
+    table = torch.randn(9, 4)
+    ids = torch.tensor([[0, 8, 2]])
+    emb = da.FusedEmbedding.from_pretrained(table, padding_idx=-1, scale=3.0)
+    assert emb.weight.data_ptr() == table.data_ptr() and not emb.weight.requires_grad and emb.padding_idx == 8
+    assert type(emb) is da.FusedEmbedding and (emb.num_embeddings, emb.embedding_dim) == (9, 4)
+    assert torch.equal(emb(ids), table[ids] * 3.0) and torch.equal(table[8], emb.weight[8])
+    emb = da.FusedEmbedding.from_pretrained(table, freeze=False)
+    emb(ids).sum().backward()
+    assert emb.weight.grad[0].eq(1).all() and emb.weight.grad[1].eq(0).all()
+    with pytest.raises(ValueError, match="shape"):
+        da.FusedEmbedding.from_pretrained(table[0])
