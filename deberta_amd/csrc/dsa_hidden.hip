@@ -32,6 +32,7 @@ DSA_EXTERN(float, float)
 namespace {
 
 constexpr int64_t kMaxRows = 0x7fffffffLL;
+constexpr int kMaxEmbedC = 1 << 30;
 
 template <typename T>
 struct Tag {
@@ -296,6 +297,8 @@ int check_embed(const dsa_embed_args* a, bool bwd) {
     if (!rows_given(a->y, a->y_stride, a->y_dtype)) return fail("dsa_embed: bad y");
     return 0;
   }
+  // the sums take a column's byte offset in 32 bits
+  if (a->C > kMaxEmbedC) return fail("dsa_embed: the backward takes at most 2^30 columns, got C=%d", a->C);
   if (!dtype_ok(a->weight_dtype)) return fail("dsa_embed: bad weight dtype");
   if (!rows_given(a->dy, a->dy_stride, a->dy_dtype)) return fail("dsa_embed: bad dy");
   if (!a->dweight || !aligned16(a->dweight)) return fail("dsa_embed: dweight must be given and 16-byte aligned");

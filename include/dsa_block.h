@@ -208,7 +208,7 @@ typedef struct dsa_embed_args {
   int64_t N;                  /* at most 2^31 - 1 */
   int64_t V;                  /* at most 2^31 - 2 */
   int64_t padding;            /* the token without a gradient, or -1 */
-  int32_t C;
+  int32_t C;                  /* backward: at most 2^30 */
   int32_t ids_bytes;          /* 8 or 4 */
   int32_t weight_dtype, y_dtype, dy_dtype;
   float scale;

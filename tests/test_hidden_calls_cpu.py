@@ -10,6 +10,7 @@ recorder went past ``torch.ops``, calls that reach the op find no CPU kernel.
 
 from __future__ import annotations
 
+import ctypes
 import re
 import shutil
 import subprocess
@@ -194,3 +195,14 @@ def test_embedding_from_a_given_table():
     assert emb.weight.grad[0].eq(1).all() and emb.weight.grad[1].eq(0).all()
     with pytest.raises(ValueError, match="shape"):
         da.FusedEmbedding.from_pretrained(table[0])
+
+
+def test_the_embeddings_backward_refuses_columns_past_32_bit_offsets():
+    """Its byte offsets inside a row are 32-bit: 2^30 float32 columns."""
+    lib = _lib.load()
+    keep = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(keep) + 255) // 256 * 256
+    args = dict(ids=at, ids_bytes=8, dy=at, dy_stride=8, dweight=at, N=2, V=5, padding=-1, scale=1.0)
+    for C, match in (((1 << 30) + 1, "2\\^30 columns"), (1 << 30, "workspace")):
+        assert lib.dsa_embed_bwd(ctypes.byref(_lib.DsaEmbedArgs(C=C, **args)), None) != 0
+        assert re.search(match, _lib.last_error())
