@@ -5,6 +5,8 @@ several rows.  Tolerances as in test_gpu_hidden.py."""
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 
@@ -12,6 +14,7 @@ import deberta_amd as da
 from deberta_amd import hidden
 from oracle import hidden as oh
 from tests._hidden import Wrapper
+from tests.test_gpu_hidden import _rms_case
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +188,40 @@ def test_more_rows_than_one_launch_holds(gpu):
     assert ((got.double() - y64).abs() <= (2.0**-4 + 32 * U) * y64.abs() + 2.0**-10 * s[rows].cpu().double()).all()
     s[rows] = 1
     assert (s == 1).all()
+
+
+# rows so that every shape of team takes two or three, the last ones fewer: 16 and
+# 32 lanes, one wave of one and of two chunks, four, eight and sixteen waves, with
+# column sums in registers and (past 8192 columns) in LDS, whole and cut rows
+@pytest.mark.parametrize("N,C", [(20011, 33), (20011, 64), (9001, 200), (9001, 201), (5001, 301), (5001, 304), (5001, 1024),
+                                 (5001, 777), (2501, 1025), (1301, 2048), (600, 2500), (600, 4096), (600, 5003), (600, 8192),
+                                 (600, 8193), (600, 16384)])
+@pytest.mark.parametrize("xt,rt,bt", [(BF, BF, FP), (BF, FP, BF), (FP, FP, FP)])
+def test_rms_teams_of_several_rows(N, C, xt, rt, bt, gpu):
+    print("rms", N, C, xt, rt, file=sys.stderr, flush=True)
+    _rms_case(gpu, (N, C), xt, rt, FP, bt=bt, p=0.1)
+
+
+def test_transforms_of_any_argument_raise(gpu):
+    """torch.func's wrappers in another argument than the first: an error, not
+    a result without them."""
+    import torch.autograd.forward_ad as fwAD
+
+    x, w, r = (_rand(*s, seed=k).to(gpu) for k, s in enumerate(((5, 24), (24,), (5, 24))))
+    for call, t in (
+        (lambda b: da.fused_dropout(x, 0.5, bias=b, seed=SEED), w),
+        (lambda b: da.fused_dropout(x, 0.5, res=b, seed=SEED), r),
+        (lambda b: da.fused_rms_norm(x, b), w),
+        (lambda b: da.fused_add_rms_norm(x, w, bias=b)[0], w),
+        (lambda b: da.fused_add_rms_norm(x, w, res=b)[0], r),
+    ):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(t.expand(3, *t.shape))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v).sum())(t)
+        with fwAD.dual_level(), pytest.raises(RuntimeError):
+            call(fwAD.make_dual(t, torch.ones_like(t)))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda i: da.fused_embedding(i, x))(torch.zeros(3, 2, dtype=torch.int64, device=gpu))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: da.fused_add_rms_norm_fp8(x, v)[1])(w.expand(3, 24))
