@@ -41,11 +41,14 @@ void by_width(int C, F f) {
   else if (C <= 512) f(i64, i1, i1);
   else if (C <= 1024) f(i64, i2, i1);
   else if (C <= 2048) f(i64, i1, i4);
-  else if (C <= 4096 && BWD) f(i64, i1, i8);
-  else if (C <= 4096) f(i64, i2, i4);
-  else if (C <= 8192 && BWD) f(i64, i1, i16);
-  else if (C <= 8192) f(i64, i2, i8);
-  else f(i64, i2, i16);
+  else if (C > 8192) f(i64, i2, i16);
+  else if constexpr (BWD) {
+    if (C <= 4096) f(i64, i1, i8);
+    else f(i64, i1, i16);
+  } else {
+    if (C <= 4096) f(i64, i2, i4);
+    else f(i64, i2, i8);
+  }
 }
 // Teams a block of the backward, and the blocks that run at once: two a
 // compute unit of four waves, one of eight or sixteen.

@@ -206,3 +206,17 @@ def test_the_embeddings_backward_refuses_columns_past_32_bit_offsets():
     for C, match in (((1 << 30) + 1, "2\\^30 columns"), (1 << 30, "workspace")):
         assert lib.dsa_embed_bwd(ctypes.byref(_lib.DsaEmbedArgs(C=C, **args)), None) != 0
         assert re.search(match, _lib.last_error())
+
+
+def test_the_library_holds_no_norm_kernel_that_no_width_reaches():
+    """Lanes, chunks and waves a row of the norm's kernels in the library: the
+    forward's two chunks a lane and the backward's one between 2049 and 8192
+    columns, and what both take elsewhere."""
+    nm = shutil.which("nm")
+    if nm is None:
+        pytest.skip("nm not available")
+    names = subprocess.run([nm, "-C", str(_lib.LIB_PATH)], capture_output=True, text=True, check=True).stdout
+    both = {(16, 1, 1), (32, 1, 1), (64, 1, 1), (64, 2, 1), (64, 1, 4), (64, 2, 16)}
+    for kernel, between in (("rms_fwd_kernel", {(64, 2, 4), (64, 2, 8)}), ("rms_bwd_kernel", {(64, 1, 8), (64, 1, 16)})):
+        found = re.findall(kernel + r"<(\d+), (\d+), (\d+)", names)
+        assert {tuple(map(int, t)) for t in found} == both | between
