@@ -417,8 +417,9 @@ def fused_add_rms_norm_fp8(
     x's shape and scales float32 ``(..., 1)``, one a row, or ``(..., C /
     group_size)``, one for each ``group_size`` columns (32, 64, 128, 256 or 512).
 
-    A scale is the group's largest ``|y|`` / 448, so that the largest value
-    becomes 448 and the others round to nearest even.  A group of zeros (or
+    With m the group's largest ``|y|`` the scale is m / 448 and q is ``y * (448 /
+    m)`` rounded to nearest even, both in float32 (a y between two bytes may go
+    to the other one than ``y / scale`` would): m itself becomes 448.  A group of zeros (or
     below the normal float32 range) has the scale 1 and q 0; one with a NaN or an
     infinity has the scale NaN and q NaN.  For serving: there is no gradient,
     and a call under autograd whose inputs need one raises."""
@@ -436,9 +437,11 @@ def fused_add_rms_norm_fp8(
         y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.to(z.dtype)
         y = y.unflatten(-1, (C // (g or C), g or C))
         top = y.abs().amax(-1, keepdim=True)
-        scale = torch.where(top < FP8_MAX * 2.0**-126, 1.0, top / FP8_MAX)
-        scale = torch.where(top.isfinite(), scale, torch.nan)
-        q = (y / scale).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
+        tiny, finite = top < FP8_MAX * 2.0**-126, top.isfinite()
+        scale = torch.where(finite, torch.where(tiny, 1.0, top / FP8_MAX), torch.nan)
+        # a tensor above: torch divides a number through the reciprocal
+        factor = torch.where(finite, torch.where(tiny, 1.0, torch.full_like(top, FP8_MAX) / top), torch.nan)
+        q = (y * factor).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
         return q, scale.squeeze(-1).float(), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
     if _eager.eager_all(x, bias, res, weight):
         return _ext().quant(x, bias, res, weight, float(eps), g)

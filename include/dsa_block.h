@@ -243,10 +243,11 @@ int dsa_dropout_bwd(const dsa_dropout_args* args, void* stream);
 
 /* y, z and rstd from x, bias, res, weight. */
 int dsa_add_rms_fwd(const dsa_rms_args* args, void* stream);
-/* y as e4m3 bytes (finite values, one NaN pattern) with scales, and z: y =
- * value * scale, scale = max |y| of the row or group / 448, 1 where that is
- * below the smallest normal float32, NaN (and the bytes NaN) where a y of it is
- * not finite. */
+/* y as e4m3 bytes (finite values, one NaN pattern) with scales, and z: with m
+ * = max |y| of the row or group, scale = m / 448 and the byte is y * (448 / m)
+ * to nearest even, all in float32, so that y = byte * scale.  Where m / 448 is
+ * below the smallest normal float32 the scale is 1 and the bytes are 0; where a
+ * y of it is not finite the scale and the bytes are NaN. */
 int dsa_add_rms_quant(const dsa_rms_args* args, void* stream);
 /* dx, dres, dweight and dbias from dy, dzu and the forward's inputs and rstd. */
 int dsa_add_rms_bwd(const dsa_rms_args* args, void* stream);

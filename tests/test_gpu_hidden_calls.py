@@ -225,3 +225,30 @@ def test_transforms_of_any_argument_raise(gpu):
         torch.func.vmap(lambda i: da.fused_embedding(i, x))(torch.zeros(3, 2, dtype=torch.int64, device=gpu))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda v: da.fused_add_rms_norm_fp8(x, v)[1])(w.expand(3, 24))
+
+
+@pytest.mark.parametrize("N,C,group", [(2000, 1024, None), (700, 2048, 128), (900, 1023, None)])
+def test_eight_bit_bytes_are_the_definitions(N, C, group, gpu):
+    """Every byte is the float64 definition's rounded once, or its neighbour
+    where the exact value lies on the border between the two as far as float32
+    can tell: by twice y's error over the scale (that of the value, and of the
+    scale at the group's largest) and four half steps of the value."""
+    G = group or C
+    x, res = _rand(N, C, seed=1, dtype=BF).to(gpu), _rand(N, C, seed=2, dtype=BF).to(gpu)
+    w = (1 + 0.2 * _rand(C, seed=3)).to(gpu)
+    with torch.no_grad():
+        q, _, _ = da.fused_add_rms_norm_fp8(x, w, EPS, res=res, group_size=group)
+        again = da.fused_add_rms_norm_fp8(x, w, EPS, res=res, group_size=group)[0]
+    assert torch.equal(q.view(torch.uint8), again.view(torch.uint8))
+    x64, r64, w64 = x.cpu().double(), res.cpu().double(), w.cpu().double()
+    z64 = x64 + r64
+    exact, s64 = oh.quantise(oh.rms_norm(z64, w64, EPS), G)
+    got, want = q.float().cpu().double(), exact.float().to(torch.float8_e4m3fn).float().double()
+    r = 1 / torch.sqrt(z64.square().mean(-1, keepdim=True) + EPS)
+    e = w64.abs() * 96 * U * ((z64 * r).abs() + (x64.abs() + r64.abs()) * r)  # of y, as in test_gpu_hidden.py
+    top = e.unflatten(-1, (C // G, G)).amax(-1).repeat_interleave(G, -1)
+    s_el = s64.repeat_interleave(G, -1)
+    tol = e / s_el + top / s_el * exact.abs() / 448 + 4 * U * exact.abs()
+    other = got != want
+    assert ((exact - (got + want) / 2).abs() <= tol)[other].all()
+    assert ((got - want).abs() <= 2.0**-3 * torch.maximum(got.abs(), want.abs()).clamp(min=2.0**-6))[other].all()

@@ -220,3 +220,26 @@ def test_the_library_holds_no_norm_kernel_that_no_width_reaches():
     for kernel, between in (("rms_fwd_kernel", {(64, 2, 4), (64, 2, 8)}), ("rms_bwd_kernel", {(64, 1, 8), (64, 1, 16)})):
         found = re.findall(kernel + r"<(\d+), (\d+), (\d+)", names)
         assert {tuple(map(int, t)) for t in found} == both | between
+
+
+@pytest.mark.parametrize("group", [None, 64])
+def test_cpu_bytes_round_the_product_that_the_kernel_rounds(group):
+    """y * (448 / m), not y / (m / 448): a few bytes in a million differ, and
+    CPU tensors would not give the GPU's."""
+    x, w = torch.randn(4096, 512, generator=torch.Generator().manual_seed(1)), 1 + 0.2 * torch.randn(512, generator=torch.Generator().manual_seed(2))
+    q, scale, _ = da.fused_add_rms_norm_fp8(x, w, group_size=group)
+    y = da.fused_rms_norm(x, w).unflatten(-1, (512 // (group or 512), group or 512))
+    m = y.abs().amax(-1, keepdim=True)
+    most = torch.full_like(m, 448.0)
+    assert torch.equal(scale, (m / most).squeeze(-1))
+    want = (y * (most / m)).clamp(-448, 448).flatten(-2).to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+
+
+def test_cpu_bytes_of_a_group_that_is_not_finite():
+    x = torch.ones(3, 64)
+    x[0, 3], x[1, 40] = float("inf"), float("nan")
+    q, scale, _ = da.fused_add_rms_norm_fp8(x, torch.ones(64), group_size=32)
+    # an infinity leaves a norm of 0 in its row but for inf * 0
+    assert scale[0, 0].isnan() and q[0, :32].float().isnan().all() and scale[0, 1] == 1 and (q[0, 32:].float() == 0).all()
+    assert scale[1].isnan().all() and q[1].float().isnan().all() and q[2].float().isfinite().all()
