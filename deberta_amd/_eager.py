@@ -14,7 +14,7 @@ the op and its fake implementation.  Both paths launch the same kernels.
 
 from __future__ import annotations
 
-from typing import Any, Callable, Optional
+from typing import Any, Callable
 
 import torch
 
@@ -35,19 +35,6 @@ def eager(t: torch.Tensor) -> bool:
         not torch.compiler.is_compiling()
         and _dispatch_depth() == 0
         and (type(t) is torch.Tensor or (type(t) is torch.nn.Parameter and not torch.jit.is_tracing()))
-    )
-
-
-def eager_all(t: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
-    """:func:`eager` for a call that goes into an extension, past Python
-    autograd functions too.  Every tensor given has to be a plain one or a
-    module's parameter: a subclass may hold its values elsewhere, and has to
-    see the op.  torch.jit.trace records the extension's empty results and not
-    its launches, so a traced call is the op's as well."""
-    return (
-        eager(t)
-        and not torch.jit.is_tracing()
-        and all(o is None or type(o) is torch.Tensor or type(o) is torch.nn.Parameter for o in others)
     )
 
 

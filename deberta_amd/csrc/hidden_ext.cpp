@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/version.h>
 
@@ -53,7 +54,7 @@ Tensor held(const char* what, const char* name, const Tensor& t) {
   const size_t need = at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(), t.storage_offset());
   TORCH_CHECK_VALUE(t.storage().data() != nullptr && t.storage().nbytes() >= need, what, ": ", name,
                     " has elements but no memory for them (a wrapper tensor, or its storage was freed)");
-  return t.resolve_neg();
+  return t.is_neg() ? t.resolve_neg() : t;
 }
 
 // x's width, x on the GPU
@@ -137,6 +138,17 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 const Tensor* at_or_null(const Maybe& t) { return has(t) ? &*t : nullptr; }
+
+// Whether the call may be made here.  torch.jit.trace records the results that
+// are allocated and not the launches, so a traced call is the registered op's; a
+// subclass with a dispatch of its own may hold its values elsewhere, and has to
+// see the op.
+bool here(std::initializer_list<const Tensor*> ts) {
+  if (torch::jit::tracer::isTracing()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->defined() && t->key_set().has(c10::DispatchKey::Python)) return false;
+  return true;
+}
 
 // The gradients of a backward whose own graph is asked for: they raise when
 // that is walked.
@@ -237,7 +249,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
-Tensor dropout(const Tensor& x, const Maybe& bias, const Maybe& res, int64_t t, const Maybe& seed) {
+Maybe dropout(const Tensor& x, const Maybe& bias, const Maybe& res, int64_t t, const Maybe& seed) {
+  if (!here({&x, at_or_null(bias), at_or_null(res), at_or_null(seed)})) return std::nullopt;
   if (!needs_grad({&x, at_or_null(bias), at_or_null(res)})) return dropout_fwd(x, bias, res, t, seed);
   return Dropout::apply(x, bias, res, t, seed);
 }
@@ -378,14 +391,15 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 };
 
 // (y, z); z is x where there is nothing to add or drop
-std::tuple<Tensor, Tensor> rms(const Tensor& x, const Maybe& bias, const Maybe& res, const Tensor& weight, double eps, ScalarType out,
-                               int64_t t, const Maybe& seed) {
+std::optional<std::tuple<Tensor, Tensor>> rms(const Tensor& x, const Maybe& bias, const Maybe& res, const Tensor& weight, double eps,
+                                              ScalarType out, int64_t t, const Maybe& seed) {
+  if (!here({&x, at_or_null(bias), at_or_null(res), &weight, at_or_null(seed)})) return std::nullopt;
   if (!needs_grad({&x, at_or_null(bias), at_or_null(res), &weight})) {
     auto [y, z, rstd] = rms_run(x, bias, res, weight, eps, out, t, seed, false);
-    return {y, z.defined() ? z : x};
+    return std::make_tuple(y, z.defined() ? z : x);
   }
   const variable_list o = AddRmsNorm::apply(x, bias, res, weight, eps, out, t, seed);
-  return {o[0], o.size() > 1 ? o[1] : x};
+  return std::make_tuple(o[0], o.size() > 1 ? o[1] : x);
 }
 
 // (y as float8_e4m3fn, its scales, z); z is undefined where it is x itself.
@@ -419,10 +433,11 @@ std::tuple<Tensor, Tensor, Tensor> quant_fwd(const Tensor& x, const Maybe& bias,
   return {q, scales, z};
 }
 
-std::tuple<Tensor, Tensor, Tensor> quant(const Tensor& x, const Maybe& bias, const Maybe& res, const Tensor& weight, double eps,
-                                         int64_t group) {
+std::optional<std::tuple<Tensor, Tensor, Tensor>> quant(const Tensor& x, const Maybe& bias, const Maybe& res, const Tensor& weight,
+                                                        double eps, int64_t group) {
+  if (!here({&x, at_or_null(bias), at_or_null(res), &weight})) return std::nullopt;
   auto [q, scales, z] = quant_run(x, bias, res, weight, eps, group);
-  return {q, scales, z.defined() ? z : x};
+  return std::make_tuple(q, scales, z.defined() ? z : x);
 }
 
 // ---------------------------------------------------------------------------
@@ -496,15 +511,16 @@ struct Embed : torch::autograd::Function<Embed> {
   }
 };
 
-Tensor embed(const Tensor& ids, const Tensor& weight, int64_t padding, double scale, ScalarType out) {
+Maybe embed(const Tensor& ids, const Tensor& weight, int64_t padding, double scale, ScalarType out) {
+  if (!here({&ids, &weight})) return std::nullopt;
   if (!needs_grad({&weight})) return embed_fwd(ids, weight, padding, scale, out);
   return Embed::apply(ids, weight, padding, scale, out);
 }
 
 }  // namespace
 
-// The functions named like an operator record autograd; _fwd and _bwd are what
-// the registered ops call.
+// The functions named like an operator record autograd, and give None for a call
+// that the registered op has to see; _fwd and _bwd are what the ops call.
 PYBIND11_MODULE(_hidden_ext, m) {
   m.attr("abi_version") = DSA_VERSION;      // whose structs it passes
   m.attr("torch_version") = TORCH_VERSION;  // whose classes it was compiled with

@@ -58,7 +58,9 @@ MAX_RMS_WIDTH = 16384
 
 @functools.lru_cache(maxsize=None)
 def _ext() -> Any:
-    """The host side of the operators on the GPU (csrc/hidden_ext.cpp)."""
+    """The host side of the operators on the GPU (csrc/hidden_ext.cpp).  Its
+    functions named like an operator return None for a call that the registered
+    op has to see: one that is traced, or with a wrapper among its tensors."""
     _lib.load()  # and checks its version
     if not EXT_PATH.exists():
         raise RuntimeError(
@@ -237,8 +239,10 @@ def fused_dropout(
     if not x.is_cuda:
         _cpu_args("fused_dropout", x, bias, res)
         return _cpu_sum(x, bias, res, t, s).to(_stream_dtype(x, res))
-    if _eager.eager_all(x, bias, res, s):
-        return _ext().dropout(x, bias, res, t, s)
+    if _eager.eager(x):
+        y = _ext().dropout(x, bias, res, t, s)
+        if y is not None:
+            return y
     return torch.ops.deberta_amd.hidden_dropout(x, bias, res, t, s)
 
 
@@ -392,8 +396,10 @@ def fused_add_rms_norm(
         z = _cpu_sum(x, bias, res, t, s)
         y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * weight.to(z.dtype)
         return y.to(out_dtype), (x if _plain(bias, res, t) else z.to(_stream_dtype(x, res)))
-    if _eager.eager_all(x, bias, res, weight, s):
-        return _ext().rms(x, bias, res, weight, float(eps), out_dtype, t, s)
+    if _eager.eager(x):
+        out = _ext().rms(x, bias, res, weight, float(eps), out_dtype, t, s)
+        if out is not None:
+            return out
     y, z, _ = torch.ops.deberta_amd.add_rms_norm(x, bias, res, weight, float(eps), out_dtype, t, s)
     return y, (x if _plain(bias, res, t) else z)
 
@@ -443,8 +449,10 @@ def fused_add_rms_norm_fp8(
         factor = torch.where(finite, torch.where(tiny, 1.0, torch.full_like(top, FP8_MAX) / top), torch.nan)
         q = (y * factor).clamp(-FP8_MAX, FP8_MAX).flatten(-2).to(torch.float8_e4m3fn)
         return q, scale.squeeze(-1).float(), (x if _plain(bias, res, 0) else z.to(_stream_dtype(x, res)))
-    if _eager.eager_all(x, bias, res, weight):
-        return _ext().quant(x, bias, res, weight, float(eps), g)
+    if _eager.eager(x):
+        out = _ext().quant(x, bias, res, weight, float(eps), g)
+        if out is not None:
+            return out
     q, scale, z = torch.ops.deberta_amd.add_rms_norm_quant(x, bias, res, weight, float(eps), g)
     return q, scale, (x if _plain(bias, res, 0) else z)
 
@@ -528,8 +536,10 @@ def fused_embedding(
             weight = weight.to(wide)  # before the lookup: its gradient sums a token's positions in this type
         y = torch.nn.functional.embedding(ids, weight, padding_idx=None if pad < 0 else pad)
         return (y.to(wide) * scale).to(out_dtype)
-    if _eager.eager_all(weight, ids):
-        return _ext().embed(ids, weight, pad, float(scale), out_dtype)
+    if _eager.eager(weight):
+        y = _ext().embed(ids, weight, pad, float(scale), out_dtype)
+        if y is not None:
+            return y
     return torch.ops.deberta_amd.embed(ids, weight, pad, float(scale), out_dtype)
 
 

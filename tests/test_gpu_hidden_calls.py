@@ -73,8 +73,8 @@ def test_tensors_without_memory_are_refused(gpu):
         lambda: da.fused_embedding(torch.zeros(2, dtype=torch.int64, device=gpu), row),
         lambda: ext.dropout_bwd(row, FP, FP, 100, seed),
         lambda: ext.rms_bwd(x, row, x, None, None, w, torch.ones(5, device=gpu), 0, None),
-        lambda: ext.dropout(x, Wrapper(w), None, 100, seed),
-        lambda: ext.dropout(x, None, None, 100, Wrapper(seed)),
+        lambda: ext.dropout_fwd(x, Wrapper(w), None, 100, seed),
+        lambda: ext.dropout_fwd(x, None, None, 100, Wrapper(seed)),
     ):
         with pytest.raises(ValueError, match="no memory"):
             call()
