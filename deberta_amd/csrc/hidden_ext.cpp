@@ -51,8 +51,11 @@ void check_device(const char* what, const char* name, const Tensor& t, const Ten
 // before their negation, which is made here.
 Tensor held(const char* what, const char* name, const Tensor& t) {
   if (t.numel() == 0) return t;
-  const size_t need = at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(), t.storage_offset());
-  TORCH_CHECK_VALUE(t.storage().data() != nullptr && t.storage().nbytes() >= need, what, ": ", name,
+  const size_t need = t.is_contiguous()
+                          ? (size_t)(t.storage_offset() + t.numel()) * t.element_size()
+                          : at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(), t.storage_offset());
+  const c10::Storage& s = t.storage();
+  TORCH_CHECK_VALUE(s.data() != nullptr && s.nbytes() >= need, what, ": ", name,
                     " has elements but no memory for them (a wrapper tensor, or its storage was freed)");
   return t.is_neg() ? t.resolve_neg() : t;
 }
