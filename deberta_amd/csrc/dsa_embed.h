@@ -50,8 +50,14 @@ constexpr int SORT_BITS = 9;    // a digit's bits at most: SORT_T >= 2^SORT_BITS
 constexpr int SORT_D = 1 << SORT_BITS;
 constexpr int SORT_W = SORT_T / 64;
 constexpr int FILL_BYTES = 65536;  // of dW, about, a fill workgroup clears
+// Positions the counting sort takes at most: as many as leave 19 bits of a word
+// to the token.  It compares every pair and is still the faster one there; the
+// two meet at about twice as many.  The gradient's kernels, counting / radix, us:
+// 513 bf16 columns of 50021 tokens 21.7 / 43.2 for 2723 positions, 35 / 52 for
+// 8192, 52 / 55 for 16384 (a build with 14 bits); 768 fp32 of 128100 81 / 95,
+// 84 / 106, 108 / 114; 1024 bf16 of 128100 43 / 58, 51 / 72, 65 / 74.
 constexpr int RANK_BITS = 13;
-constexpr int RANK_N = 1 << RANK_BITS;  // positions the counting sort takes at most
+constexpr int RANK_N = 1 << RANK_BITS;
 
 struct EmbedRows {
   const void *ids, *w;
@@ -433,7 +439,10 @@ DSA_DEV void join_parts(const EmbedSums& p, uint32_t ch, uint32_t last, int q, i
 
 // A block: JOIN_W chunks and 512 columns; wave q looks whether a token begins in
 // its chunk and goes on past the chunk's end.  One that ends within JOIN_ONE
-// chunks is joined by the wave, a longer one by the whole block.
+// chunks is joined by the wave, which loads eight chunks' sums at once, a longer
+// one by the whole block, tokens in turn.  The gradient's kernels with every token
+// by the block, and with 2, 8 and 32 chunks by the wave: 2723 x 513 30.3, 24.2,
+// 22.6, 22.6 us, 30000 x 768 of 2000 tokens 56.8, 51.2, 49.9, 50.4.
 constexpr uint32_t JOIN_ONE = 8;
 constexpr int JOIN_W = 8;
 

@@ -18,13 +18,16 @@
 // the next row's in flight while it waits for this one's (behind a condition
 // it waits for both): lanes past the row load its last chunk, a residual or
 // gradient that is not there is read from a tensor that is, always the same
-// row, and not used.
+// row, and not used.  Not so where a row ends in a cut chunk (TAIL): its loads
+// are behind the condition that the tensor goes on behind the row (row8).
 //
 // HBM bounds all but the smallest: 16384 x 768 bf16 with bias, dropout and
 // residual 21.8 us forward (101 MB, 4.6 TB/s) and 30.0 backward (151 MB, 5.0),
 // 16384 x 4096 bf16 on a float32 stream 164 (940 MB, 5.7) and 270 (1342 MB,
-// 5.0); 9971 x 1024 in 8 bits 14.0 (71 MB, 5.1).  Odd bf16 widths run at 60 to
-// 85% of that: every other row then starts between two words.
+// 5.0); 9971 x 1024 in 8 bits 14.0 (71 MB, 5.1).  Of the rate at the next
+// multiple of eight, odd bf16 widths (33.5 million values, 513 to 8191 columns)
+// reach 77 to 96% forward and 57 to 84% backward; dropout, whose accesses are as
+// unaligned and unconditional but for the last chunk, 82 to 92%.
 #pragma once
 
 #include <type_traits>
@@ -301,7 +304,11 @@ struct RawBwd {
 // once), so that the partial sums are few.  A row's own latency is then
 // what bounds it: the next row is loaded while the row is worked on, where
 // its registers allow (PRE), and w and the bias stay in registers (KEEP).
-// Sixteen waves have 128 registers each: their column sums lie in LDS.
+// Sixteen waves have 128 registers each.  With two chunks a lane (past 8192
+// columns) their column sums lie in LDS, w and the bias are read again for every
+// row and no row is loaded ahead; with one chunk all of it is in registers.
+// Neither form fits whole: the compiler spills up to 14 registers a lane where
+// rows are whole and 5 to 57 where they are cut.
 template <int L, int NC, int W, typename TX, typename TR, typename TZ, typename TDY, bool TAIL>
 __global__ __launch_bounds__(rms_threads<W>()) void rms_bwd_kernel(RmsRows p) {
   typedef RawBwd<NC, TX, TR, TZ, TDY, TAIL> Raw;
