@@ -15,6 +15,11 @@ Public surface:
                               fused_add_rms_norm, fused_rms_norm,
                               fused_add_rms_norm_fp8: the operators on hidden
                               states (hidden_keep_mask: dropout's bits)
+  FusedMLMHead, fused_token_logprobs (TokenLogprobs), fused_distillation_loss
+                              the operators on a vocabulary's logits: log
+                              probabilities of given tokens with entropy and top
+                              alternatives, distillation from a teacher's top
+                              logits, and the masked language model's head
   normalize_attention_kernel  the attention-kernel selector
 The compute runs in libdsa.so (hand-written HIP for gfx950) through the
 torch.library ops ``deberta_amd::dsa_fwd`` / ``deberta_amd::dsa_bwd``.
@@ -43,6 +48,7 @@ from deberta_amd.hidden import (
 )
 from deberta_amd.masks import SegmentMask, build_doc_block_mask, get_attention_mask, normalize_keep_mask
 from deberta_amd.relpos import build_relative_position, make_log_bucket_position, relative_offset_table
+from deberta_amd.vocab import FusedMLMHead, TokenLogprobs, fused_distillation_loss, fused_token_logprobs
 
 __all__ = [
     "DisentangledSelfAttention",
@@ -72,4 +78,8 @@ __all__ = [
     "fused_rms_norm",
     "fused_add_rms_norm_fp8",
     "hidden_keep_mask",
+    "FusedMLMHead",
+    "TokenLogprobs",
+    "fused_token_logprobs",
+    "fused_distillation_loss",
 ]

@@ -1,7 +1,7 @@
 """Builds ``libdsa.so`` (the HIP kernels and their C ABI) in-tree with hipcc for
 gfx950, and ``_hidden_ext.so`` (the host side of the operators on hidden
-states: PyTorch tensors and autograd over that C ABI) with g++, or the ROCm
-toolchain's own clang++ where there is no g++."""
+states and on a vocabulary's logits: PyTorch tensors and autograd over that C
+ABI) with g++, or the ROCm toolchain's own clang++ where there is no g++."""
 
 from __future__ import annotations
 
@@ -29,11 +29,12 @@ SOURCES = (
     ("dsa_rms_inst.hip", ("-DDSA_TX=bf16", "-DDSA_TR=float")),
     ("dsa_rms_inst.hip", ("-DDSA_TX=float", "-DDSA_TR=bf16")),
     ("dsa_rms_inst.hip", ("-DDSA_TX=float", "-DDSA_TR=float")),
+    ("dsa_vocab.hip", ()),
 )
 # bench.py's MFMA throughput probe (include/dsa_probe.h), a library of its own
 PROBE_PATH = PKG_DIR / "libdsa_probe.so"
 PROBE_SOURCES = (("dsa_probe.hip", ()),)
-# the operators on hidden states for PyTorch tensors: host code, linked to libdsa.so
+# the operators on hidden states and logits for PyTorch tensors: host code (it includes vocab_ext.h), linked to libdsa.so
 EXT_PATH = PKG_DIR / "_hidden_ext.so"
 EXT_SOURCE = CSRC_DIR / "hidden_ext.cpp"
 ARCH = "gfx950"
@@ -135,7 +136,8 @@ def _run(cmd) -> None:
 def build(verbose: bool = False) -> Path:
     """Compile every source: ``deberta_amd/libdsa.so`` (the kernels and their
     C ABI), ``deberta_amd/libdsa_probe.so`` (the MFMA probe) and
-    ``deberta_amd/_hidden_ext.so`` (the hidden-state operators' host side).
+    ``deberta_amd/_hidden_ext.so`` (the hidden-state and vocabulary operators'
+    host side).
 
     Always recompiles.  Each library is written to a temporary name first and
     renamed into place, so a process that already loaded the old file keeps a

@@ -24,7 +24,7 @@ DSA_STAGE_FOLD = 8
 DSA_STAGE_TABLE = 16  # the first half of FOLD: per-offset sums (workspace)
 DSA_STAGE_SUM = 32  # the second half: their fold onto dkr / dqr
 
-EXPECTED_VERSION = 14
+EXPECTED_VERSION = 15
 
 _i64x3 = ctypes.c_int64 * 3
 _i64x2 = ctypes.c_int64 * 2
@@ -299,6 +299,76 @@ class DsaEmbedArgs(ctypes.Structure):
     ]
 
 
+class DsaLogprobsArgs(ctypes.Structure):
+    """dsa_logprobs_args (include/dsa_vocab.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_stride", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("ignore_index", ctypes.c_int64),
+        ("logprobs", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p),
+        ("top_ids", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dlogprobs", ctypes.c_void_p),
+        ("dentropy", ctypes.c_void_p),
+        ("dlse", ctypes.c_void_p),
+        ("dtop", ctypes.c_void_p),
+        ("dlogprobs_stride", ctypes.c_int64),
+        ("dentropy_stride", ctypes.c_int64),
+        ("dlse_stride", ctypes.c_int64),
+        ("dlogits", ctypes.c_void_p),
+        ("dlogits_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("N", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("top_k", ctypes.c_int32),
+        ("ids_bytes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("inv_temperature", ctypes.c_float),
+    ]
+
+
+class DsaDistillArgs(ctypes.Structure):
+    """dsa_distill_args (include/dsa_vocab.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_stride", ctypes.c_int64),
+        ("teacher_ids", ctypes.c_void_p),
+        ("teacher", ctypes.c_void_p),
+        ("teacher_lse", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dloss", ctypes.c_void_p),
+        ("dloss_stride", ctypes.c_int64),
+        ("dlogits", ctypes.c_void_p),
+        ("dlogits_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("N", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("K", ctypes.c_int32),
+        ("ids_bytes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("teacher_dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+    ]
+
+
+# Entry points of include/dsa_vocab.h (the operators on a vocabulary's logits).
+VOCAB_EXPORTS = (
+    "dsa_vocab_workspace_bytes",
+    "dsa_logprobs_fwd",
+    "dsa_logprobs_bwd",
+    "dsa_distill_fwd",
+    "dsa_distill_bwd",
+)
+
 # Entry points of include/dsa_block.h (the fused row kernels).
 BLOCK_EXPORTS = (
     "dsa_block_workspace_bytes",
@@ -378,6 +448,8 @@ def load() -> ctypes.CDLL:
         lib.dsa_block_workspace_bytes.restype = ctypes.c_size_t
         lib.dsa_embed_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int64]
         lib.dsa_embed_workspace_bytes.restype = ctypes.c_size_t
+        lib.dsa_vocab_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+        lib.dsa_vocab_workspace_bytes.restype = ctypes.c_size_t
         for name, st in (
             ("dsa_add_ln_fwd", DsaLnArgs),
             ("dsa_add_ln_bwd", DsaLnArgs),
@@ -392,6 +464,10 @@ def load() -> ctypes.CDLL:
             ("dsa_add_rms_bwd", DsaRmsArgs),
             ("dsa_embed_fwd", DsaEmbedArgs),
             ("dsa_embed_bwd", DsaEmbedArgs),
+            ("dsa_logprobs_fwd", DsaLogprobsArgs),
+            ("dsa_logprobs_bwd", DsaLogprobsArgs),
+            ("dsa_distill_fwd", DsaDistillArgs),
+            ("dsa_distill_bwd", DsaDistillArgs),
         ):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]

@@ -1,6 +1,7 @@
-// hidden_ext.cpp — the operators on hidden states for PyTorch tensors: the
-// argument checks, the results' memory, the calls of libdsa.so's entry points
-// (include/dsa_block.h) on the current stream, and their autograd nodes.
+// hidden_ext.cpp — the operators on hidden states, and (vocab_ext.h) those on a
+// vocabulary's logits, for PyTorch tensors: the argument checks, the results'
+// memory, the calls of libdsa.so's entry points (include/dsa_block.h,
+// include/dsa_vocab.h) on the current stream, and their autograd nodes.
 //
 // It is host code of its own because a call's host time is what bounds these
 // operators on all but large batches.  A forward and backward of 256 x 128
@@ -21,6 +22,7 @@
 
 #include "../../include/dsa.h"
 #include "../../include/dsa_block.h"
+#include "../../include/dsa_vocab.h"
 
 namespace {
 
@@ -155,12 +157,11 @@ bool here(std::initializer_list<const Tensor*> ts) {
 
 // The gradients of a backward whose own graph is asked for: they raise when
 // that is walked.
-variable_list once(variable_list g, bool graph) {
+variable_list once(variable_list g, bool graph, const char* why = "the operators on hidden states are not twice differentiable") {
   if (!graph) return g;
   for (Tensor& t : g)
     if (t.defined()) t = t.detach().set_requires_grad(true);
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      "the operators on hidden states are not twice differentiable", (int64_t)g.size());
+  const auto error = std::make_shared<torch::autograd::DelayedError>(why, (int64_t)g.size());
   return (*error)(std::move(g));
 }
 
@@ -520,6 +521,8 @@ Maybe embed(const Tensor& ids, const Tensor& weight, int64_t padding, double sca
   return Embed::apply(ids, weight, padding, scale, out);
 }
 
+#include "vocab_ext.h"
+
 }  // namespace
 
 // The functions named like an operator record autograd, and give None for a call
@@ -538,4 +541,10 @@ PYBIND11_MODULE(_hidden_ext, m) {
   m.def("embed", torch::wrap_pybind_function_no_gil(embed));
   m.def("embed_fwd", torch::wrap_pybind_function_no_gil(embed_fwd));
   m.def("embed_bwd", torch::wrap_pybind_function_no_gil(embed_bwd));
+  m.def("logprobs", torch::wrap_pybind_function_no_gil(logprobs));
+  m.def("logprobs_fwd", torch::wrap_pybind_function_no_gil(logprobs_fwd));
+  m.def("logprobs_bwd", torch::wrap_pybind_function_no_gil(logprobs_bwd));
+  m.def("distill", torch::wrap_pybind_function_no_gil(distill));
+  m.def("distill_fwd", torch::wrap_pybind_function_no_gil(distill_fwd));
+  m.def("distill_bwd", torch::wrap_pybind_function_no_gil(distill_bwd));
 }

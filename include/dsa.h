@@ -301,7 +301,7 @@ const char* dsa_last_error(void);
 /* Library version, for the loader's compatibility check: DSA_VERSION of the
  * headers that the library was built from.  Code compiled against these headers
  * compares the two before it passes a struct. */
-#define DSA_VERSION 14
+#define DSA_VERSION 15
 int dsa_version(void);
 
 #ifdef __cplusplus
