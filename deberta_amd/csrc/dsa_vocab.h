@@ -12,7 +12,10 @@
 //
 // x - m is formed before its scaling: m / T rounded by itself would move every
 // probability of a row whose logits are large, and a row of the type's lowest
-// value (a mask that leaves nothing) would overflow; so it has p = 1 / V.
+// value (a mask that leaves nothing) would overflow; so it has p = 1 / V.  (One
+// fused product from a rounded origin, with this form beside it for such rows, and
+// the entropy's guard against 0 times -inf taken out of the loop: a fifth fewer
+// instructions, and no faster: 67 to 104 registers a lane cost what they saved.)
 //
 // The k largest come out of the same pass.  It keeps the maximum of each
 // segment of 64 columns.  The k segments whose maxima are largest (equal ones:
@@ -33,6 +36,7 @@ namespace voc {
 constexpr int kSeg = 64;      // columns of a segment
 constexpr int kBins = 1024;   // of a selection's histogram
 constexpr int kMost = 128;    // entries of a row
+constexpr int kRow = 1 << 30;  // vectors: as many as a row has
 constexpr int kUnroll = 4;    // 16-byte loads in flight a lane
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -49,6 +53,10 @@ struct VocabRows {
   int64_t row0;    // the launch's first row
   int V, top, K, ids64, teacher_bf16;
   int keys;        // LDS words for a selection's keys
+  int parts, per;  // blocks a row, 16-byte vectors a block
+  float4* part;    // [N, parts]: m, s, u of a part
+  uint32_t* seg;   // [N, segs]: the segments' maxima
+  int segs;
   float inv_t, t;
   float c;         // log2(e) / T
 };
@@ -132,16 +140,19 @@ DSA_DEV int64_t load_id(const void* ids, int ids64, int64_t i) {
 // ---------------------------------------------------------------------------
 // the running sums
 
+// x's exponent in a row with maximum m: c = log2(e) / T
+DSA_DEV float exponent(float x, float m, float c) { return (x - m) * c; }
+
 struct Run {
-  float m, s, u;
+  float m, s, u;  // u in units of ln 2
 };
 DSA_DEV Run run_none() { return Run{kLowest, 0.f, 0.f}; }
 
-// the sums as of a larger maximum
+// the sums as of a maximum that is no smaller
 template <bool ENT>
 DSA_DEV void raise(Run& r, float m, float c) {
-  const float d = fmaxf((r.m - m) * c, kFar), f = exp2_(d);
-  if (ENT) r.u = f * fmaf(d, r.s, r.u);  // in units of ln 2
+  const float d = fmaxf(exponent(r.m, m, c), kFar), f = exp2_(d);
+  if (ENT) r.u = f * fmaf(d, r.s, r.u);
   r.s *= f;
   r.m = m;
 }
@@ -151,7 +162,7 @@ DSA_DEV void add(Run& r, const float* x, float most, float c) {
   float s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float t = (x[e] - r.m) * c, p = exp2_(t);
+    const float t = exponent(x[e], r.m, c), p = exp2_(t);
     s[e & 1] += p;
     if (ENT) u[e & 1] = fmaf(p, fmaxf(t, kFar), u[e & 1]);  // 0 where t is -inf
   }
@@ -194,20 +205,21 @@ DSA_DEV Run block_run(Run r, float c, float* red) {
 }
 
 // ---------------------------------------------------------------------------
-// a row in 16-byte accesses: it starts `pad` values behind a 16-byte border,
-// and positions count from there.  Vectors v0 .. v1 - 1 lie in the row whole;
-// the values before and behind them are taken one by one, a lane each.
+// a row in 16-byte accesses: it starts `pad` values behind a 128-byte border, and
+// positions count from there, so that a wave's access is of whole lines.  Vectors
+// v0 .. v1 - 1 lie in the row whole; the values before and behind them are taken
+// one by one, a lane each.
 template <typename T>
 struct Line {
   static constexpr int N = Vec<T>::N;
   const T* row;
   const T* base;  // of position 0
-  int pad, v0, v1, head, edges, tail0;
-  DSA_DEV Line(const void* x, int64_t stride, int64_t r, int V) {
+  int V, pad, v0, v1, head, edges, tail0;
+  DSA_DEV Line(const void* x, int64_t stride, int64_t r, int cols) : V(cols) {
     row = static_cast<const T*>(x) + r * stride;
-    pad = (int)(reinterpret_cast<uintptr_t>(row) & 15u) / (int)sizeof(T);
+    pad = (int)(reinterpret_cast<uintptr_t>(row) & 127u) / (int)sizeof(T);
     base = row - pad;
-    v0 = pad ? 1 : 0;
+    v0 = (pad + N - 1) / N;
     v1 = max((int)(((int64_t)pad + V) / N), v0);
     head = min(V, v0 * N - pad);
     tail0 = min(V, v1 * N - pad);  // the row's first value behind the vectors
@@ -217,51 +229,70 @@ struct Line {
   DSA_DEV raw load(int v) const { return reinterpret_cast<const raw*>(base)[v]; }
 };
 
-// The sums of a thread over its share of the row; with SEG the segments'
-// maxima into keys (all of them: the caller has cleared them, and waits).
+// The sums of a thread over its share of positions from `from` to `to` vectors (a
+// multiple of 64 each, or the row's end); with SEG the keys of the maxima of the
+// `segs` segments from there on, for which the caller waits.
 template <typename T, int NT, bool ENT, bool SEG>
-DSA_DEV Run stream(const Line<T>& l, float c, uint32_t* keys) {
-  constexpr int N = Vec<T>::N, E = kUnroll * N;
+DSA_DEV Run stream(const Line<T>& l, int from, int to, float c, uint32_t* keys, int segs) {
+  constexpr int N = Vec<T>::N, E = kUnroll * N, L = kSeg / N;
   const int tid = threadIdx.x;
+  const int first = max(from, l.v0), end = min(to, l.v1);
   Run r = run_none();
-  const int end = l.v1 > l.v0 ? l.v1 : 0;
-  for (int vb = 0; vb < end; vb += NT * kUnroll) {
-    raw q[kUnroll];
+  if (SEG) {
+    for (int i = tid; i < segs; i += NT) keys[i] = 0xff800000u;  // -inf
+    __syncthreads();
+  }
+  // the next batch is loaded before this one is worked on (behind the end the
+  // last vector again)
+  raw next[kUnroll];
+  if (first < end) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) q[i] = l.load(min(max(vb + i * NT + tid, l.v0), l.v1 - 1));
-    if (vb < l.v0 || vb + NT * kUnroll > l.v1) {
+    for (int i = 0; i < kUnroll; ++i) next[i] = l.load(min(max(from + i * NT + tid, first), end - 1));
+    for (int vb = from; vb < end; vb += NT * kUnroll) {
+      raw q[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        const int v = vb + i * NT + tid;
-        if (v < l.v0 || v >= l.v1) q[i] = raw_none<T>();
+      for (int i = 0; i < kUnroll; ++i) q[i] = next[i];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) next[i] = l.load(min(vb + (i + kUnroll) * NT + tid, end - 1));
+      if (vb < first || vb + NT * kUnroll > end) {
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+          const int v = vb + i * NT + tid;
+          if (v < first || v >= end) q[i] = raw_none<T>();
+        }
       }
-    }
-    float x[E], most[kUnroll];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      unpack<T>(q[i], x + i * N);
-      most[i] = max_of<N>(x + i * N);
-    }
-    add<E, ENT>(r, x, max_of<kUnroll>(most), c);
-    if (SEG) {
+      float x[E], most[kUnroll];
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
-        float g = most[i];  // over the 64 / N lanes of the segment
-        g = max2(g, hid::dpp<0xB1>(g));
-        g = max2(g, hid::dpp<0x4E>(g));
-        g = max2(g, hid::dpp<0x141>(g));
-        if (N == 4) g = max2(g, hid::dpp<0x140>(g));
-        const int v = vb + i * NT + tid;
-        if (tid % (kSeg / N) == 0 && v < l.v1) keys[v / (kSeg / N)] = key_of<T>(g);
+        unpack<T>(q[i], x + i * N);
+        most[i] = max_of<N>(x + i * N);
+      }
+      add<E, ENT>(r, x, max_of<kUnroll>(most), c);
+      if (SEG) {
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+          float g = most[i];  // over the L lanes of the segment
+          g = max2(g, hid::dpp<0xB1>(g));
+          g = max2(g, hid::dpp<0x4E>(g));
+          g = max2(g, hid::dpp<0x141>(g));
+          if (N == 4) g = max2(g, hid::dpp<0x140>(g));
+          const int v = vb + i * NT + tid;
+          if (tid % L == 0 && v < end) keys[(v - from) / L] = __builtin_bit_cast(uint32_t, g);
+        }
       }
     }
   }
-  if (SEG) __syncthreads();
-  if (tid < l.edges) {
-    const int j = l.edge(tid);
+  if (SEG) {
+    __syncthreads();
+    for (int i = tid; i < segs; i += NT) keys[i] = key_of<T>(__builtin_bit_cast(float, keys[i]));
+    __syncthreads();
+  }
+  const int head = from == 0 ? l.head : 0, tail = l.v1 >= from && l.v1 < to ? l.V - l.tail0 : 0;
+  if (tid < head + tail) {
+    const int j = tid < head ? tid : l.tail0 + (tid - head);
     const float x = (float)l.row[j];
     add<1, ENT>(r, &x, max2(x, kLowest), c);
-    if (SEG) atomicMax(&keys[(l.pad + j) / kSeg], key_of<T>(x));
+    if (SEG) atomicMax(&keys[(l.pad + j) / kSeg - from / L], key_of<T>(x));
   }
   return r;
 }
@@ -269,21 +300,28 @@ DSA_DEV Run stream(const Line<T>& l, float c, uint32_t* keys) {
 // ---------------------------------------------------------------------------
 // the largest
 
+constexpr uint32_t kCands = 512;  // segments, and values, that compete in write_top
+
 struct Shared {
   uint32_t* keys;
-  uint32_t* hist;  // kBins
-  int* list;       // kMost
+  uint32_t* hist;    // kBins
+  uint64_t* cand;    // kCands
+  int* seg;          // kCands
+  int* list;         // kMost
   uint32_t* picked;  // kMost
-  uint32_t* word;  // 24
+  uint32_t* word;    // 24
 };
-constexpr int kSharedWords = kBins + 2 * kMost + 24;
-DSA_DEV Shared shared_at(uint32_t* lds, int keys) {
+constexpr int kSharedWords = kBins + 3 * kCands + 2 * kMost + 24;
+DSA_DEV Shared shared_at(uint32_t* lds, int keys) {  // keys: a multiple of 4
   Shared s;
   s.keys = lds;
   s.hist = lds + keys;
-  s.list = reinterpret_cast<int*>(s.hist + kBins);
-  s.picked = s.hist + kBins + kMost;
-  s.word = s.hist + kBins + 2 * kMost;
+  uint32_t* at = s.hist + kBins;
+  s.cand = reinterpret_cast<uint64_t*>(at);
+  s.seg = reinterpret_cast<int*>(at + 2 * kCands);
+  s.list = s.seg + kCands;
+  s.picked = reinterpret_cast<uint32_t*>(s.list + kMost);
+  s.word = s.picked + kMost;
   return s;
 }
 
@@ -309,19 +347,23 @@ DSA_DEV uint32_t block_before(uint32_t x, uint32_t* w) {
   return all - x;
 }
 
-// The places of the `need` largest of keys[0 .. n), equal ones by their place,
-// into sh.list in the order of their places (0 < need <= n, need <= kMost).
+// The places of the `need` largest of key(0) .. key(n - 1), equal ones by their
+// place, into sh.list in the order of their places (0 < need <= n, need <= kMost,
+// n < 2^16).
 //
 // Keys are counted into bins of equal width between the least and the largest,
 // the bin that holds the last one wanted is cut into bins again, and so on until
 // all of a bin are wanted or its keys are equal: one round where the keys span
 // at most 1024, at most four (10 bits a round).
-template <int NT>
-DSA_DEV void choose(const Shared& sh, int n, int need) {
+template <int NT, typename F>
+DSA_DEV void choose(const Shared& sh, int n, int need, F key) {
   constexpr int W = NT / 64, PER = kBins / NT;
   const int tid = threadIdx.x;
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i = tid; i < n; i += NT) lo = min(lo, sh.keys[i]), hi = max(hi, sh.keys[i]);
+  for (int i = tid; i < n; i += NT) {
+    const uint32_t k = key(i);
+    lo = min(lo, k), hi = max(hi, k);
+  }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) lo = min(lo, (uint32_t)__shfl_xor(lo, o)), hi = max(hi, (uint32_t)__shfl_xor(hi, o));
   if constexpr (W > 1) {
@@ -338,7 +380,7 @@ DSA_DEV void choose(const Shared& sh, int n, int need) {
     for (int i = tid; i < kBins; i += NT) sh.hist[i] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += NT) {
-      const uint32_t k = sh.keys[i];
+      const uint32_t k = key(i);
       if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
     }
     __syncthreads();
@@ -364,45 +406,190 @@ DSA_DEV void choose(const Shared& sh, int n, int need) {
   const int per = (n + NT - 1) / NT, first = min(n, tid * per), last = min(n, first + per);
   uint32_t counts = 0;  // above lo, and at lo in the upper half
   for (int i = first; i < last; ++i) {
-    const uint32_t k = sh.keys[i];
+    const uint32_t k = key(i);
     counts += k > lo ? 1u : k == lo ? 0x10000u : 0u;
   }
   const uint32_t before = block_before<NT>(counts, sh.word);
   uint32_t over = before & 0xffffu, at = before >> 16;
   for (int i = first; i < last; ++i) {
-    const uint32_t k = sh.keys[i];
+    const uint32_t k = key(i);
     if (k > lo || (k == lo && at < equal)) sh.list[over + min(at, equal)] = i;
     over += k > lo, at += k == lo;
   }
   __syncthreads();
 }
 
-// The row's largest, from its segments' maxima in sh.keys.
+// A number that at least k of the threads' values reach: the k-th largest of the
+// maxima of 256 groups of threads, cut to its upper 16 bits, which one wave
+// finds a bit at a time by counting the groups that reach it.
+template <int NT>
+DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh) {
+  static_assert(NT >= 256 && NT <= kBins && kMost <= 256, "");
+  const int tid = threadIdx.x;
+  uint32_t* all = sh.hist;
+  all[tid] = most;
+  __syncthreads();
+  if (tid < 64) {
+    uint32_t g[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      g[u] = 0;
+      for (int i = tid + 64 * u; i < NT; i += 256) g[u] = max(g[u], all[i]);
+    }
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t trial = t | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) n += __popcll(__ballot(g[u] >= trial));
+      t = n >= k ? trial : t;
+    }
+    if (tid == 0) sh.word[0] = t;
+  }
+  __syncthreads();
+  return sh.word[0];
+}
+
+DSA_DEV int round_8(int n) { return (n + 7) & ~7; }
+
+template <typename T>
+DSA_DEV uint32_t wide_key(uint32_t k) { return sizeof(T) == 2 ? k << 16 : k; }
+
+// One of the row's largest.
+template <typename T>
+DSA_DEV void put_top(const VocabRows& p, int64_t r, int rank, int j, uint32_t key, float m, float ln_s) {
+  p.top_ids[r * p.top + rank] = j;
+  p.top_lp[r * p.top + rank] = fmaf(exponent(of_key<T>(key), m, p.c), kLn2, -ln_s);
+}
+
+// The row's largest, from its segments' maxima in sh.keys: those of the k
+// segments whose maxima are largest (read again at every step: this is for rows
+// with thousands of equal values).
 template <typename T, int NT>
-DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, float m, float ln_s) {
+DSA_DEV void top_of_segments(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, float m, float ln_s) {
   const int tid = threadIdx.x, k = p.top;
   const int segs = (l.pad + p.V - 1) / kSeg + 1, found = min(k, segs);
-  choose<NT>(sh, segs, found);
+  choose<NT>(sh, segs, found, [&](int i) { return sh.keys[i]; });
   if (tid < found) sh.picked[tid] = (uint32_t)sh.list[tid];
   __syncthreads();
-  for (int i = tid; i < found * kSeg; i += NT) {
-    const int j = (int)sh.picked[i / kSeg] * kSeg + i % kSeg - l.pad;
-    sh.keys[i] = j >= 0 && j < p.V ? key_of<T>((float)l.row[j]) : 0u;
+  const auto column = [&](int i) { return (int)sh.picked[i / kSeg] * kSeg + i % kSeg - l.pad; };
+  const auto key = [&](int i) {
+    const int j = column(i);
+    return j >= 0 && j < p.V ? key_of<T>((float)l.row[j]) : 0u;
+  };
+  choose<NT>(sh, found * kSeg, k, key);
+  if (tid < k) sh.hist[tid] = key(sh.list[tid]);
+  __syncthreads();
+  if (tid < k) {
+    const uint32_t mine = sh.hist[tid];
+    int rank = 0;
+    for (int o = 0; o < k; ++o) rank += sh.hist[o] > mine || (sh.hist[o] == mine && o < tid);
+    put_top<T>(p, r, rank, column(sh.list[tid]), mine, m, ln_s);
+  }
+}
+
+// f(vector's values, column of the first, of the n that are the row's) for the
+// 16-byte pieces of the first `found` segments of sh.seg, four loads of a thread
+// in flight.
+template <typename T, int NT, typename F>
+DSA_DEV void values_of(const Line<T>& l, const Shared& sh, int found, F f) {
+  constexpr int N = Vec<T>::N, L = kSeg / N, U = 4;
+  const int n = found * L;
+  for (int i0 = threadIdx.x; i0 < n; i0 += U * NT) {
+    int v[U];
+    raw q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      v[u] = i < n ? sh.seg[i / L] * L + i % L : -1;
+      q[u] = raw_none<T>();
+      if (v[u] >= l.v0 && v[u] < l.v1) q[u] = l.load(v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v[u] < 0) continue;
+      float x[N];
+      const int j = v[u] * N - l.pad;
+      if (v[u] >= l.v0 && v[u] < l.v1) {
+        unpack<T>(q[u], x);
+        f(x, j, 0, N);
+      } else {
+        const int lo = max(0, -j), hi = min(N, l.V - j);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = e >= lo && e < hi ? (float)l.row[j + e] : -__builtin_inff();
+        f(x, j, lo, hi);
+      }
+    }
+  }
+}
+
+// The same where few values compete, as nearly always: a bound that k values
+// reach leaves a few segments, and of those a few values, whose ranks are counted
+// (value and place in one number, so that equal values go by their place).  Where
+// there are more than kCands of either, top_of_segments takes over.
+template <typename T, int NT>
+DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, float m, float ln_s) {
+  constexpr int N = Vec<T>::N;
+  const int tid = threadIdx.x, k = p.top;
+  const int segs = (l.pad + p.V - 1) / kSeg + 1;
+  const uint32_t least = wide_key<T>(key_of<T>(-__builtin_inff()));
+  uint32_t most = 0;
+  for (int i = tid; i < segs; i += NT) most = max(most, sh.keys[i]);
+  if (tid == 0) sh.word[1] = 0, sh.word[2] = 0;
+  uint32_t bound = reached<NT>(wide_key<T>(most), k, sh);
+  for (int i = tid; i < segs; i += NT) {
+    if (wide_key<T>(sh.keys[i]) < bound) continue;
+    const uint32_t at = atomicAdd(&sh.word[1], 1u);
+    if (at < kCands) sh.seg[at] = i;
   }
   __syncthreads();
-  choose<NT>(sh, found * kSeg, k);
-  for (int t = tid; t < k; t += NT) {
-    const int i = sh.list[t];
-    const uint32_t mine = sh.keys[i];
-    int rank = 0;
-    for (int o = 0; o < k; ++o) {
-      const uint32_t other = sh.keys[sh.list[o]];
-      rank += other > mine || (other == mine && o < t);
+  const uint32_t found = sh.word[1];
+  for (int round = 0; round < 2 && found <= kCands; ++round) {
+    // the segments' bound may be far below their values', where there are few segments
+    if (round == 1 || (segs < 4 * k && found * kSeg > kCands)) {
+      round = 1;
+      float top = -__builtin_inff();
+      values_of<T, NT>(l, sh, (int)found, [&](const float* x, int, int, int) { top = max2(top, max_of<N>(x)); });
+      bound = max(bound, reached<NT>(wide_key<T>(key_of<T>(top)), k, sh));
     }
-    const int j = (int)sh.picked[i / kSeg] * kSeg + i % kSeg - l.pad;
-    p.top_ids[r * k + rank] = j;
-    p.top_lp[r * k + rank] = (of_key<T>(mine) - m) * p.inv_t - ln_s;
+    const bool all = bound <= least;  // NaN are -inf here
+    const float limit = all ? -__builtin_inff() : of_key<T>(sizeof(T) == 2 ? bound >> 16 : bound);
+    values_of<T, NT>(l, sh, (int)found, [&](const float* x, int j, int lo, int hi) {
+      if (!all && !(max_of<N>(x) >= limit)) return;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (e < lo || e >= hi || !(all || x[e] >= limit)) continue;
+        const uint32_t at = atomicAdd(&sh.word[2], 1u);
+        if (at < kCands) sh.cand[at] = (uint64_t)key_of<T>(x[e]) << 32 | (uint32_t)~(j + e);
+      }
+    });
+    __syncthreads();
+    const int n = (int)sh.word[2];
+    if (n <= (int)kCands) {
+      // up to a multiple of 8, which is what a step compares
+      if (tid >= n && tid < round_8(n)) sh.cand[tid] = 0;
+      if (NT < (int)kCands && tid + NT >= n && tid + NT < round_8(n)) sh.cand[tid + NT] = 0;
+      __syncthreads();
+      for (int t = tid; t < n; t += NT) {
+        const uint64_t mine = sh.cand[t];
+        int rank = 0;
+        for (int o = 0; o < n; o += 8) {
+          uint64_t other[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) other[u] = sh.cand[o + u];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) rank += other[u] > mine;
+        }
+        if (rank < k) put_top<T>(p, r, rank, (int)~(uint32_t)mine, (uint32_t)(mine >> 32), m, ln_s);
+      }
+      return;
+    }
+    __syncthreads();
+    if (tid == 0) sh.word[2] = 0;
+    __syncthreads();
   }
+  top_of_segments<T, NT>(l, p, r, sh, m, ln_s);
 }
 
 // ---------------------------------------------------------------------------
@@ -421,12 +608,16 @@ DSA_DEV void write_none(const VocabRows& p, int64_t r) {
   for (int t = tid; t < p.top; t += NT) p.top_lp[r * p.top + t] = 0.f, p.top_ids[r * p.top + t] = -1;
 }
 
-// One thread: the row's results.
+// The given token's logit, NaN outside the vocabulary.
 template <typename T>
-DSA_DEV void write_row(const Line<T>& l, const VocabRows& p, int64_t r, const Run& all, float ln_s, int64_t id) {
+DSA_DEV float given(const Line<T>& l, const VocabRows& p, int64_t id) {
+  return p.lp && id >= 0 && id < p.V ? (float)l.row[id] : __builtin_nanf("");
+}
+
+// One thread: the row's results; x: the given token's logit.
+DSA_DEV void write_row(const VocabRows& p, int64_t r, const Run& all, float ln_s, float x) {
   const float ent = ln_s - kLn2 * all.u / all.s;
-  if (p.lp)
-    p.lp[r] = id >= 0 && id < p.V ? ((float)l.row[id] - all.m) * p.inv_t - ln_s : __builtin_nanf("");
+  if (p.lp) p.lp[r] = fmaf(exponent(x, all.m, p.c), kLn2, -ln_s);
   if (p.ent) p.ent[r] = ent;
   if (p.lse) p.lse[r] = fmaf(all.m, p.inv_t, ln_s);
   if (p.stats) p.stats[r] = float4{all.m, ln_s, ent, 1.f / all.s};
@@ -434,7 +625,7 @@ DSA_DEV void write_row(const Line<T>& l, const VocabRows& p, int64_t r, const Ru
 
 template <typename T, int NT, bool TOP>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x;
   const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;
@@ -443,14 +634,84 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
     return;
   }
   const Line<T> l(p.x, p.xs, r, p.V);
-  if (TOP) {
-    for (int i = threadIdx.x; i < p.keys; i += NT) lds[i] = 0;
-    __syncthreads();
-  }
-  const Run all = block_run<NT, true>(stream<T, NT, true, TOP>(l, p.c, lds), p.c, red);
+  const float x = given(l, p, id);  // early: its way from memory is long
+  const Run all = block_run<NT, true>(stream<T, NT, true, TOP>(l, 0, kRow, p.c, lds, p.segs), p.c, red);
   const float ln_s = logf(all.s);
-  if (threadIdx.x == 0) write_row(l, p, r, all, ln_s, id);
-  if (TOP) {
+  if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
+  if constexpr (TOP) {
+    __syncthreads();
+    write_top<T, NT>(l, p, r, shared_at(lds, p.keys), all.m, ln_s);
+  }
+}
+
+// A part of a row by a block, where rows are few or long: its sums, and its
+// segments' maxima, for the row's join.
+template <typename T, int NT, bool ENT, bool SEG>
+DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys, float* red) {
+  constexpr int L = kSeg / Vec<T>::N;
+  const Line<T> l(p.x, p.xs, r, p.V);
+  const int from = part * p.per;
+  const int first = from / L, n = min(p.per / L, p.segs - first);  // segments
+  const Run all = block_run<NT, ENT>(stream<T, NT, ENT, SEG>(l, from, from + p.per, p.c, keys, n), p.c, red);
+  if (threadIdx.x == 0) p.part[r * p.parts + part] = float4{all.m, all.s, all.u, 0.f};
+  if (SEG) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT) p.seg[r * p.segs + first + i] = keys[i];
+  }
+}
+
+template <typename T, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
+  extern __shared__ __align__(16) uint32_t lds[];
+  __shared__ float red[3 * (NT / 64)];
+  const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
+  if (p.ids && load_id(p.ids, p.ids64, r) == p.ignore) return;
+  write_part<T, NT, true, TOP>(p, r, blockIdx.x % (uint32_t)p.parts, lds, red);
+}
+
+// The row's sums out of its parts', in every thread of the block.
+template <int NT, bool ENT>
+DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float* red) {
+  Run all = run_none();
+  for (int i = threadIdx.x; i < p.parts; i += NT) {
+    const float4 q = p.part[r * p.parts + i];
+    Run w{q.x, q.y, q.z};
+    const float m = max2(all.m, w.m);
+    raise<ENT>(all, m, p.c);
+    raise<ENT>(w, m, p.c);
+    all.s += w.s, all.u += w.u;
+  }
+  return block_run<NT, ENT>(all, p.c, red);
+}
+
+template <typename T, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_join_kernel(VocabRows p) {
+  extern __shared__ __align__(16) uint32_t lds[];
+  __shared__ float red[3 * (NT / 64)];
+  const int64_t r = p.row0 + blockIdx.x;
+  const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;
+  if (p.ids && id == p.ignore) {
+    write_none<NT>(p, r);
+    return;
+  }
+  const Line<T> l(p.x, p.xs, r, p.V);
+  const float x = given(l, p, id);
+  if constexpr (TOP) {
+    // eight loads in flight a thread; keys past the segments are not read
+    const uint32_t* seg = p.seg + r * p.segs;
+    for (int i = threadIdx.x; i < p.segs; i += 8 * NT) {
+      uint32_t k[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) k[u] = seg[min(i + u * NT, p.segs - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u * NT < p.segs) lds[i + u * NT] = k[u];
+    }
+  }
+  const Run all = join_parts<NT, true>(p, r, red);
+  const float ln_s = logf(all.s);
+  if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
+  if constexpr (TOP) {
     __syncthreads();
     write_top<T, NT>(l, p, r, shared_at(lds, p.keys), all.m, ln_s);
   }
@@ -510,27 +771,23 @@ DSA_DEV Entries entries_of(const VocabRows& p, int64_t r) {
   return e;
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
-  __shared__ float red[3 * (NT / 64)];
-  const int64_t r = p.row0 + blockIdx.x;
-  const Entries e = entries_of(p, r);  // by every wave
-  if (!e.any) {
-    if (threadIdx.x == 0) {
-      p.loss[r] = 0.f;
-      if (p.stats) p.stats[r] = float4{0.f, 0.f, 0.f, 0.f};
-    }
-    return;
-  }
-  const Line<T> l(p.x, p.xs, r, p.V);
-  const Run all = block_run<NT, false>(stream<T, NT, false, false>(l, p.c, nullptr), p.c, red);
+// What a row without entries gives.
+DSA_DEV void write_no_loss(const VocabRows& p, int64_t r) {
+  if (threadIdx.x != 0) return;
+  p.loss[r] = 0.f;
+  if (p.stats) p.stats[r] = float4{0.f, 0.f, 0.f, 0.f};
+}
+
+// By one wave: the row's loss.
+template <typename T>
+DSA_DEV void write_loss(const VocabRows& p, int64_t r, const Entries& e, const Run& all) {
+  const T* row = static_cast<const T*>(p.x) + r * p.xs;
   const float ln_s = logf(all.s);
-  if (threadIdx.x >= 64) return;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (e.id[i] < 0 || e.id[i] >= p.V || e.q[i] == 0.f) continue;
-    const float log_p = ((float)l.row[e.id[i]] - all.m) * p.inv_t - ln_s;
+    const float log_p = fmaf(exponent((float)row[e.id[i]], all.m, p.c), kLn2, -ln_s);
     sum += e.q[i] * (e.log_q[i] - log_p);
   }
   sum = hid::lanes_sum<64>(sum);
@@ -538,6 +795,44 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
     p.loss[r] = e.bad ? __builtin_nanf("") : p.t * p.t * sum;
     if (p.stats) p.stats[r] = float4{all.m, ln_s, 0.f, 1.f / all.s};
   }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
+  __shared__ float red[3 * (NT / 64)];
+  const int64_t r = p.row0 + blockIdx.x;
+  const Entries e = entries_of(p, r);  // by every wave
+  if (!e.any) {
+    write_no_loss(p, r);
+    return;
+  }
+  const Line<T> l(p.x, p.xs, r, p.V);
+  const Run all = block_run<NT, false>(stream<T, NT, false, false>(l, 0, kRow, p.c, nullptr, 0), p.c, red);
+  if (threadIdx.x < 64) write_loss<T>(p, r, e, all);
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_part_kernel(VocabRows p) {
+  __shared__ float red[3 * (NT / 64)];
+  const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
+  bool any = false;  // by every wave
+  for (int k = threadIdx.x & 63; k < p.K; k += 64) any |= load_id(p.ids, p.ids64, r * p.K + k) >= 0;
+  if (__ballot(any) == 0) return;
+  write_part<T, NT, false, false>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr, red);
+}
+
+// A wave a row.  (4096 rows of 128 entries 14 us, each entry's logit a line of its
+// own from memory; handed on by the parts, which had them in the caches, 6 and 5
+// more in the parts.)
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(VocabRows p) {
+  const int64_t r = p.row0 + blockIdx.x;
+  const Entries e = entries_of(p, r);
+  if (!e.any) {
+    write_no_loss(p, r);
+    return;
+  }
+  write_loss<T>(p, r, e, join_parts<64, false>(p, r, nullptr));
 }
 
 // ---------------------------------------------------------------------------
@@ -550,8 +845,8 @@ struct Grad {
   int n;
 };
 template <bool B>
-DSA_DEV float grad_of(const Grad& g, float c, float x) {
-  const float t = (x - g.m) * c, e = exp2_(t);
+DSA_DEV float grad_of(const Grad& g, float t) {
+  const float e = exp2_(t);
   return B ? e * fmaf(g.b, fmaxf(t, kFar), g.a) : e * g.a;
 }
 
@@ -569,42 +864,65 @@ DSA_DEV void pack(const float* v, raw& r) {
   }
 }
 
-// A row of the gradient in 16-byte stores; the logits' row may lie otherwise
-// to 16-byte borders.
-template <typename T, int NT, bool B>
-DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Grad& g, const int* col, const float* term) {
+// A block's part of a row: vectors lo .. hi - 1, and the row's single values with
+// the first part.
+template <typename T>
+struct Part {
+  Line<T> l;
+  int from, lo, hi, edges;
+  DSA_DEV Part(const VocabRows& p, int64_t r, int part) : l(p.dx, p.dxs, r, p.V) {
+    from = part * p.per, lo = max(from, l.v0), hi = min(l.v1, from + p.per);
+    edges = part == 0 ? l.edges : 0;
+  }
+  DSA_DEV bool has(int j) const {
+    const int at = l.pad + j, v = at / Line<T>::N;
+    return v >= l.v0 && v < l.v1 ? v >= lo && v < hi : edges > 0;
+  }
+};
+
+// A part of a row of the gradient in 16-byte stores; the logits' row may lie
+// otherwise to 16-byte borders.  FAR: past the caches, for gradients that do not
+// stay in them (their lines would be written back while the next kernel reads).
+template <typename T, int NT, bool B, bool FAR>
+DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Part<T>& part, const Grad& g, const int* col, const float* term) {
   constexpr int N = Vec<T>::N;
   typedef typename std::conditional<sizeof(T) == 2, raw2, raw4>::type rawu;
   const int tid = threadIdx.x;
-  const Line<T> l(p.dx, p.dxs, r, p.V);
+  const Line<T>& l = part.l;
   T* out = const_cast<T*>(l.row);
   const T* row = static_cast<const T*>(p.x) + r * p.xs;
   const T* base = row - l.pad;
-  for (int vb = l.v0; vb < l.v1; vb += NT * kUnroll) {
+  for (int vb = part.from; vb < part.hi && part.lo < part.hi; vb += NT * kUnroll) {
     raw q[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      q[i] = *reinterpret_cast<const rawu*>(base + (int64_t)min(vb + i * NT + tid, l.v1 - 1) * N);
+    for (int i = 0; i < kUnroll; ++i) {
+      const rawu* at = reinterpret_cast<const rawu*>(base + (int64_t)min(max(vb + i * NT + tid, part.lo), part.hi - 1) * N);
+      q[i] = FAR ? __builtin_nontemporal_load(at) : *at;
+    }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int v = vb + i * NT + tid;
       float x[N];
       unpack<T>(q[i], x);
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = grad_of<B>(g, p.c, x[e]);
+      for (int e = 0; e < N; ++e) x[e] = grad_of<B>(g, exponent(x[e], g.m, p.c));
       pack<T>(x, q[i]);
-      if (v < l.v1) reinterpret_cast<raw*>(out - l.pad)[v] = q[i];
+      if (v >= part.lo && v < part.hi) {
+        raw* to = reinterpret_cast<raw*>(out - l.pad) + v;
+        if (FAR) __builtin_nontemporal_store(q[i], to);
+        else *to = q[i];
+      }
     }
   }
-  if (tid < l.edges) {
+  if (tid < part.edges) {
     const int j = l.edge(tid);
-    out[j] = (T)grad_of<B>(g, p.c, (float)row[j]);
+    out[j] = (T)grad_of<B>(g, exponent((float)row[j], g.m, p.c));
   }
   // the columns with terms are written again, behind the barrier
   __syncthreads();
   for (int t = tid; t < g.n; t += NT) {
     const int j = col[t];
-    if (j < 0) continue;
+    if (j < 0 || !part.has(j)) continue;
     float sum = 0.f;
     bool first = true;
     for (int o = 0; o < g.n; ++o) {
@@ -612,27 +930,28 @@ DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Grad& g, const int*
       if (same) sum += term[o];
       if (same && o < t) first = false;
     }
-    if (first) out[j] = (T)(grad_of<B>(g, p.c, (float)row[j]) + sum);
+    if (first) out[j] = (T)(grad_of<B>(g, exponent((float)row[j], g.m, p.c)) + sum);
   }
 }
 
 template <typename T, int NT>
-DSA_DEV void write_zeros(const VocabRows& p, int64_t r) {
-  const Line<T> l(p.dx, p.dxs, r, p.V);
-  T* out = const_cast<T*>(l.row);
-  for (int v = l.v0 + threadIdx.x; v < l.v1; v += NT) reinterpret_cast<raw*>(out - l.pad)[v] = raw{0u, 0u, 0u, 0u};
-  if ((int)threadIdx.x < l.edges) out[l.edge(threadIdx.x)] = (T)0.f;
+DSA_DEV void write_zeros(const Part<T>& part) {
+  T* out = const_cast<T*>(part.l.row);
+  for (int v = part.from + threadIdx.x; v < part.hi; v += NT)
+    if (v >= part.lo) reinterpret_cast<raw*>(out - part.l.pad)[v] = raw{0u, 0u, 0u, 0u};
+  if ((int)threadIdx.x < part.edges) out[part.l.edge(threadIdx.x)] = (T)0.f;
 }
 
-template <typename T, int NT, bool B>
+template <typename T, int NT, bool B, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
   __shared__ int col[kMost + 1];
   __shared__ float term[kMost + 1];
   const int tid = threadIdx.x;
-  const int64_t r = p.row0 + blockIdx.x;
+  const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
+  const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
   const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;
   if (p.ids && id == p.ignore) {
-    write_zeros<T, NT>(p, r);
+    write_zeros<T, NT>(part);
     return;
   }
   const float4 st = p.stats[r];
@@ -663,17 +982,18 @@ __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
   if (B && !(st.w <= -kLowest)) a = __builtin_nanf("");
   d.a = a;
   d.b = -gh * p.inv_t * kLn2 * st.w;
-  write_grad<T, NT, B>(p, r, d, col, term);
+  write_grad<T, NT, B, FAR>(p, r, part, d, col, term);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool FAR>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(VocabRows p) {
   __shared__ int col[kMost];
   __shared__ float term[kMost];
-  const int64_t r = p.row0 + blockIdx.x;
+  const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
+  const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
   const Entries e = entries_of(p, r);
   if (!e.any) {
-    write_zeros<T, NT>(p, r);
+    write_zeros<T, NT>(part);
     return;
   }
   const float4 st = p.stats[r];
@@ -688,7 +1008,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(VocabRows p) {
       if (k < p.K) col[k] = e.id[i] < p.V ? (int)e.id[i] : -1, term[k] = -g * e.q[i];
     }
   }
-  write_grad<T, NT, false>(p, r, d, col, term);
+  write_grad<T, NT, false, FAR>(p, r, part, d, col, term);
 }
 
 }  // namespace voc

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/dsa_vocab.h"
 #include "dsa_host.h"
@@ -15,7 +16,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 1LL << 40;
 constexpr int64_t kMaxV = (1LL << 31) - 128;  // positions of a row and its 16-byte borders are 32-bit
-constexpr int64_t kLaunchRows = 1LL << 22;    // a launch's threads fit 32 bits
+constexpr int64_t kLaunchBlocks = 1LL << 22;  // a launch's threads fit 32 bits
 
 bool elem_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
@@ -38,11 +39,12 @@ int check_sizes(const char* what, int64_t N, int64_t V, int dt) {
 
 bool good_scale(float s) { return s >= 0x1p-100f && s <= 0x1p100f; }
 
-// Launches `launch(row0, rows)` over all rows.
+// Launches `launch(row0, rows)` over all rows, `parts` blocks each.
 template <typename F>
-int by_rows(int64_t N, const char* what, F launch) {
-  for (int64_t r = 0; r < N; r += kLaunchRows) {
-    launch(r, (unsigned)std::min(kLaunchRows, N - r));
+int by_rows(int64_t N, int parts, const char* what, F launch) {
+  const int64_t most = std::max<int64_t>(1, kLaunchBlocks / parts);
+  for (int64_t r = 0; r < N; r += most) {
+    launch(r, (unsigned)std::min(most, N - r));
     if (launch_check(what)) return 1;
   }
   return 0;
@@ -124,39 +126,136 @@ int check_distill(const dsa_distill_args* a, bool bwd) {
   return a->dlogits_stride < a->V && a->N > 1 ? fail("%s: dlogits' rows overlap", what) : 0;
 }
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;   // of a block that has a row
+constexpr int kPart = 256;      // of one that has a part of a row
+constexpr int kPartMost = 2048, kPartLeast = 256;  // 16-byte vectors of a part
+constexpr int kBack = 512;
+constexpr int kBackPer = 2048;
+// Gradients past the caches from here on.  With the two products that read it a
+// step of 160 x 128100 bf16 (41 MB) takes 537 us through the caches and 541 past
+// them, of 512 rows (131 MB) 663 and 655, of 1229 rows 1382 and 1356.
+constexpr uint64_t kFarBytes = 64u << 20;
 
+// How a forward cuts its rows.
+struct Cut {
+  int parts, per, segs;
+  size_t part_bytes, bytes;
+};
+
+// Whether rows go in parts, joined by a second launch.  Few long rows leave most
+// of the card idle by themselves: 1 x 128100 bf16 11.5 us whole, 8.4 in parts (the
+// host's share), 128 rows 12.6 and 11.0, 192 rows 13.4 and 14.1; with the 10 largest
+// 17.0 and 11.4, 128 rows 18.2 and 17.8, 192 rows 19.1 and 20.8; 64000 columns are as
+// fast whole (7.3 and 8.3, 11.9 and 10.6).  And many bytes are read faster where
+// neighbouring blocks read neighbouring lines: the loss of 1229 x 128100 with its
+// gradient 161.6 and 152.2, of 777 x 50021 fp32 80.1 and 76.9 (in between, 512 x
+// 128100 24.0 and 26.6), but not with the largest to find, whose search then has
+// nothing to hide behind: 64 of 2048 rows 106 and 121.
+bool in_parts(int64_t N, int64_t row_bytes, int top) {
+  const int64_t bytes = N * std::min<int64_t>(row_bytes, 1LL << 31);
+  if (row_bytes >= 160 << 10 && bytes < 36 << 20) return true;
+  return !top && bytes >= 128 << 20;
+}
+
+Cut cut_of(int64_t N, int64_t V, int dt, int top) {
+  Cut c{};
+  const int64_t most = V / (dt == DSA_BF16 ? 8 : 4) + 9;  // vectors, wherever a row begins
+  c.segs = (int)(V / voc::kSeg) + 2;
+  c.parts = 1, c.per = kPartMost;
+  if (!in_parts(N, V * elem_bytes(dt), top)) return c;
+  // 128100 bf16 in 63 parts 4.2 us, in 8 parts 5.0
+  while (c.per > kPartLeast && N * cdiv(most, c.per) < 512) c.per /= 2;
+  c.parts = (int)cdiv(most, c.per);
+  if (c.parts == 1) return c;
+  c.part_bytes = (size_t)N * c.parts * sizeof(float4);
+  c.bytes = c.part_bytes + (top ? (size_t)N * c.segs * 4 : 0);
+  return c;
+}
+int take(voc::VocabRows& p, const Cut& c, void* ws, size_t bytes, const char* what) {
+  p.parts = c.parts, p.per = c.per, p.segs = c.segs;
+  if (c.bytes == 0) return 0;
+  if (!ws || bytes < c.bytes || !aligned16(ws)) return fail("%s: the workspace needs %zu bytes, 16-byte aligned", what, c.bytes);
+  p.part = static_cast<float4*>(ws);
+  p.seg = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + c.part_bytes);
+  return 0;
+}
+// backward
 template <typename T>
+void cut_back(voc::VocabRows& p) {
+  p.per = kBackPer;
+  p.parts = (int)cdiv(p.V / voc::Vec<T>::N + 9, p.per);
+}
+
+template <typename T, bool TOP>
 int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
-  if (!p.top)
-    return by_rows(N, "logprobs_fwd_kernel", [&](int64_t r, unsigned rows) {
+  size_t lds = 0;
+  if (TOP) {
+    p.keys = round_up(p.segs, 4);
+    lds = (size_t)(p.keys + voc::kSharedWords) * 4;
+  }
+  if (p.parts == 1)
+    return by_rows(N, 1, "logprobs_fwd_kernel", [&](int64_t r, unsigned rows) {
       p.row0 = r;
-      hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, false>), dim3(rows), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, TOP>), dim3(rows), dim3(kThreads), lds, st, p);
     });
-  const int segs = p.V / voc::kSeg + 2;  // at most, wherever a row begins
-  p.keys = std::max(segs, std::min(p.top, segs) * voc::kSeg);
-  const size_t lds = (size_t)(p.keys + voc::kSharedWords) * 4;
-  return by_rows(N, "logprobs_fwd_kernel", [&](int64_t r, unsigned rows) {
-    p.row0 = r;
-    hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, true>), dim3(rows), dim3(kThreads), lds, st, p);
-  });
+  const size_t part_lds = TOP ? (size_t)p.per * 16 / sizeof(T) / voc::kSeg * 4 : 0;
+  return by_rows(N, p.parts, "logprobs_part_kernel", [&](int64_t r, unsigned rows) {
+           p.row0 = r;
+           hipLaunchKernelGGL((voc::logprobs_part_kernel<T, kPart, TOP>), dim3(rows * p.parts), dim3(kPart), part_lds, st, p);
+         }) ||
+         by_rows(N, 1, "logprobs_join_kernel", [&](int64_t r, unsigned rows) {
+           p.row0 = r;
+           constexpr int NT = TOP ? 256 : 64;
+           hipLaunchKernelGGL((voc::logprobs_join_kernel<T, NT, TOP>), dim3(rows), dim3(NT), lds, st, p);
+         });
+}
+
+// f(FAR): whether a gradient of so many bytes goes past the caches
+template <typename F>
+void by_far(int64_t N, int V, size_t elem, F f) {
+  if ((uint64_t)N * V * elem >= kFarBytes) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 template <typename T>
 int logprobs_bwd(voc::VocabRows p, int64_t N, hipStream_t st) {
-  return by_rows(N, "logprobs_bwd_kernel", [&](int64_t r, unsigned rows) {
+  cut_back<T>(p);
+  return by_rows(N, p.parts, "logprobs_bwd_kernel", [&](int64_t r, unsigned rows) {
     p.row0 = r;
-    if (p.dent) hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kThreads, true>), dim3(rows), dim3(kThreads), 0, st, p);
-    else hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kThreads, false>), dim3(rows), dim3(kThreads), 0, st, p);
+    const dim3 grid(rows * p.parts), block(kBack);
+    by_far(N, p.V, sizeof(T), [&](auto f) {
+      constexpr bool FAR = decltype(f)::value;
+      if (p.dent) hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kBack, true, FAR>), grid, block, 0, st, p);
+      else hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kBack, false, FAR>), grid, block, 0, st, p);
+    });
   });
 }
 
 template <typename T>
-int distill(voc::VocabRows p, int64_t N, bool bwd, hipStream_t st) {
-  return by_rows(N, bwd ? "distill_bwd_kernel" : "distill_fwd_kernel", [&](int64_t r, unsigned rows) {
+int distill_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
+  if (p.parts == 1)
+    return by_rows(N, 1, "distill_fwd_kernel", [&](int64_t r, unsigned rows) {
+      p.row0 = r;
+      hipLaunchKernelGGL((voc::distill_fwd_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, st, p);
+    });
+  return by_rows(N, p.parts, "distill_part_kernel", [&](int64_t r, unsigned rows) {
+           p.row0 = r;
+           hipLaunchKernelGGL((voc::distill_part_kernel<T, kPart>), dim3(rows * p.parts), dim3(kPart), 0, st, p);
+         }) ||
+         by_rows(N, 1, "distill_join_kernel", [&](int64_t r, unsigned rows) {
+           p.row0 = r;
+           hipLaunchKernelGGL((voc::distill_join_kernel<T>), dim3(rows), dim3(64), 0, st, p);
+         });
+}
+
+template <typename T>
+int distill_bwd(voc::VocabRows p, int64_t N, hipStream_t st) {
+  cut_back<T>(p);
+  return by_rows(N, p.parts, "distill_bwd_kernel", [&](int64_t r, unsigned rows) {
     p.row0 = r;
-    if (bwd) hipLaunchKernelGGL((voc::distill_bwd_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, st, p);
-    else hipLaunchKernelGGL((voc::distill_fwd_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, st, p);
+    by_far(N, p.V, sizeof(T), [&](auto f) {
+      hipLaunchKernelGGL((voc::distill_bwd_kernel<T, kBack, decltype(f)::value>), dim3(rows * p.parts), dim3(kBack), 0, st, p);
+    });
   });
 }
 
@@ -164,15 +263,19 @@ int distill(voc::VocabRows p, int64_t N, bool bwd, hipStream_t st) {
 
 extern "C" {
 
-size_t dsa_vocab_workspace_bytes(int64_t, int64_t, int32_t, int32_t) { return 0; }
+size_t dsa_vocab_workspace_bytes(int64_t N, int64_t V, int32_t dtype, int32_t top_k) {
+  return N > 0 && N <= kMaxRows && V > 0 && V <= kMaxV ? cut_of(N, V, dtype, top_k).bytes : 0;
+}
 
 int dsa_logprobs_fwd(const dsa_logprobs_args* a, void* stream) {
   g_err.clear();
   if (check_logprobs(a, false)) return 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (refuse_capture(st, "dsa_logprobs_fwd")) return 1;
-  const voc::VocabRows p = rows_of(a);
-  return a->dtype == DSA_BF16 ? logprobs_fwd<dsa::bf16>(p, a->N, st) : logprobs_fwd<float>(p, a->N, st);
+  voc::VocabRows p = rows_of(a);
+  if (take(p, cut_of(a->N, a->V, a->dtype, a->top_k), a->workspace, a->workspace_bytes, "dsa_logprobs_fwd")) return 1;
+  if (a->top_k) return a->dtype == DSA_BF16 ? logprobs_fwd<dsa::bf16, true>(p, a->N, st) : logprobs_fwd<float, true>(p, a->N, st);
+  return a->dtype == DSA_BF16 ? logprobs_fwd<dsa::bf16, false>(p, a->N, st) : logprobs_fwd<float, false>(p, a->N, st);
 }
 
 int dsa_logprobs_bwd(const dsa_logprobs_args* a, void* stream) {
@@ -189,8 +292,9 @@ int dsa_distill_fwd(const dsa_distill_args* a, void* stream) {
   if (check_distill(a, false)) return 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (refuse_capture(st, "dsa_distill_fwd")) return 1;
-  const voc::VocabRows p = rows_of(a);
-  return a->dtype == DSA_BF16 ? distill<dsa::bf16>(p, a->N, false, st) : distill<float>(p, a->N, false, st);
+  voc::VocabRows p = rows_of(a);
+  if (take(p, cut_of(a->N, a->V, a->dtype, 0), a->workspace, a->workspace_bytes, "dsa_distill_fwd")) return 1;
+  return a->dtype == DSA_BF16 ? distill_fwd<dsa::bf16>(p, a->N, st) : distill_fwd<float>(p, a->N, st);
 }
 
 int dsa_distill_bwd(const dsa_distill_args* a, void* stream) {
@@ -199,7 +303,7 @@ int dsa_distill_bwd(const dsa_distill_args* a, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (refuse_capture(st, "dsa_distill_bwd")) return 1;
   const voc::VocabRows p = rows_of(a);
-  return a->dtype == DSA_BF16 ? distill<dsa::bf16>(p, a->N, true, st) : distill<float>(p, a->N, true, st);
+  return a->dtype == DSA_BF16 ? distill_bwd<dsa::bf16>(p, a->N, st) : distill_bwd<float>(p, a->N, st);
 }
 
 }  // extern "C"

@@ -14,7 +14,7 @@
  * are given, every other tensor is contiguous.  Logits are DSA_F32 or
  * DSA_BF16; arithmetic, sums and results are float32.  Equal inputs give equal
  * bits (no float atomics); the order of a row's sums goes by where it begins
- * between two 16-byte borders and by N and V.
+ * between two 128-byte borders and by N and V.
  *
  * A logit of -inf has probability 0 and adds nothing to sums, entropy or
  * gradients.  A row with a NaN or +inf among its logits, or without a finite
@@ -92,7 +92,8 @@ typedef struct dsa_distill_args {
 } dsa_distill_args;
 
 /* Workspace bytes of a forward on N rows of V values of `dtype`, with the top_k
- * largest (0 for none and for the distillation loss).  May be 0. */
+ * largest (0 for none and for the distillation loss).  May be 0; the calls refuse
+ * a smaller workspace. */
 size_t dsa_vocab_workspace_bytes(int64_t N, int64_t V, int32_t dtype, int32_t top_k);
 
 /* logprobs, entropy, lse, the largest and stats from logits and ids. */
