@@ -864,6 +864,12 @@ DSA_DEV void pack(const float* v, raw& r) {
   }
 }
 
+template <bool FAR>
+DSA_DEV void store(raw* to, raw v) {
+  if (FAR) __builtin_nontemporal_store(v, to);
+  else *to = v;
+}
+
 // A block's part of a row: vectors lo .. hi - 1, and the row's single values with
 // the first part.
 template <typename T>
@@ -907,11 +913,7 @@ DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Part<T>& part, cons
 #pragma unroll
       for (int e = 0; e < N; ++e) x[e] = grad_of<B>(g, exponent(x[e], g.m, p.c));
       pack<T>(x, q[i]);
-      if (v >= part.lo && v < part.hi) {
-        raw* to = reinterpret_cast<raw*>(out - l.pad) + v;
-        if (FAR) __builtin_nontemporal_store(q[i], to);
-        else *to = q[i];
-      }
+      if (v >= part.lo && v < part.hi) store<FAR>(reinterpret_cast<raw*>(out - l.pad) + v, q[i]);
     }
   }
   if (tid < part.edges) {
@@ -934,11 +936,13 @@ DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Part<T>& part, cons
   }
 }
 
-template <typename T, int NT>
+// A row that is left out, past the caches too: the loss of 4096 x 128100 of which 85%
+// are left out 285 us through them, 240 past them.
+template <typename T, int NT, bool FAR>
 DSA_DEV void write_zeros(const Part<T>& part) {
   T* out = const_cast<T*>(part.l.row);
   for (int v = part.from + threadIdx.x; v < part.hi; v += NT)
-    if (v >= part.lo) reinterpret_cast<raw*>(out - part.l.pad)[v] = raw{0u, 0u, 0u, 0u};
+    if (v >= part.lo) store<FAR>(reinterpret_cast<raw*>(out - part.l.pad) + v, raw{0u, 0u, 0u, 0u});
   if ((int)threadIdx.x < part.edges) out[part.l.edge(threadIdx.x)] = (T)0.f;
 }
 
@@ -951,7 +955,7 @@ __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
   const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
   const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;
   if (p.ids && id == p.ignore) {
-    write_zeros<T, NT>(part);
+    write_zeros<T, NT, FAR>(part);
     return;
   }
   const float4 st = p.stats[r];
@@ -993,7 +997,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(VocabRows p) {
   const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
   const Entries e = entries_of(p, r);
   if (!e.any) {
-    write_zeros<T, NT>(part);
+    write_zeros<T, NT, FAR>(part);
     return;
   }
   const float4 st = p.stats[r];
