@@ -545,6 +545,7 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
   }
   __syncthreads();
   const uint32_t found = sh.word[1];
+  __syncthreads();  // what follows writes the word again
   for (int round = 0; round < 2 && found <= kCands; ++round) {
     // the segments' bound may be far below their values', where there are few segments
     if (round == 1 || (segs < 4 * k && found * kSeg > kCands)) {

@@ -134,7 +134,7 @@ constexpr int kBackPer = 2048;
 // Gradients past the caches from here on.  With the two products that read it a
 // step of 160 x 128100 bf16 (41 MB) takes 537 us through the caches and 541 past
 // them, of 512 rows (131 MB) 663 and 655, of 1229 rows 1382 and 1356.
-constexpr uint64_t kFarBytes = 64u << 20;
+constexpr double kFarBytes = 64 << 20;
 
 // How a forward cuts its rows.
 struct Cut {
@@ -152,7 +152,7 @@ struct Cut {
 // 128100 24.0 and 26.6), but not with the largest to find, whose search then has
 // nothing to hide behind: 64 of 2048 rows 106 and 121.
 bool in_parts(int64_t N, int64_t row_bytes, int top) {
-  const int64_t bytes = N * std::min<int64_t>(row_bytes, 1LL << 31);
+  const double bytes = (double)N * (double)row_bytes;
   if (row_bytes >= 160 << 10 && bytes < 36 << 20) return true;
   return !top && bytes >= 128 << 20;
 }
@@ -213,7 +213,7 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
 // f(FAR): whether a gradient of so many bytes goes past the caches
 template <typename F>
 void by_far(int64_t N, int V, size_t elem, F f) {
-  if ((uint64_t)N * V * elem >= kFarBytes) f(std::true_type{});
+  if ((double)N * V * (double)elem >= kFarBytes) f(std::true_type{});
   else f(std::false_type{});
 }
 

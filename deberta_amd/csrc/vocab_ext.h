@@ -56,12 +56,11 @@ struct PerRow {
   }
 };
 
-const float* stats_of(const char* what, const Tensor& stats, int64_t N, const Tensor& logits) {
+Tensor stats_of(const char* what, const Tensor& stats, int64_t N, const Tensor& logits) {
   check_with(what, "stats", stats, logits);
-  TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.dim() == 2 && stats.size(0) == N && stats.size(1) == 4 &&
-                        (reinterpret_cast<uintptr_t>(stats.const_data_ptr()) & 15u) == 0,
-                    what, ": bad stats");
-  return stats.const_data_ptr<float>();
+  TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.dim() == 2 && stats.size(0) == N && stats.size(1) == 4, what,
+                    ": bad stats");
+  return held(what, "stats", stats);
 }
 
 template <typename A>
@@ -124,7 +123,8 @@ Tensor logprobs_grad(const Tensor& dlogprobs, const Tensor& dentropy, const Tens
   dsa_logprobs_args a{};
   a.N = l.N, a.V = l.V, a.dtype = l.dt, a.inv_temperature = (float)(1.0 / temperature), a.ignore_index = ignore;
   const Tensor dx = empty(logits, logits.scalar_type());
-  a.stats = const_cast<float*>(stats_of(what, stats, l.N, logits));
+  const Tensor st = stats_of(what, stats, l.N, logits);
+  a.stats = const_cast<float*>(st.const_data_ptr<float>());
   const PerRow gl(what, "dlogprobs", dlogprobs, logits), ge(what, "dentropy", dentropy, logits), gs(what, "dlse", dlse, logits);
   Tensor idr, tops, gt;
   if (ids.defined()) idr = whole(what, "ids", ids, row_shape(logits), logits), a.ids_bytes = (int32_t)idr.element_size();
@@ -133,7 +133,7 @@ Tensor logprobs_grad(const Tensor& dlogprobs, const Tensor& dentropy, const Tens
     TORCH_CHECK_VALUE(top_ids.defined() && top_ids.dim() == logits.dim() && top_ids.size(-1) <= std::min<int64_t>(l.V, DSA_VOCAB_MAX_ENTRIES), what, ": dtop needs top_ids");
     auto shape = row_shape(logits).vec();
     shape.push_back(top_ids.size(-1));
-    tops = whole(what, "top_ids", top_ids.to(at::kLong), shape, logits);
+    tops = whole(what, "top_ids", held(what, "top_ids", top_ids).to(at::kLong), shape, logits);
     check_with(what, "dtop", dtop, logits);
     TORCH_CHECK_VALUE(dtop.sizes() == tops.sizes() && dtop.scalar_type() == at::kFloat, what, ": dtop must be float32 of shape ", tops.sizes());
     gt = held(what, "dtop", dtop).contiguous();
@@ -275,7 +275,8 @@ Tensor distill_bwd(const Tensor& dloss, const Tensor& logits, const Tensor& teac
   const char* what = "distill_loss_bwd";
   Distill d(what, logits, teacher_ids, teacher_logits, teacher_lse, temperature);
   const PerRow g(what, "dloss", dloss, logits);
-  d.a.stats = const_cast<float*>(stats_of(what, stats, d.l.N, logits));
+  const Tensor st = stats_of(what, stats, d.l.N, logits);
+  d.a.stats = const_cast<float*>(st.const_data_ptr<float>());
   const Tensor dx = empty(logits, logits.scalar_type());
   if (d.l.N == 0) return dx;
   d.a.dloss = g.data, d.a.dloss_stride = g.stride;
@@ -304,6 +305,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
 
 Maybe distill(const Tensor& logits, const Tensor& teacher_ids, const Tensor& teacher_logits, const Maybe& teacher_lse, double temperature) {
   if (!here({&logits, &teacher_ids, &teacher_logits, at_or_null(teacher_lse)})) return std::nullopt;
-  if (!needs_grad({&logits})) return std::get<0>(distill_run(logits, teacher_ids, teacher_logits, teacher_lse, temperature, false));
+  // a teacher's tangent is refused by the node, its gradient before this call
+  if (!needs_grad({&logits, &teacher_logits, at_or_null(teacher_lse)})) return std::get<0>(distill_run(logits, teacher_ids, teacher_logits, teacher_lse, temperature, false));
   return DistillLoss::apply(logits, teacher_ids, teacher_logits, teacher_lse, temperature);
 }

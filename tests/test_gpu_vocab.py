@@ -180,7 +180,7 @@ def test_all_of_a_row(gpu):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=str)
-@pytest.mark.parametrize("V", [300, 20011])
+@pytest.mark.parametrize("V", [300, 20011, 50021, 128100])
 def test_ties_and_orders(V, dtype, gpu):
     """Values in the orders that a selection is worst at: all equal, two values,
     rising, falling, the largest side by side, zeros of both signs, one far out."""
@@ -581,10 +581,6 @@ def test_refusals(gpu):
         d(x, t_ids, teacher, 1.0, torch.zeros(3, device=gpu, dtype=BF))
     with pytest.raises(ValueError, match="no gradient for the teacher"):
         d(x, t_ids, teacher.clone().requires_grad_())
-    freed = _rand(3, 8, seed=1).to(gpu)
-    freed.untyped_storage().resize_(0)
-    with pytest.raises(ValueError, match="no memory"):
-        f(freed, ids)
 
 
 def test_compiled_calls(gpu):

@@ -330,6 +330,24 @@ def test_distill_entry_points_refuse(names, change, match):
         assert re.search(match, _lib.last_error()), _lib.last_error()
 
 
+def test_rows_in_parts_need_their_workspace():
+    """Which the library sizes: for few long rows, for many bytes, and nothing
+    for what one block a row reads."""
+    lib, bytes_of = _lib.load(), _lib.load().dsa_vocab_workspace_bytes
+    assert bytes_of(1, 128100, _lib.DSA_BF16, 0) > 0 and bytes_of(1, 128100, _lib.DSA_BF16, 5) > bytes_of(1, 128100, _lib.DSA_BF16, 0)
+    assert bytes_of(1229, 128100, _lib.DSA_BF16, 0) > 0 and bytes_of(1229, 128100, _lib.DSA_BF16, 64) == 0
+    assert bytes_of(512, 32768, _lib.DSA_BF16, 0) == 0 == bytes_of(0, 128100, _lib.DSA_F32, 0)
+    assert bytes_of(1 << 40, (1 << 31) - 128, _lib.DSA_F32, 0) > 1 << 50  # sizes that pass 64 bits as products
+    a = {**_LOGPROBS, "V": 128100, "logits_stride": 128100, "N": 1}
+    d = {**_DISTILL, "V": 128100, "logits_stride": 128100, "N": 1}
+    need = bytes_of(1, 128100, _lib.DSA_F32, 0)
+    for ws in (dict(), dict(workspace=_AT, workspace_bytes=need - 1), dict(workspace=_AT + 4, workspace_bytes=need)):
+        assert lib.dsa_logprobs_fwd(ctypes.byref(_lib.DsaLogprobsArgs(**a, **ws)), None) != 0
+        assert f"workspace needs {need} bytes" in _lib.last_error()
+        assert lib.dsa_distill_fwd(ctypes.byref(_lib.DsaDistillArgs(**d, **ws)), None) != 0
+        assert "workspace needs" in _lib.last_error()
+
+
 def test_null_arguments_are_errors():
     lib = _lib.load()
     for name in _lib.VOCAB_EXPORTS[1:]:
