@@ -226,13 +226,17 @@ struct Line {
     edges = head + (V - tail0);
   }
   DSA_DEV int edge(int i) const { return i < head ? i : tail0 + (i - head); }
-  DSA_DEV raw load(int v) const { return reinterpret_cast<const raw*>(base)[v]; }
+  template <bool FAR = false>
+  DSA_DEV raw load(int v) const {
+    const raw* at = reinterpret_cast<const raw*>(base) + v;
+    return FAR ? __builtin_nontemporal_load(at) : *at;
+  }
 };
 
 // The sums of a thread over its share of positions from `from` to `to` vectors (a
 // multiple of 64 each, or the row's end); with SEG the keys of the maxima of the
-// `segs` segments from there on, for which the caller waits.
-template <typename T, int NT, bool ENT, bool SEG>
+// `segs` segments from there on, for which the caller waits.  FAR: past the caches.
+template <typename T, int NT, bool ENT, bool SEG, bool FAR>
 DSA_DEV Run stream(const Line<T>& l, int from, int to, float c, uint32_t* keys, int segs) {
   constexpr int N = Vec<T>::N, E = kUnroll * N, L = kSeg / N;
   const int tid = threadIdx.x;
@@ -247,13 +251,13 @@ DSA_DEV Run stream(const Line<T>& l, int from, int to, float c, uint32_t* keys, 
   raw next[kUnroll];
   if (first < end) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) next[i] = l.load(min(max(from + i * NT + tid, first), end - 1));
+    for (int i = 0; i < kUnroll; ++i) next[i] = l.template load<FAR>(min(max(from + i * NT + tid, first), end - 1));
     for (int vb = from; vb < end; vb += NT * kUnroll) {
       raw q[kUnroll];
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) q[i] = next[i];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) next[i] = l.load(min(vb + (i + kUnroll) * NT + tid, end - 1));
+      for (int i = 0; i < kUnroll; ++i) next[i] = l.template load<FAR>(min(vb + (i + kUnroll) * NT + tid, end - 1));
       if (vb < first || vb + NT * kUnroll > end) {
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
@@ -624,7 +628,7 @@ DSA_DEV void write_row(const VocabRows& p, int64_t r, const Run& all, float ln_s
   if (p.stats) p.stats[r] = float4{all.m, ln_s, ent, 1.f / all.s};
 }
 
-template <typename T, int NT, bool TOP>
+template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
   __shared__ float red[3 * (NT / 64)];
@@ -636,7 +640,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   }
   const Line<T> l(p.x, p.xs, r, p.V);
   const float x = given(l, p, id);  // early: its way from memory is long
-  const Run all = block_run<NT, true>(stream<T, NT, true, TOP>(l, 0, kRow, p.c, lds, p.segs), p.c, red);
+  const Run all = block_run<NT, true>(stream<T, NT, true, TOP, FAR>(l, 0, kRow, p.c, lds, p.segs), p.c, red);
   const float ln_s = logf(all.s);
   if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
   if constexpr (TOP) {
@@ -647,13 +651,13 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
 
 // A part of a row by a block, where rows are few or long: its sums, and its
 // segments' maxima, for the row's join.
-template <typename T, int NT, bool ENT, bool SEG>
+template <typename T, int NT, bool ENT, bool SEG, bool FAR>
 DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys, float* red) {
   constexpr int L = kSeg / Vec<T>::N;
   const Line<T> l(p.x, p.xs, r, p.V);
   const int from = part * p.per;
   const int first = from / L, n = min(p.per / L, p.segs - first);  // segments
-  const Run all = block_run<NT, ENT>(stream<T, NT, ENT, SEG>(l, from, from + p.per, p.c, keys, n), p.c, red);
+  const Run all = block_run<NT, ENT>(stream<T, NT, ENT, SEG, FAR>(l, from, from + p.per, p.c, keys, n), p.c, red);
   if (threadIdx.x == 0) p.part[r * p.parts + part] = float4{all.m, all.s, all.u, 0.f};
   if (SEG) {
     __syncthreads();
@@ -661,13 +665,13 @@ DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys,
   }
 }
 
-template <typename T, int NT, bool TOP>
+template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   if (p.ids && load_id(p.ids, p.ids64, r) == p.ignore) return;
-  write_part<T, NT, true, TOP>(p, r, blockIdx.x % (uint32_t)p.parts, lds, red);
+  write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds, red);
 }
 
 // The row's sums out of its parts', in every thread of the block.
@@ -798,7 +802,7 @@ DSA_DEV void write_loss(const VocabRows& p, int64_t r, const Entries& e, const R
   }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool FAR>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x;
@@ -808,18 +812,18 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
     return;
   }
   const Line<T> l(p.x, p.xs, r, p.V);
-  const Run all = block_run<NT, false>(stream<T, NT, false, false>(l, 0, kRow, p.c, nullptr, 0), p.c, red);
+  const Run all = block_run<NT, false>(stream<T, NT, false, false, FAR>(l, 0, kRow, p.c, nullptr, 0), p.c, red);
   if (threadIdx.x < 64) write_loss<T>(p, r, e, all);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool FAR>
 __global__ __launch_bounds__(NT) void distill_part_kernel(VocabRows p) {
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   bool any = false;  // by every wave
   for (int k = threadIdx.x & 63; k < p.K; k += 64) any |= load_id(p.ids, p.ids64, r * p.K + k) >= 0;
   if (__ballot(any) == 0) return;
-  write_part<T, NT, false, false>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr, red);
+  write_part<T, NT, false, false, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr, red);
 }
 
 // A wave a row.  (4096 rows of 128 entries 14 us, each entry's logit a line of its

@@ -135,6 +135,20 @@ constexpr int kBackPer = 2048;
 // step of 160 x 128100 bf16 (41 MB) takes 537 us through the caches and 541 past
 // them, of 512 rows (131 MB) 663 and 655, of 1229 rows 1382 and 1356.
 constexpr double kFarBytes = 64 << 20;
+// Logits that a forward reads past the caches: of the last level's size and more,
+// where no backward reads them again (the 64 largest of 2048 x 128100 bf16 108.3
+// and 105.4 us), and those of a distillation from twice that on (4096 rows with the
+// gradient 582 and 551; 1229 rows, 315 MB, 171 and 168).  Not those of a loss, whose
+// rows may be left out, so that fewer bytes are read again than there are: 1229
+// rows 152 and 164, 4096 of which 85% are left out 240 and 292.
+constexpr double kFarLogits = 256 << 20;
+
+template <typename F>
+void by_bool(bool b, F f) {
+  if (b) f(std::true_type{});
+  else f(std::false_type{});
+}
+double bytes_of(int64_t N, int64_t V, size_t elem) { return (double)N * (double)V * (double)elem; }
 
 // How a forward cuts its rows.
 struct Cut {
@@ -152,7 +166,7 @@ struct Cut {
 // 128100 24.0 and 26.6), but not with the largest to find, whose search then has
 // nothing to hide behind: 64 of 2048 rows 106 and 121.
 bool in_parts(int64_t N, int64_t row_bytes, int top) {
-  const double bytes = (double)N * (double)row_bytes;
+  const double bytes = bytes_of(N, row_bytes, 1);
   if (row_bytes >= 160 << 10 && bytes < 36 << 20) return true;
   return !top && bytes >= 128 << 20;
 }
@@ -193,15 +207,21 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
     p.keys = round_up(p.segs, 4);
     lds = (size_t)(p.keys + voc::kSharedWords) * 4;
   }
+  const bool far = !p.stats && bytes_of(N, p.V, sizeof(T)) >= kFarLogits;
   if (p.parts == 1)
     return by_rows(N, 1, "logprobs_fwd_kernel", [&](int64_t r, unsigned rows) {
       p.row0 = r;
-      hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, TOP>), dim3(rows), dim3(kThreads), lds, st, p);
+      by_bool(far, [&](auto f) {
+        hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, TOP, decltype(f)::value>), dim3(rows), dim3(kThreads), lds, st, p);
+      });
     });
   const size_t part_lds = TOP ? (size_t)p.per * 16 / sizeof(T) / voc::kSeg * 4 : 0;
   return by_rows(N, p.parts, "logprobs_part_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
-           hipLaunchKernelGGL((voc::logprobs_part_kernel<T, kPart, TOP>), dim3(rows * p.parts), dim3(kPart), part_lds, st, p);
+           by_bool(far, [&](auto f) {
+             constexpr bool FAR = !TOP && decltype(f)::value;  // with the largest, parts are for few bytes
+             hipLaunchKernelGGL((voc::logprobs_part_kernel<T, kPart, TOP, FAR>), dim3(rows * p.parts), dim3(kPart), part_lds, st, p);
+           });
          }) ||
          by_rows(N, 1, "logprobs_join_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
@@ -210,20 +230,13 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
          });
 }
 
-// f(FAR): whether a gradient of so many bytes goes past the caches
-template <typename F>
-void by_far(int64_t N, int V, size_t elem, F f) {
-  if ((double)N * V * (double)elem >= kFarBytes) f(std::true_type{});
-  else f(std::false_type{});
-}
-
 template <typename T>
 int logprobs_bwd(voc::VocabRows p, int64_t N, hipStream_t st) {
   cut_back<T>(p);
   return by_rows(N, p.parts, "logprobs_bwd_kernel", [&](int64_t r, unsigned rows) {
     p.row0 = r;
     const dim3 grid(rows * p.parts), block(kBack);
-    by_far(N, p.V, sizeof(T), [&](auto f) {
+    by_bool(bytes_of(N, p.V, sizeof(T)) >= kFarBytes, [&](auto f) {
       constexpr bool FAR = decltype(f)::value;
       if (p.dent) hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kBack, true, FAR>), grid, block, 0, st, p);
       else hipLaunchKernelGGL((voc::logprobs_bwd_kernel<T, kBack, false, FAR>), grid, block, 0, st, p);
@@ -233,14 +246,19 @@ int logprobs_bwd(voc::VocabRows p, int64_t N, hipStream_t st) {
 
 template <typename T>
 int distill_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
+  const bool far = bytes_of(N, p.V, sizeof(T)) >= (p.stats ? 2 * kFarLogits : kFarLogits);
   if (p.parts == 1)
     return by_rows(N, 1, "distill_fwd_kernel", [&](int64_t r, unsigned rows) {
       p.row0 = r;
-      hipLaunchKernelGGL((voc::distill_fwd_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, st, p);
+      by_bool(far, [&](auto f) {
+        hipLaunchKernelGGL((voc::distill_fwd_kernel<T, kThreads, decltype(f)::value>), dim3(rows), dim3(kThreads), 0, st, p);
+      });
     });
   return by_rows(N, p.parts, "distill_part_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
-           hipLaunchKernelGGL((voc::distill_part_kernel<T, kPart>), dim3(rows * p.parts), dim3(kPart), 0, st, p);
+           by_bool(far, [&](auto f) {
+             hipLaunchKernelGGL((voc::distill_part_kernel<T, kPart, decltype(f)::value>), dim3(rows * p.parts), dim3(kPart), 0, st, p);
+           });
          }) ||
          by_rows(N, 1, "distill_join_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
@@ -253,7 +271,7 @@ int distill_bwd(voc::VocabRows p, int64_t N, hipStream_t st) {
   cut_back<T>(p);
   return by_rows(N, p.parts, "distill_bwd_kernel", [&](int64_t r, unsigned rows) {
     p.row0 = r;
-    by_far(N, p.V, sizeof(T), [&](auto f) {
+    by_bool(bytes_of(N, p.V, sizeof(T)) >= kFarBytes, [&](auto f) {
       hipLaunchKernelGGL((voc::distill_bwd_kernel<T, kBack, decltype(f)::value>), dim3(rows * p.parts), dim3(kBack), 0, st, p);
     });
   });
