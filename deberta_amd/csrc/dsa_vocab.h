@@ -37,6 +37,7 @@ constexpr int kSeg = 64;      // columns of a segment
 constexpr int kBins = 1024;   // of a selection's histogram
 constexpr int kMost = 128;    // entries of a row
 constexpr int kRow = 1 << 30;  // vectors: as many as a row has
+constexpr int kPartWaves = 4;  // of a block that has a part of a row
 constexpr int kUnroll = 4;    // 16-byte loads in flight a lane
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -54,7 +55,7 @@ struct VocabRows {
   int V, top, K, ids64, teacher_bf16;
   int keys;        // LDS words for a selection's keys
   int parts, per;  // blocks a row, 16-byte vectors a block
-  float4* part;    // [N, parts]: m, s, u of a part
+  float4* part;    // [N, parts, kPartWaves]: m, s, u of a wave's share
   uint32_t* seg;   // [N, segs]: the segments' maxima
   int segs;
   float inv_t, t;
@@ -171,18 +172,25 @@ DSA_DEV void add(Run& r, const float* x, float most, float c) {
 }
 
 DSA_DEV float wave_max_f(float x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = max2(x, __shfl_xor(x, o));
-  return x;
+  x = max2(x, hid::dpp<0xB1>(x));
+  x = max2(x, hid::dpp<0x4E>(x));
+  x = max2(x, hid::dpp<0x141>(x));
+  x = max2(x, hid::dpp<0x140>(x));  // of 16 lanes
+  return max2(max3(hid::lane_value(x, 0), hid::lane_value(x, 16), hid::lane_value(x, 32)), hid::lane_value(x, 48));
+}
+// The wave's sums out of its lanes', in every lane.
+template <bool ENT>
+DSA_DEV Run wave_run(Run r, float c) {
+  raise<ENT>(r, wave_max_f(r.m), c);
+  r.s = hid::lanes_sum<64>(r.s);
+  if (ENT) r.u = hid::lanes_sum<64>(r.u);
+  return r;
 }
 // The block's sums out of its threads', in every thread; red: 3 words a wave.
 template <int NT, bool ENT>
 DSA_DEV Run block_run(Run r, float c, float* red) {
   constexpr int W = NT / 64;
-  const float m = wave_max_f(r.m);
-  raise<ENT>(r, m, c);
-  r.s = hid::lanes_sum<64>(r.s);
-  if (ENT) r.u = hid::lanes_sum<64>(r.u);
+  r = wave_run<ENT>(r, c);
   if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) {
       float* w = red + 3 * (threadIdx.x >> 6);
@@ -649,16 +657,17 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   }
 }
 
-// A part of a row by a block, where rows are few or long: its sums, and its
+// A part of a row by a block, where rows are few or long: its waves' sums, and its
 // segments' maxima, for the row's join.
 template <typename T, int NT, bool ENT, bool SEG, bool FAR>
-DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys, float* red) {
+DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys) {
   constexpr int L = kSeg / Vec<T>::N;
   const Line<T> l(p.x, p.xs, r, p.V);
   const int from = part * p.per;
   const int first = from / L, n = min(p.per / L, p.segs - first);  // segments
-  const Run all = block_run<NT, ENT>(stream<T, NT, ENT, SEG, FAR>(l, from, from + p.per, p.c, keys, n), p.c, red);
-  if (threadIdx.x == 0) p.part[r * p.parts + part] = float4{all.m, all.s, all.u, 0.f};
+  const Run w = wave_run<ENT>(stream<T, NT, ENT, SEG, FAR>(l, from, from + p.per, p.c, keys, n), p.c);
+  if ((threadIdx.x & 63) == 0)
+    p.part[(r * p.parts + part) * (NT / 64) + threadIdx.x / 64] = float4{w.m, w.s, w.u, 0.f};
   if (SEG) {
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += NT) p.seg[r * p.segs + first + i] = keys[i];
@@ -668,18 +677,18 @@ DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys,
 template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
-  __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   if (p.ids && load_id(p.ids, p.ids64, r) == p.ignore) return;
-  write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds, red);
+  write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds);
 }
 
 // The row's sums out of its parts', in every thread of the block.
 template <int NT, bool ENT>
 DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float* red) {
   Run all = run_none();
-  for (int i = threadIdx.x; i < p.parts; i += NT) {
-    const float4 q = p.part[r * p.parts + i];
+  const int n = p.parts * kPartWaves;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float4 q = p.part[r * n + i];
     Run w{q.x, q.y, q.z};
     const float m = max2(all.m, w.m);
     raise<ENT>(all, m, p.c);
@@ -818,12 +827,11 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(VocabRows p) {
 
 template <typename T, int NT, bool FAR>
 __global__ __launch_bounds__(NT) void distill_part_kernel(VocabRows p) {
-  __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   bool any = false;  // by every wave
   for (int k = threadIdx.x & 63; k < p.K; k += 64) any |= load_id(p.ids, p.ids64, r * p.K + k) >= 0;
   if (__ballot(any) == 0) return;
-  write_part<T, NT, false, false, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr, red);
+  write_part<T, NT, false, false, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr);
 }
 
 // A wave a row.  (4096 rows of 128 entries 14 us, each entry's logit a line of its

@@ -127,7 +127,7 @@ int check_distill(const dsa_distill_args* a, bool bwd) {
 }
 
 constexpr int kThreads = 512;   // of a block that has a row
-constexpr int kPart = 256;      // of one that has a part of a row
+constexpr int kPart = 64 * voc::kPartWaves;  // of one that has a part of a row
 constexpr int kPartMost = 2048, kPartLeast = 256;  // 16-byte vectors of a part
 constexpr int kBack = 512;
 constexpr int kBackPer = 2048;
@@ -181,7 +181,7 @@ Cut cut_of(int64_t N, int64_t V, int dt, int top) {
   while (c.per > kPartLeast && N * cdiv(most, c.per) < 512) c.per /= 2;
   c.parts = (int)cdiv(most, c.per);
   if (c.parts == 1) return c;
-  c.part_bytes = (size_t)N * c.parts * sizeof(float4);
+  c.part_bytes = (size_t)N * c.parts * voc::kPartWaves * sizeof(float4);
   c.bytes = c.part_bytes + (top ? (size_t)N * c.segs * 4 : 0);
   return c;
 }
