@@ -115,6 +115,25 @@ DSA_DEV float max_of(const float* v) {
   return m;
 }
 
+// The maxima of four numbers over each L = 8 or 16 neighbouring lanes, one
+// instruction a step and number.  A step reads what the last but three wrote: the
+// two wait states between a vector instruction and another that reads its register
+// across lanes; two more for what was written before.
+template <int L>
+DSA_DEV void max_of_lanes(float (&v)[4]) {
+  static_assert(L == 8 || L == 16, "");
+#define DSA_STEP(how)                                                \
+  "v_max_f32_dpp %0, %0, %0 " how " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_max_f32_dpp %1, %1, %1 " how " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_max_f32_dpp %2, %2, %2 " how " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_max_f32_dpp %3, %3, %3 " how " row_mask:0xf bank_mask:0xf\n\t"
+  asm("s_nop 1\n\t" DSA_STEP("quad_perm:[1,0,3,2]") DSA_STEP("quad_perm:[2,3,0,1]") DSA_STEP("row_half_mirror")
+      : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+  if (L == 16)
+    asm("s_nop 1\n\t" DSA_STEP("row_mirror") : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+#undef DSA_STEP
+}
+
 DSA_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Whole numbers that order as the values do (NaN as -inf, -0 as +0), above 0.
@@ -281,15 +300,12 @@ DSA_DEV Run stream(const Line<T>& l, int from, int to, float c, uint32_t* keys, 
       }
       add<E, ENT>(r, x, max_of<kUnroll>(most), c);
       if (SEG) {
+        max_of_lanes<L>(most);
+        if (tid % L == 0) {
+          uint32_t* to = keys + (vb - from + tid) / L;
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-          float g = most[i];  // over the L lanes of the segment
-          g = max2(g, hid::dpp<0xB1>(g));
-          g = max2(g, hid::dpp<0x4E>(g));
-          g = max2(g, hid::dpp<0x141>(g));
-          if (N == 4) g = max2(g, hid::dpp<0x140>(g));
-          const int v = vb + i * NT + tid;
-          if (tid % L == 0 && v < end) keys[(v - from) / L] = __builtin_bit_cast(uint32_t, g);
+          for (int i = 0; i < kUnroll; ++i)
+            if (vb + i * NT + tid < end) to[i * (NT / L)] = __builtin_bit_cast(uint32_t, most[i]);
         }
       }
     }
