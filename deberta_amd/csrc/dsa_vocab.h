@@ -15,15 +15,28 @@
 // value (a mask that leaves nothing) would overflow; so it has p = 1 / V.  (One
 // fused product from a rounded origin, with this form beside it for such rows, and
 // the entropy's guard against 0 times -inf taken out of the loop: a fifth fewer
-// instructions, and no faster: 67 to 104 registers a lane cost what they saved.)
+// instructions and no faster, 58 to 94 registers a lane cost what they saved.)
 //
 // The k largest come out of the same pass.  It keeps the maximum of each
-// segment of 64 columns.  The k segments whose maxima are largest (equal ones:
-// the first) hold the k largest values: each of these k maxima is one of them
-// or below them, so a value outside these segments, at most its own segment's
-// maximum, has k larger ones before it.  Only those are read again (k 128-byte
-// lines of bf16), and the k largest of them are chosen.  Nothing depends on
-// the data but which lines these are.
+// segment of 64 columns.  A number that the maxima of k segments reach is reached
+// by k values at least, so the k largest lie in the segments that reach it and
+// are among their values that do: about as many lines of the row as there are
+// values to find are read again, and the ranks of what reaches the bound are counted
+// (write_top).  Where thousands of values are equal the k segments whose maxima
+// are largest (equal ones: the first) are selected exactly, and of their values the
+// k largest (top_of_segments): a value outside of them, at most its own segment's
+// maximum, has k larger ones before it.
+//
+// HBM bounds it where there are many rows; of 128100 bf16 columns, us and TB/s of
+// what has to move (a read reaches 6.3 here, a fill 6.9, a copy 5.0):
+//   forward   1229 rows in parts 56.6 + 5.0 to join (315 MB, 5.1), 4096 rows of a
+//             distillation 159 + 17 (1.05 GB, 6.0); 64 largest of 2048 rows, whole, 112 in a
+//             trace and 99 to 101 a pass (525 MB, 5.2)
+//   backward  1229 rows 94.7 (630 MB, 6.6, in part from the last-level cache), 4096 rows
+//             of a distillation 383 (2.10 GB, 5.5), of a loss with 85% of the rows left
+//             out 197 (1.21 GB, 6.1)
+// With few rows it is the chain of a launch, a part's batch, a join and its reads: one
+// row 3.8 + 6.3 us with its 5 largest, 17 by one block.
 #pragma once
 
 #include <type_traits>

@@ -14,7 +14,7 @@ namespace voc = dsa::voc;
 
 namespace {
 
-constexpr int64_t kMaxRows = 1LL << 40;
+constexpr int64_t kMaxRows = 1LL << 36;  // a workspace of them in parts is below 2^61 bytes
 constexpr int64_t kMaxV = (1LL << 31) - 128;  // positions of a row and its 16-byte borders are 32-bit
 constexpr int64_t kLaunchBlocks = 1LL << 22;  // a launch's threads fit 32 bits
 
@@ -32,7 +32,7 @@ int check_rows(const char* what, const char* name, const void* p, int64_t stride
 
 int check_sizes(const char* what, int64_t N, int64_t V, int dt) {
   if (!dtype_ok(dt)) return fail("%s: unknown dtype %d", what, dt);
-  if (N < 0 || N > kMaxRows) return fail("%s: N must be in [0, 2^40], got %lld", what, (long long)N);
+  if (N < 0 || N > kMaxRows) return fail("%s: N must be in [0, 2^36], got %lld", what, (long long)N);
   if (V < 1 || V > kMaxV) return fail("%s: V must be in [1, 2^31 - 128], got %lld", what, (long long)V);
   return 0;
 }

@@ -10,7 +10,7 @@
  *
  * Conventions are those of dsa.h: the caller owns every buffer, work goes on
  * the caller's stream, a nonzero return carries a message in dsa_last_error().
- * Rows hold V contiguous values; the logits' and the gradient's row strides
+ * Rows (2^36 at most) hold V contiguous values; the logits' and the gradient's row strides
  * are given, every other tensor is contiguous.  Logits are DSA_F32 or
  * DSA_BF16; arithmetic, sums and results are float32.  Equal inputs give equal
  * bits (no float atomics); the order of a row's sums goes by where it begins

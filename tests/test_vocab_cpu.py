@@ -291,7 +291,7 @@ _DISTILL = dict(logits=_AT, logits_stride=8, teacher_ids=_AT, ids_bytes=8, teach
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(dtype=2), "dtype"), (dict(N=-1), "N must"), (dict(V=0), "V must"), (dict(V=1 << 31), "V must"),
+    (dict(dtype=2), "dtype"), (dict(N=-1), "N must"), (dict(N=(1 << 36) + 1), "N must"), (dict(V=0), "V must"), (dict(V=1 << 31), "V must"),
     (dict(inv_temperature=0.0), "inv_temperature"), (dict(inv_temperature=NAN), "inv_temperature"), (dict(inv_temperature=INF), "inv_temperature"),
     (dict(top_k=9), "top_k"), (dict(top_k=-1), "top_k"), (dict(top_k=1, V=(1 << 19) + 1, logits_stride=1 << 20, dlogits_stride=1 << 20), "at most"),
     (dict(ids_bytes=2), "ids_bytes"), (dict(logits=None), "logits are required"), (dict(logits=_AT + 2), "aligned"),
@@ -337,7 +337,8 @@ def test_rows_in_parts_need_their_workspace():
     assert bytes_of(1, 128100, _lib.DSA_BF16, 0) > 0 and bytes_of(1, 128100, _lib.DSA_BF16, 5) > bytes_of(1, 128100, _lib.DSA_BF16, 0)
     assert bytes_of(1229, 128100, _lib.DSA_BF16, 0) > 0 and bytes_of(1229, 128100, _lib.DSA_BF16, 64) == 0
     assert bytes_of(512, 32768, _lib.DSA_BF16, 0) == 0 == bytes_of(0, 128100, _lib.DSA_F32, 0)
-    assert bytes_of(1 << 40, (1 << 31) - 128, _lib.DSA_F32, 0) > 1 << 50  # sizes that pass 64 bits as products
+    # the most rows of the most columns: no product of theirs passes 64 bits
+    assert 1 << 59 < bytes_of(1 << 36, (1 << 31) - 128, _lib.DSA_F32, 0) < 1 << 61
     a = {**_LOGPROBS, "V": 128100, "logits_stride": 128100, "N": 1}
     d = {**_DISTILL, "V": 128100, "logits_stride": 128100, "N": 1}
     need = bytes_of(1, 128100, _lib.DSA_F32, 0)
