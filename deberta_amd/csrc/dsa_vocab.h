@@ -106,9 +106,9 @@ DSA_DEV raw raw_none() {
   return raw{w, w, w, w};
 }
 
-// The larger of two or three, a NaN giving way.  The instruction by itself:
-// fmaxf of values that come from memory quiets each one first, an instruction
-// a value.
+// The larger of two or three, a NaN giving way (a signalling one where
+// nan_gives_way has run).  The instruction by itself: fmaxf of values that come
+// from memory quiets each one first, an instruction a value.
 DSA_DEV float max2(float a, float b) {
   float r;
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
@@ -118,6 +118,13 @@ DSA_DEV float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+// Takes the wave out of IEEE mode (bit 9 of the mode register), in which the maximum
+// of a number and a signalling NaN is a NaN: it would hide the values beside it from
+// a row's largest.  Before the wave's first load, which stays behind it.
+DSA_DEV void nan_gives_way() {
+  __builtin_amdgcn_s_setreg(1 | 9 << 6, 0);
+  asm volatile("" ::: "memory");
 }
 template <int N>
 DSA_DEV float max_of(const float* v) {
@@ -668,6 +675,7 @@ DSA_DEV void write_row(const VocabRows& p, int64_t r, const Run& all, float ln_s
 template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
+  if (TOP) nan_gives_way();
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x;
   const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;
@@ -706,6 +714,7 @@ DSA_DEV void write_part(const VocabRows& p, int64_t r, int part, uint32_t* keys)
 template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
+  if (TOP) nan_gives_way();
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   if (p.ids && load_id(p.ids, p.ids64, r) == p.ignore) return;
   write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds);
@@ -730,6 +739,7 @@ DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float* red) {
 template <typename T, int NT, bool TOP>
 __global__ __launch_bounds__(NT) void logprobs_join_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
+  if (TOP) nan_gives_way();
   __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x;
   const int64_t id = p.ids ? load_id(p.ids, p.ids64, r) : 0;

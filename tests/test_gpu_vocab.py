@@ -236,6 +236,38 @@ def test_masked_columns_and_rows(dtype, gpu):
     assert abs(o.entropy.item() - want) <= 200 * U * 8 and abs(o.logprobs.item() + want) <= 230 * U
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+def test_signalling_nan_among_the_largest(dtype, gpu):
+    """A NaN counts as -inf among the largest whichever its bits are, and hides no
+    value beside it: quiet and signalling ones at the row's single values, in its
+    vectors and in its segments, in whole rows and in rows in parts."""
+    bits = {BF: (torch.int16, 0x7F81, -0x7F), FP: (torch.int32, 0x7F800001, -0x7FFFFF)}[dtype]
+    for V, k in ((9, 9), (13, 1), (70, 5), (777, 20), (3001, 128), (90001, 7)):
+        _say("signalling", dtype, V, k)
+        g = torch.Generator().manual_seed(V)
+        x = torch.randperm(4 * V, generator=g).view(4, V)
+        x = (x % 256 - 128).to(dtype) if dtype == BF else (x - 2 * V).to(dtype)
+        order = torch.rand(4, V, generator=g)
+        raw = x.view(bits[0]).clone()
+        few = order < 0.02
+        few[0] = order[0] < 0.5
+        few[1, :3] = few[1, -3:] = True  # beside the row's borders
+        few[2] = False
+        few[2, V // 2] = few[0, 1] = few[3, V - 2] = True
+        raw[few] = bits[1]
+        raw[3, order[3] < 0.1] = bits[2]  # with the sign
+        x = raw.view(dtype)
+        assert x.isnan().sum() == (raw == bits[1]).sum() + (raw == bits[2]).sum()
+        clean = torch.where(x.isnan(), -INF, x.float())
+        want = torch.sort(clean, dim=-1, descending=True, stable=True).indices[..., :k]
+        for first in (0, 1, 3):  # where a row begins between two borders
+            wide = torch.zeros(4, V + 5, dtype=bits[0])
+            wide[:, first : first + V] = raw
+            o = da.fused_token_logprobs(wide.to(gpu).view(dtype)[:, first : first + V], top_k=k)
+            assert torch.equal(o.top_ids.cpu(), want), (V, k, first)
+            assert o.top_logprobs.isnan().all() and o.logsumexp.isnan().all() and o.entropy.isnan().all()
+
+
 def test_large_values_keep_their_differences(gpu):
     """Rows moved by a constant: their own rounding, not that of the constant's
     product with 1 / T (which is 2^-8 here), is what is left."""
