@@ -845,7 +845,7 @@ DSA_DEV void write_loss(const VocabRows& p, int64_t r, const Entries& e, const R
   }
   sum = hid::lanes_sum<64>(sum);
   if (threadIdx.x == 0) {
-    p.loss[r] = e.bad ? __builtin_nanf("") : p.t * p.t * sum;
+    p.loss[r] = e.bad ? __builtin_nanf("") : p.t * (p.t * sum);  // T^2 may be no float32's
     if (p.stats) p.stats[r] = float4{all.m, ln_s, 0.f, 1.f / all.s};
   }
 }

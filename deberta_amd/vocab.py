@@ -332,7 +332,7 @@ def _cpu_distillation(
     q = log_q.exp()
     z, _ = _cpu_scaled(logits, ~given.any(-1), temperature)
     log_p = torch.log_softmax(z, -1).gather(-1, ids.clamp(min=0))
-    return temperature * temperature * torch.where(q == 0, 0.0, q * (log_q - log_p)).sum(-1)
+    return temperature * (temperature * torch.where(q == 0, 0.0, q * (log_q - log_p)).sum(-1))
 
 
 def fused_distillation_loss(
@@ -358,6 +358,7 @@ def fused_distillation_loss(
     the student's is; a row without entries is not read, its loss and gradient are
     0.  An id that occurs twice counts twice.  An id of V or more makes the row's
     loss NaN, and its gradient unless the loss' is 0 (on CPU tensors it raises).
+    The loss' rounding is T^2 times that of the sum, which a large T brings near 0.
     The gradient is the student's alone: a teacher that needs one raises."""
     t = _check_temperature("fused_distillation_loss", temperature)
     if torch.is_grad_enabled() and (teacher_logits.requires_grad or (teacher_lse is not None and teacher_lse.requires_grad)):

@@ -455,6 +455,28 @@ def test_distill_one_token_many_times(gpu):
     _check_distill(x, torch.full((3, 128), 77), _rand(3, 128, seed=2))
 
 
+def test_distill_extreme_temperatures(gpu):
+    """T^2 past float32 on either side.  One entry, so q = 1: the loss is
+    T^2 (-log p), at a small T T (max - x), at a large one T^2 log V; a product
+    with rounded log2(e) / T and ln 2, two with T, and a sum of V terms."""
+    x = _rand(4, 101, seed=1)
+    ids = x.argmin(-1, keepdim=True)
+    zero = torch.zeros(4, 1)
+    for T in (2.0**-100, 2.0**-70):
+        loss = da.fused_distillation_loss(x.to(gpu), ids.to(gpu), zero.to(gpu), T).cpu().double()
+        want = T * (x.double().amax(-1) - x.double().amin(-1))
+        assert ((loss - want).abs() <= 8 * U * want).all(), T
+    T = 2.0**60
+    loss = da.fused_distillation_loss(x.to(gpu), ids.to(gpu), zero.to(gpu), T).cpu().double()
+    want = T * T * torch.tensor(101.0, dtype=torch.float64).log()
+    assert ((loss - want).abs() <= 230 * U * want).all()
+    for T in (2.0**-100, 2.0**100):  # a vocabulary of one: no loss
+        y = x[:, :1].to(gpu).requires_grad_()
+        loss = da.fused_distillation_loss(y, torch.zeros(4, 1, dtype=torch.int64, device=gpu), zero.to(gpu), T)
+        (d,) = torch.autograd.grad(loss.sum(), y)
+        assert (loss == 0).all() and (d == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [BF, FP], ids=str)
 def test_distill_masks(dtype, gpu):
     V, lowest = 333, torch.finfo(dtype).min

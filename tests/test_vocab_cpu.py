@@ -147,6 +147,16 @@ def test_cpu_distillation(T):
     assert da.fused_distillation_loss(x, ids, teacher, T)[0] == INF
 
 
+def test_cpu_distillation_at_extreme_temperatures():
+    """T^2 past float32 on either side: T (max - x), and no loss over one token."""
+    x, zero = _rand(4, 101), torch.zeros(4, 1)
+    want = 2.0**-100 * (x.double().amax(-1) - x.double().amin(-1))
+    got = da.fused_distillation_loss(x, x.argmin(-1, keepdim=True), zero, 2.0**-100).double()
+    assert ((got - want).abs() <= 8 * 2.0**-24 * want).all()
+    for T in (2.0**-100, 2.0**100):
+        assert (da.fused_distillation_loss(x[:, :1], zero[:, :1].long(), zero, T) == 0).all()
+
+
 @pytest.mark.parametrize("shape", [(0, 9), (2, 0, 9)], ids=str)
 def test_cpu_no_rows(shape):
     x = torch.zeros(shape)
@@ -282,6 +292,12 @@ def test_header_matches_the_exports_and_structs(tmp_path):
             assert int(out[f"{c}.{f}"]) == getattr(s, f).offset, (c, f)
 
 
+def _what_changes(v):
+    """A case's name: the fields that it changes, without addresses, which differ
+    from process to process."""
+    return ",".join(v) if isinstance(v, dict) else str(v)
+
+
 _KEEP = ctypes.create_string_buffer(4096)
 _AT = (ctypes.addressof(_KEEP) + 255) // 256 * 256
 _LOGPROBS = dict(logits=_AT, logits_stride=8, ids=_AT, ids_bytes=8, logprobs=_AT, entropy=_AT, lse=_AT, stats=_AT, N=2, V=8, dtype=0,
@@ -296,7 +312,7 @@ _DISTILL = dict(logits=_AT, logits_stride=8, teacher_ids=_AT, ids_bytes=8, teach
     (dict(top_k=9), "top_k"), (dict(top_k=-1), "top_k"), (dict(top_k=1, V=(1 << 19) + 1, logits_stride=1 << 20, dlogits_stride=1 << 20), "at most"),
     (dict(ids_bytes=2), "ids_bytes"), (dict(logits=None), "logits are required"), (dict(logits=_AT + 2), "aligned"),
     (dict(logits_stride=-8), "stride"), (dict(ids=_AT + 4), "aligned"), (dict(stats=_AT + 4), "16-byte"),
-], ids=str)
+], ids=_what_changes)
 def test_logprobs_entry_points_refuse(change, match):
     lib = _lib.load()
     for name in ("dsa_logprobs_fwd", "dsa_logprobs_bwd"):
@@ -310,7 +326,7 @@ def test_logprobs_entry_points_refuse(change, match):
     ("dsa_logprobs_bwd", dict(ids=None), "need ids"), ("dsa_logprobs_bwd", dict(dtop=_AT), "top_k and top_ids"),
     ("dsa_logprobs_bwd", dict(dlogprobs_stride=2), "strides"), ("dsa_logprobs_bwd", dict(dlogits=None), "dlogits are required"),
     ("dsa_logprobs_bwd", dict(dlogits_stride=7), "overlap"), ("dsa_logprobs_bwd", dict(dlogits=_AT + 1), "aligned"),
-], ids=str)
+], ids=_what_changes)
 def test_logprobs_entry_points_refuse_what_one_needs(name, change, match):
     assert getattr(_lib.load(), name)(ctypes.byref(_lib.DsaLogprobsArgs(**{**_LOGPROBS, **change})), None) != 0
     assert re.search(match, _lib.last_error()), _lib.last_error()
@@ -323,7 +339,7 @@ def test_logprobs_entry_points_refuse_what_one_needs(name, change, match):
     ("both", dict(logits=None), "logits are required"), ("both", dict(stats=_AT + 8), "16-byte"), ("dsa_distill_fwd", dict(loss=None), "loss"),
     ("dsa_distill_bwd", dict(stats=None), "stats and dloss"), ("dsa_distill_bwd", dict(dloss=None), "stats and dloss"),
     ("dsa_distill_bwd", dict(dloss_stride=3), "stride"), ("dsa_distill_bwd", dict(dlogits_stride=4), "overlap"),
-], ids=str)
+], ids=_what_changes)
 def test_distill_entry_points_refuse(names, change, match):
     for name in ("dsa_distill_fwd", "dsa_distill_bwd") if names == "both" else (names,):
         assert getattr(_lib.load(), name)(ctypes.byref(_lib.DsaDistillArgs(**{**_DISTILL, **change})), None) != 0
