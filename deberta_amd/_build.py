@@ -144,12 +144,12 @@ def build(verbose: bool = False) -> Path:
     consistent image.
 
     Where torch's or Python's C++ headers are not installed the kernels are
-    built alone, with a warning: the operators on hidden states then raise on
-    device tensors, everything else runs.
+    built alone, with a warning: the operators on hidden states and logits then
+    raise on device tensors, everything else runs.
     """
     missing = _missing_headers()
     if missing:
-        warnings.warn(f"{EXT_PATH.name} is not built, {', '.join(missing)} not found: the operators on hidden states will not run")
+        warnings.warn(f"{EXT_PATH.name} is not built, {', '.join(missing)} not found: the operators on hidden states and logits will not run")
         EXT_PATH.unlink(missing_ok=True)  # not to be taken for this build's
         _compile(PROBE_SOURCES, PROBE_PATH, verbose)
         return _compile(SOURCES, LIB_PATH, verbose)

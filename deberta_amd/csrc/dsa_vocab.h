@@ -467,9 +467,24 @@ DSA_DEV void choose(const Shared& sh, int n, int need, F key) {
   __syncthreads();
 }
 
+// The k-th largest of 64 G numbers, G a lane, cut to its upper 16 bits, by one
+// wave: a bit at a time, by counting the numbers that reach it.
+template <int G>
+DSA_DEV uint32_t kth_largest(const uint32_t (&g)[G], int k) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t trial = t | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < G; ++u) n += __popcll(__ballot(g[u] >= trial));
+    t = n >= k ? trial : t;
+  }
+  return t;
+}
 // A number that at least k of the threads' values reach: the k-th largest of the
-// maxima of 256 groups of threads, cut to its upper 16 bits, which one wave
-// finds a bit at a time by counting the groups that reach it.
+// maxima of 64 groups of threads, or of 256 where more are wanted (of 64 the k-th
+// largest is no bound to speak of for k near 64).
 template <int NT>
 DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh) {
   static_assert(NT >= 256 && NT <= kBins && kMost <= 256, "");
@@ -478,25 +493,40 @@ DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh) {
   all[tid] = most;
   __syncthreads();
   if (tid < 64) {
-    uint32_t g[4];
+    uint32_t g[4], one[1] = {0};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       g[u] = 0;
       for (int i = tid + 64 * u; i < NT; i += 256) g[u] = max(g[u], all[i]);
+      one[0] = max(one[0], g[u]);
     }
-    uint32_t t = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t trial = t | 1u << bit;
-      int n = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) n += __popcll(__ballot(g[u] >= trial));
-      t = n >= k ? trial : t;
-    }
+    const uint32_t t = k <= 32 ? kth_largest(one, k) : kth_largest(g, k);
     if (tid == 0) sh.word[0] = t;
   }
   __syncthreads();
   return sh.word[0];
+}
+
+// Appends to a list of *count entries: f(e, place) for every bit e < 8 of the lanes'
+// m, with one addition a wave.
+template <typename F>
+DSA_DEV void append(uint32_t m, uint32_t* count, F f) {
+  const uint64_t some = __ballot(m != 0);
+  if (some == 0) return;
+  // how many the lanes before have, and all: the bits of the lanes' counts
+  const uint32_t mine = (uint32_t)__popc(m);
+  uint32_t total = 0, at = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint64_t with = __ballot(mine >> b & 1);
+    total += (uint32_t)__popcll(with) << b;
+    at += __builtin_amdgcn_mbcnt_hi((uint32_t)(with >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)with, 0)) << b;
+  }
+  if (m == 0) return;
+  uint32_t first = 0;
+  if ((int)(threadIdx.x & 63) == __builtin_ctzll(some)) first = atomicAdd(count, total);
+  at += __builtin_amdgcn_readfirstlane(first);
+  for (; m; m &= m - 1) f(__builtin_ctz(m), at++);
 }
 
 DSA_DEV int round_8(int n) { return (n + 7) & ~7; }
@@ -583,13 +613,27 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
   const int segs = (l.pad + p.V - 1) / kSeg + 1;
   const uint32_t least = wide_key<T>(key_of<T>(-__builtin_inff()));
   uint32_t most = 0;
-  for (int i = tid; i < segs; i += NT) most = max(most, sh.keys[i]);
+  constexpr int U = 2048 / NT;  // keys of a thread in a step
+  for (int i = 0; i < segs; i += U * NT) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * NT + tid;
+      const uint32_t key = sh.keys[min(at, segs - 1)];
+      most = max(most, at < segs ? key : 0u);
+    }
+  }
   if (tid == 0) sh.word[1] = 0, sh.word[2] = 0;
   uint32_t bound = reached<NT>(wide_key<T>(most), k, sh);
-  for (int i = tid; i < segs; i += NT) {
-    if (wide_key<T>(sh.keys[i]) < bound) continue;
-    const uint32_t at = atomicAdd(&sh.word[1], 1u);
-    if (at < kCands) sh.seg[at] = i;
+  for (int i = 0; i < segs; i += U * NT) {
+    uint32_t in = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * NT + tid;
+      in |= (uint32_t)(at < segs && wide_key<T>(sh.keys[min(at, segs - 1)]) >= bound) << u;
+    }
+    append(in, &sh.word[1], [&](int u, uint32_t at) {
+      if (at < kCands) sh.seg[at] = i + u * NT + tid;
+    });
   }
   __syncthreads();
   const uint32_t found = sh.word[1];
@@ -605,13 +649,12 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
     const bool all = bound <= least;  // NaN are -inf here
     const float limit = all ? -__builtin_inff() : of_key<T>(sizeof(T) == 2 ? bound >> 16 : bound);
     values_of<T, NT>(l, sh, (int)found, [&](const float* x, int j, int lo, int hi) {
-      if (!all && !(max_of<N>(x) >= limit)) return;
+      uint32_t in = 0;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (e < lo || e >= hi || !(all || x[e] >= limit)) continue;
-        const uint32_t at = atomicAdd(&sh.word[2], 1u);
-        if (at < kCands) sh.cand[at] = (uint64_t)key_of<T>(x[e]) << 32 | (uint32_t)~(j + e);
-      }
+      for (int e = 0; e < N; ++e) in |= (uint32_t)(e >= lo && e < hi && (all || x[e] >= limit)) << e;
+      append(in, &sh.word[2], [&](int e, uint32_t at) {
+        if (at < kCands) sh.cand[at] = (uint64_t)key_of<T>((float)l.row[j + e]) << 32 | (uint32_t)~(j + e);
+      });
     });
     __syncthreads();
     const int n = (int)sh.word[2];
@@ -720,13 +763,18 @@ __global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
   write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds);
 }
 
-// The row's sums out of its parts', in every thread of the block.
-template <int NT, bool ENT>
-DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float* red) {
-  Run all = run_none();
+// The row's sums out of its parts', in every thread of the block; q: the thread's
+// first of them (part_of).
+DSA_DEV float4 part_of(const VocabRows& p, int64_t r) {
   const int n = p.parts * kPartWaves;
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const float4 q = p.part[r * n + i];
+  return (int)threadIdx.x < n ? p.part[r * n + threadIdx.x] : float4{kLowest, 0.f, 0.f, 0.f};
+}
+template <int NT, bool ENT>
+DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float4 q, float* red) {
+  Run all{q.x, q.y, q.z};
+  const int n = p.parts * kPartWaves;
+  for (int i = NT + threadIdx.x; i < n; i += NT) {
+    q = p.part[r * n + i];
     Run w{q.x, q.y, q.z};
     const float m = max2(all.m, w.m);
     raise<ENT>(all, m, p.c);
@@ -749,19 +797,21 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(VocabRows p) {
   }
   const Line<T> l(p.x, p.xs, r, p.V);
   const float x = given(l, p, id);
+  const float4 q = part_of(p, r);
   if constexpr (TOP) {
-    // eight loads in flight a thread; keys past the segments are not read
+    // the loads of 2048 keys in flight; keys past the segments are not read
+    constexpr int U = 2048 / NT;
     const uint32_t* seg = p.seg + r * p.segs;
-    for (int i = threadIdx.x; i < p.segs; i += 8 * NT) {
-      uint32_t k[8];
+    for (int i = threadIdx.x; i < p.segs; i += U * NT) {
+      uint32_t k[U];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) k[u] = seg[min(i + u * NT, p.segs - 1)];
+      for (int u = 0; u < U; ++u) k[u] = seg[min(i + u * NT, p.segs - 1)];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < U; ++u)
         if (i + u * NT < p.segs) lds[i + u * NT] = k[u];
     }
   }
-  const Run all = join_parts<NT, true>(p, r, red);
+  const Run all = join_parts<NT, true>(p, r, q, red);
   const float ln_s = logf(all.s);
   if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
   if constexpr (TOP) {
@@ -884,7 +934,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(VocabRows p) {
     write_no_loss(p, r);
     return;
   }
-  write_loss<T>(p, r, e, join_parts<64, false>(p, r, nullptr));
+  write_loss<T>(p, r, e, join_parts<64, false>(p, r, part_of(p, r), nullptr));
 }
 
 // ---------------------------------------------------------------------------

@@ -17,11 +17,14 @@ struct Logits {
 };
 
 c10::IntArrayRef row_shape(const Tensor& logits) { return logits.sizes().slice(0, logits.dim() - 1); }
-Tensor floats(const Tensor& on, c10::IntArrayRef shape) { return at::empty(shape, on.options().dtype(at::kFloat)); }
+// Results, allocated without the dispatcher's two calls for at::empty (a call on one
+// row makes five of them).
+Tensor fresh(const Tensor& on, c10::IntArrayRef shape, ScalarType t) { return at::detail::empty_cuda(shape, t, on.device(), std::nullopt); }
+Tensor floats(const Tensor& on, c10::IntArrayRef shape) { return fresh(on, shape, at::kFloat); }
 Tensor with_columns(const Tensor& logits, int64_t k, ScalarType t) {
   auto shape = row_shape(logits).vec();
   shape.push_back(k);
-  return at::empty(shape, logits.options().dtype(t));
+  return fresh(logits, shape, t);
 }
 Tensor row_stats(const Tensor& logits, int64_t N) { return floats(logits, {N, 4}); }
 
@@ -67,7 +70,7 @@ template <typename A>
 Tensor vocab_workspace(A& a, int32_t top, const Tensor& on) {
   const size_t n = dsa_vocab_workspace_bytes(a.N, a.V, a.dtype, top);
   if (n == 0) return Tensor();
-  const Tensor ws = bytes(on, n);
+  const Tensor ws = fresh(on, {(int64_t)n}, at::kByte);
   a.workspace = ws.data_ptr(), a.workspace_bytes = n;
   return ws;
 }

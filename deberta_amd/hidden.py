@@ -64,7 +64,7 @@ def _ext() -> Any:
     _lib.load()  # and checks its version
     if not EXT_PATH.exists():
         raise RuntimeError(
-            f"{EXT_PATH} is missing: the operators on hidden states are not built. Run `python -m deberta_amd._build` first."
+            f"{EXT_PATH} is missing: the operators on hidden states and logits are not built. Run `python -m deberta_amd._build` first."
         )
     from deberta_amd import _hidden_ext
 
