@@ -225,30 +225,36 @@ DSA_DEV Run wave_run(Run r, float c) {
   if (ENT) r.u = hid::lanes_sum<64>(r.u);
   return r;
 }
-// The block's sums out of its threads', in every thread; red: 3 words a wave.
+// The block's sums out of its threads', red: 3 words a wave.  leave_run by all of
+// them, then, behind a barrier, run_of by whoever needs them.
+template <bool ENT>
+DSA_DEV void leave_run(Run r, float c, float* red) {
+  r = wave_run<ENT>(r, c);
+  if ((threadIdx.x & 63) == 0) {
+    float* w = red + 3 * (threadIdx.x >> 6);
+    w[0] = r.m, w[1] = r.s, w[2] = r.u;
+  }
+}
+template <int NT, bool ENT>
+DSA_DEV Run run_of(const float* red, float c) {
+  float most = kLowest;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) most = max2(most, red[3 * i]);
+  Run all{most, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    Run w{red[3 * i], red[3 * i + 1], red[3 * i + 2]};
+    raise<ENT>(w, most, c);
+    all.s += w.s, all.u += w.u;
+  }
+  return all;
+}
 template <int NT, bool ENT>
 DSA_DEV Run block_run(Run r, float c, float* red) {
-  constexpr int W = NT / 64;
-  r = wave_run<ENT>(r, c);
-  if constexpr (W > 1) {
-    if ((threadIdx.x & 63) == 0) {
-      float* w = red + 3 * (threadIdx.x >> 6);
-      w[0] = r.m, w[1] = r.s, w[2] = r.u;
-    }
-    __syncthreads();
-    float most = kLowest;
-#pragma unroll
-    for (int i = 0; i < W; ++i) most = max2(most, red[3 * i]);
-    Run all{most, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      Run w{red[3 * i], red[3 * i + 1], red[3 * i + 2]};
-      raise<ENT>(w, most, c);
-      all.s += w.s, all.u += w.u;
-    }
-    r = all;
-  }
-  return r;
+  if constexpr (NT == 64) return wave_run<ENT>(r, c);
+  leave_run<ENT>(r, c, red);
+  __syncthreads();
+  return run_of<NT, ENT>(red, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -358,8 +364,9 @@ struct Shared {
   int* list;         // kMost
   uint32_t* picked;  // kMost
   uint32_t* word;    // 24
+  float* sums;       // m, ln s
 };
-constexpr int kSharedWords = kBins + 3 * kCands + 2 * kMost + 24;
+constexpr int kSharedWords = kBins + 3 * kCands + 2 * kMost + 24 + 2;
 DSA_DEV Shared shared_at(uint32_t* lds, int keys) {  // keys: a multiple of 4
   Shared s;
   s.keys = lds;
@@ -370,6 +377,7 @@ DSA_DEV Shared shared_at(uint32_t* lds, int keys) {  // keys: a multiple of 4
   s.list = s.seg + kCands;
   s.picked = reinterpret_cast<uint32_t*>(s.list + kMost);
   s.word = s.picked + kMost;
+  s.sums = reinterpret_cast<float*>(s.word + 24);
   return s;
 }
 
@@ -484,9 +492,10 @@ DSA_DEV uint32_t kth_largest(const uint32_t (&g)[G], int k) {
 }
 // A number that at least k of the threads' values reach: the k-th largest of the
 // maxima of 64 groups of threads, or of 256 where more are wanted (of 64 the k-th
-// largest is no bound to speak of for k near 64).
-template <int NT>
-DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh) {
+// largest is no bound to speak of for k near 64).  Meanwhile the second wave does
+// `other`.
+template <int NT, typename F>
+DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh, F other) {
   static_assert(NT >= 256 && NT <= kBins && kMost <= 256, "");
   const int tid = threadIdx.x;
   uint32_t* all = sh.hist;
@@ -502,6 +511,8 @@ DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh) {
     }
     const uint32_t t = k <= 32 ? kth_largest(one, k) : kth_largest(g, k);
     if (tid == 0) sh.word[0] = t;
+  } else if (tid < 128) {
+    other();
   }
   __syncthreads();
   return sh.word[0];
@@ -536,16 +547,16 @@ DSA_DEV uint32_t wide_key(uint32_t k) { return sizeof(T) == 2 ? k << 16 : k; }
 
 // One of the row's largest.
 template <typename T>
-DSA_DEV void put_top(const VocabRows& p, int64_t r, int rank, int j, uint32_t key, float m, float ln_s) {
+DSA_DEV void put_top(const VocabRows& p, int64_t r, int rank, int j, uint32_t key, const Shared& sh) {
   p.top_ids[r * p.top + rank] = j;
-  p.top_lp[r * p.top + rank] = fmaf(exponent(of_key<T>(key), m, p.c), kLn2, -ln_s);
+  p.top_lp[r * p.top + rank] = fmaf(exponent(of_key<T>(key), sh.sums[0], p.c), kLn2, -sh.sums[1]);
 }
 
 // The row's largest, from its segments' maxima in sh.keys: those of the k
 // segments whose maxima are largest (read again at every step: this is for rows
 // with thousands of equal values).
 template <typename T, int NT>
-DSA_DEV void top_of_segments(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, float m, float ln_s) {
+DSA_DEV void top_of_segments(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh) {
   const int tid = threadIdx.x, k = p.top;
   const int segs = (l.pad + p.V - 1) / kSeg + 1, found = min(k, segs);
   choose<NT>(sh, segs, found, [&](int i) { return sh.keys[i]; });
@@ -563,7 +574,7 @@ DSA_DEV void top_of_segments(const Line<T>& l, const VocabRows& p, int64_t r, co
     const uint32_t mine = sh.hist[tid];
     int rank = 0;
     for (int o = 0; o < k; ++o) rank += sh.hist[o] > mine || (sh.hist[o] == mine && o < tid);
-    put_top<T>(p, r, rank, column(sh.list[tid]), mine, m, ln_s);
+    put_top<T>(p, r, rank, column(sh.list[tid]), mine, sh);
   }
 }
 
@@ -602,18 +613,38 @@ DSA_DEV void values_of(const Line<T>& l, const Shared& sh, int found, F f) {
   }
 }
 
+// The given token's logit, NaN outside the vocabulary.
+template <typename T>
+DSA_DEV float given(const Line<T>& l, const VocabRows& p, int64_t id) {
+  return p.lp && id >= 0 && id < p.V ? (float)l.row[id] : __builtin_nanf("");
+}
+
+// One thread: the row's results; x: the given token's logit.
+DSA_DEV void write_row(const VocabRows& p, int64_t r, const Run& all, float ln_s, float x) {
+  const float ent = ln_s - kLn2 * all.u / all.s;
+  if (p.lp) p.lp[r] = fmaf(exponent(x, all.m, p.c), kLn2, -ln_s);
+  if (p.ent) p.ent[r] = ent;
+  if (p.lse) p.lse[r] = fmaf(all.m, p.inv_t, ln_s);
+  if (p.stats) p.stats[r] = float4{all.m, ln_s, ent, 1.f / all.s};
+}
+
 // The same where few values compete, as nearly always: a bound that k values
 // reach leaves a few segments, and of those a few values, whose ranks are counted
 // (value and place in one number, so that equal values go by their place).  Where
-// there are more than kCands of either, top_of_segments takes over.
+// there are more than kCands of either, top_of_segments takes over.  The row's other
+// results too, from its waves' sums in red and the given token's logit x: a wave has
+// them ready while another looks for the bound (64 largest of 2048 x 128100 bf16 96.7
+// to 95.8 us, 10 of 512 x 128128 32.0 to 31.5, against one after the other).  Keys and
+// red may be fresh: a barrier comes first.
 template <typename T, int NT>
-DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, float m, float ln_s) {
+DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh, const float* red, float x) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x, k = p.top;
   const int segs = (l.pad + p.V - 1) / kSeg + 1;
   const uint32_t least = wide_key<T>(key_of<T>(-__builtin_inff()));
-  uint32_t most = 0;
   constexpr int U = 2048 / NT;  // keys of a thread in a step
+  uint32_t most = 0;
+  __syncthreads();
   for (int i = 0; i < segs; i += U * NT) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -623,7 +654,14 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
     }
   }
   if (tid == 0) sh.word[1] = 0, sh.word[2] = 0;
-  uint32_t bound = reached<NT>(wide_key<T>(most), k, sh);
+  uint32_t bound = reached<NT>(wide_key<T>(most), k, sh, [&] {
+    const Run sums = run_of<NT, true>(red, p.c);
+    const float ln_s = logf(sums.s);
+    if (tid == 64) {
+      write_row(p, r, sums, ln_s, x);
+      sh.sums[0] = sums.m, sh.sums[1] = ln_s;
+    }
+  });
   for (int i = 0; i < segs; i += U * NT) {
     uint32_t in = 0;
 #pragma unroll
@@ -644,7 +682,7 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
       round = 1;
       float top = -__builtin_inff();
       values_of<T, NT>(l, sh, (int)found, [&](const float* x, int, int, int) { top = max2(top, max_of<N>(x)); });
-      bound = max(bound, reached<NT>(wide_key<T>(key_of<T>(top)), k, sh));
+      bound = max(bound, reached<NT>(wide_key<T>(key_of<T>(top)), k, sh, [] {}));
     }
     const bool all = bound <= least;  // NaN are -inf here
     const float limit = all ? -__builtin_inff() : of_key<T>(sizeof(T) == 2 ? bound >> 16 : bound);
@@ -673,7 +711,7 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
 #pragma unroll
           for (int u = 0; u < 8; ++u) rank += other[u] > mine;
         }
-        if (rank < k) put_top<T>(p, r, rank, (int)~(uint32_t)mine, (uint32_t)(mine >> 32), m, ln_s);
+        if (rank < k) put_top<T>(p, r, rank, (int)~(uint32_t)mine, (uint32_t)(mine >> 32), sh);
       }
       return;
     }
@@ -681,7 +719,7 @@ DSA_DEV void write_top(const Line<T>& l, const VocabRows& p, int64_t r, const Sh
     if (tid == 0) sh.word[2] = 0;
     __syncthreads();
   }
-  top_of_segments<T, NT>(l, p, r, sh, m, ln_s);
+  top_of_segments<T, NT>(l, p, r, sh);
 }
 
 // ---------------------------------------------------------------------------
@@ -700,21 +738,6 @@ DSA_DEV void write_none(const VocabRows& p, int64_t r) {
   for (int t = tid; t < p.top; t += NT) p.top_lp[r * p.top + t] = 0.f, p.top_ids[r * p.top + t] = -1;
 }
 
-// The given token's logit, NaN outside the vocabulary.
-template <typename T>
-DSA_DEV float given(const Line<T>& l, const VocabRows& p, int64_t id) {
-  return p.lp && id >= 0 && id < p.V ? (float)l.row[id] : __builtin_nanf("");
-}
-
-// One thread: the row's results; x: the given token's logit.
-DSA_DEV void write_row(const VocabRows& p, int64_t r, const Run& all, float ln_s, float x) {
-  const float ent = ln_s - kLn2 * all.u / all.s;
-  if (p.lp) p.lp[r] = fmaf(exponent(x, all.m, p.c), kLn2, -ln_s);
-  if (p.ent) p.ent[r] = ent;
-  if (p.lse) p.lse[r] = fmaf(all.m, p.inv_t, ln_s);
-  if (p.stats) p.stats[r] = float4{all.m, ln_s, ent, 1.f / all.s};
-}
-
 template <typename T, int NT, bool TOP, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   extern __shared__ __align__(16) uint32_t lds[];
@@ -728,12 +751,13 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(VocabRows p) {
   }
   const Line<T> l(p.x, p.xs, r, p.V);
   const float x = given(l, p, id);  // early: its way from memory is long
-  const Run all = block_run<NT, true>(stream<T, NT, true, TOP, FAR>(l, 0, kRow, p.c, lds, p.segs), p.c, red);
-  const float ln_s = logf(all.s);
-  if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
+  const Run mine = stream<T, NT, true, TOP, FAR>(l, 0, kRow, p.c, lds, p.segs);
   if constexpr (TOP) {
-    __syncthreads();
-    write_top<T, NT>(l, p, r, shared_at(lds, p.keys), all.m, ln_s);
+    leave_run<true>(mine, p.c, red);
+    write_top<T, NT>(l, p, r, shared_at(lds, p.keys), red, x);
+  } else {
+    const Run all = block_run<NT, true>(mine, p.c, red);
+    if (threadIdx.x == 0) write_row(p, r, all, logf(all.s), x);
   }
 }
 
@@ -763,14 +787,13 @@ __global__ __launch_bounds__(NT) void logprobs_part_kernel(VocabRows p) {
   write_part<T, NT, true, TOP, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, lds);
 }
 
-// The row's sums out of its parts', in every thread of the block; q: the thread's
-// first of them (part_of).
+// A thread's share of a row's parts; q: its first (part_of).
 DSA_DEV float4 part_of(const VocabRows& p, int64_t r) {
   const int n = p.parts * kPartWaves;
   return (int)threadIdx.x < n ? p.part[r * n + threadIdx.x] : float4{kLowest, 0.f, 0.f, 0.f};
 }
 template <int NT, bool ENT>
-DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float4 q, float* red) {
+DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float4 q) {
   Run all{q.x, q.y, q.z};
   const int n = p.parts * kPartWaves;
   for (int i = NT + threadIdx.x; i < n; i += NT) {
@@ -781,7 +804,7 @@ DSA_DEV Run join_parts(const VocabRows& p, int64_t r, float4 q, float* red) {
     raise<ENT>(w, m, p.c);
     all.s += w.s, all.u += w.u;
   }
-  return block_run<NT, ENT>(all, p.c, red);
+  return all;
 }
 
 template <typename T, int NT, bool TOP>
@@ -811,12 +834,13 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(VocabRows p) {
         if (i + u * NT < p.segs) lds[i + u * NT] = k[u];
     }
   }
-  const Run all = join_parts<NT, true>(p, r, q, red);
-  const float ln_s = logf(all.s);
-  if (threadIdx.x == 0) write_row(p, r, all, ln_s, x);
+  const Run mine = join_parts<NT, true>(p, r, q);
   if constexpr (TOP) {
-    __syncthreads();
-    write_top<T, NT>(l, p, r, shared_at(lds, p.keys), all.m, ln_s);
+    leave_run<true>(mine, p.c, red);
+    write_top<T, NT>(l, p, r, shared_at(lds, p.keys), red, x);
+  } else {
+    const Run all = block_run<NT, true>(mine, p.c, red);
+    if (threadIdx.x == 0) write_row(p, r, all, logf(all.s), x);
   }
 }
 
@@ -934,7 +958,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(VocabRows p) {
     write_no_loss(p, r);
     return;
   }
-  write_loss<T>(p, r, e, join_parts<64, false>(p, r, part_of(p, r), nullptr));
+  write_loss<T>(p, r, e, wave_run<false>(join_parts<64, false>(p, r, part_of(p, r)), p.c));
 }
 
 // ---------------------------------------------------------------------------
