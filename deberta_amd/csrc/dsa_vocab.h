@@ -29,14 +29,14 @@
 //
 // HBM bounds it where there are many rows; of 128100 bf16 columns, us and TB/s of
 // what has to move (a read reaches 6.3 here, a fill 6.9, a copy 5.0):
-//   forward   1229 rows in parts 56.6 + 5.0 to join (315 MB, 5.1), 4096 rows of a
-//             distillation 159 + 17 (1.05 GB, 6.0); 64 largest of 2048 rows, whole, 112 in a
-//             trace and 99 to 101 a pass (525 MB, 5.2)
-//   backward  1229 rows 94.7 (630 MB, 6.6, in part from the last-level cache), 4096 rows
-//             of a distillation 383 (2.10 GB, 5.5), of a loss with 85% of the rows left
+//   forward   1229 rows in parts 55 + 5 to join (315 MB, 5.3), 4096 rows of a
+//             distillation 152 + 17 (1.05 GB, 6.2); 64 largest of 2048 rows, whole, 107 in a
+//             trace and 93 to 96 a pass (525 MB, 5.5)
+//   backward  1229 rows 94 (630 MB, 6.7, in part from the last-level cache), 4096 rows
+//             of a distillation 379 (2.10 GB, 5.5), of a loss with 85% of the rows left
 //             out 197 (1.21 GB, 6.1)
 // With few rows it is the chain of a launch, a part's batch, a join and its reads: one
-// row 3.8 + 6.3 us with its 5 largest, 17 by one block.
+// row 3.8 + 5.1 us with its 5 largest, 16 by one block (and its host side 8.7).
 #pragma once
 
 #include <type_traits>
@@ -491,9 +491,10 @@ DSA_DEV uint32_t kth_largest(const uint32_t (&g)[G], int k) {
   return t;
 }
 // A number that at least k of the threads' values reach: the k-th largest of the
-// maxima of 64 groups of threads, or of 256 where more are wanted (of 64 the k-th
-// largest is no bound to speak of for k near 64).  Meanwhile the second wave does
-// `other`.
+// maxima of 64 groups of threads up to k = 32, of 256 from there on, where the k-th
+// of 64 is too low a bound (512 x 128128 bf16, of 256 and of 64 groups: 16 largest
+// 29.4 and 28.8 us, 32 29.8 and 29.3, 48 30.1 and 30.8, 64 30.9 and 46.6).  Meanwhile
+// the second wave does `other`.
 template <int NT, typename F>
 DSA_DEV uint32_t reached(uint32_t most, int k, const Shared& sh, F other) {
   static_assert(NT >= 256 && NT <= kBins && kMost <= 256, "");

@@ -136,8 +136,8 @@ constexpr int kBackPer = 2048;
 // them, of 512 rows (131 MB) 663 and 655, of 1229 rows 1382 and 1356.
 constexpr double kFarBytes = 64 << 20;
 // Logits that a forward reads past the caches: of the last level's size and more,
-// where no backward reads them again (the 64 largest of 2048 x 128100 bf16 108.3
-// and 105.4 us), and those of a distillation from twice that on (4096 rows with the
+// where no backward reads them again (the 64 largest of 2048 x 128100 bf16 102
+// and 95 us), and those of a distillation from twice that on (4096 rows with the
 // gradient 582 and 551; 1229 rows, 315 MB, 171 and 168).  Not those of a loss, whose
 // rows may be left out, so that fewer bytes are read again than there are: 1229
 // rows 152 and 164, 4096 of which 85% are left out 240 and 292.
@@ -157,14 +157,14 @@ struct Cut {
 };
 
 // Whether rows go in parts, joined by a second launch.  Few long rows leave most
-// of the card idle by themselves: 1 x 128100 bf16 11.5 us whole, 8.4 in parts (the
-// host's share), 128 rows 12.6 and 11.0, 192 rows 13.4 and 14.1; with the 10 largest
-// 17.0 and 11.4, 128 rows 18.2 and 17.8, 192 rows 19.1 and 20.8; 64000 columns are as
-// fast whole (7.3 and 8.3, 11.9 and 10.6).  And many bytes are read faster where
+// of the card idle by themselves: 1 x 128100 bf16 11.0 us whole, 9.6 in parts (the
+// host's share), 128 rows 12.2 and 11.3, 192 rows 13.1 and 13.6; with the 10 largest
+// 16.2 and 10.4, 128 rows 17.2 and 15.6, 192 rows 18.1 and 18.6; 64000 columns are as
+// fast whole (7.2 and 9.4, 10.9 and 10.5).  And many bytes are read faster where
 // neighbouring blocks read neighbouring lines: the loss of 1229 x 128100 with its
 // gradient 161.6 and 152.2, of 777 x 50021 fp32 80.1 and 76.9 (in between, 512 x
-// 128100 24.0 and 26.6), but not with the largest to find, whose search then has
-// nothing to hide behind: 64 of 2048 rows 106 and 121.
+// 128100 23.9 and 26.5), but not with the largest to find, whose search then has
+// nothing to hide behind: 64 of 2048 rows 93 and 115.
 bool in_parts(int64_t N, int64_t row_bytes, int top) {
   const double bytes = bytes_of(N, row_bytes, 1);
   if (row_bytes >= 160 << 10 && bytes < 36 << 20) return true;
