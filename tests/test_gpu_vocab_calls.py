@@ -93,6 +93,22 @@ def test_a_pending_sign_counts(gpu):
         assert torch.equal(call(neg), call(lambda t: -t))
 
 
+def test_results_are_allocated_as_others(gpu):
+    """Results are inference tensors in inference mode, and in the allocator's count."""
+    x, ids = _rand(5, 24, seed=1).to(gpu), torch.tensor([3, 0, 4, 1, 2], device=gpu)
+    want = da.fused_token_logprobs(x, ids, top_k=3)
+    with torch.inference_mode():
+        got = da.fused_token_logprobs(x, ids, top_k=3)
+        loss = da.fused_distillation_loss(x, ids[:, None], x[:, :1])
+    assert all(t.is_inference() for t in (*got, loss)) and not any(t.is_inference() for t in want)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    before = torch.cuda.memory_allocated()
+    big = da.fused_token_logprobs(torch.zeros(1 << 20, 2, device=gpu))
+    assert torch.cuda.memory_allocated() - before == 2 * 4 << 20  # entropy and lse; the logits are gone
+    del big
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_traced_calls_compute(gpu):
     """torch.jit.trace records the ops, not what the extension allocates."""
     x, y = _rand(5, 300, seed=1).to(gpu), _rand(5, 300, seed=2).to(gpu)
