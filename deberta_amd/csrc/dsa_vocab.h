@@ -966,7 +966,8 @@ __global__ __launch_bounds__(64) void distill_join_kernel(VocabRows p) {
 // backward: e = exp2((x - m) c), dx = e (a + b (x - m) c) and, at a few
 // columns, a term more
 
-// the row's constants, and the columns with a term of their own in LDS
+// the row's constants, and how many columns have a term of their own in LDS (behind
+// them up to a multiple of 4 column -1)
 struct Grad {
   float m, a, b;
   int n;
@@ -1052,12 +1053,21 @@ DSA_DEV void write_grad(const VocabRows& p, int64_t r, const Part<T>& part, cons
   for (int t = tid; t < g.n; t += NT) {
     const int j = col[t];
     if (j < 0 || !part.has(j)) continue;
+    // those of the same column in their order, four a step (4096 x 4000 bf16 with 128
+    // entries 40 us one by one, 31 so; a pass of 1229 x 128100 with 64 169.7 and 167.2)
     float sum = 0.f;
     bool first = true;
-    for (int o = 0; o < g.n; ++o) {
-      const bool same = col[o] == j;
-      if (same) sum += term[o];
-      if (same && o < t) first = false;
+    for (int o = 0; o < g.n; o += 4) {
+      const int4 c = *reinterpret_cast<const int4*>(col + o);
+      const float4 w = *reinterpret_cast<const float4*>(term + o);
+      const int cs[4] = {c.x, c.y, c.z, c.w};
+      const float ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool same = cs[i] == j;
+        sum += same ? ws[i] : 0.f;
+        first = first && !(same && o + i < t);
+      }
     }
     if (first) out[j] = (T)(grad_of<B>(g, exponent((float)row[j], g.m, p.c)) + sum);
   }
@@ -1075,8 +1085,8 @@ DSA_DEV void write_zeros(const Part<T>& part) {
 
 template <typename T, int NT, bool B, bool FAR>
 __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
-  __shared__ int col[kMost + 1];
-  __shared__ float term[kMost + 1];
+  __shared__ __align__(16) int col[kMost + 4];
+  __shared__ __align__(16) float term[kMost + 4];
   const int tid = threadIdx.x;
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
@@ -1104,6 +1114,7 @@ __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
   }
   const bool in = p.dlp && id >= 0 && id < p.V;
   if (tid == 0) col[0] = in ? (int)id : -1, term[0] = g * p.inv_t;
+  if (tid < 3) col[1 + k + tid] = -1;  // up to a multiple of 4
   Grad d;
   d.m = st.x, d.n = 1 + k;
   // p_j (a + b ln p_j) / T with ln p_j = ln 2 t - ln s, p_j = e / s
@@ -1118,8 +1129,8 @@ __global__ __launch_bounds__(NT) void logprobs_bwd_kernel(VocabRows p) {
 
 template <typename T, int NT, bool FAR>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(VocabRows p) {
-  __shared__ int col[kMost];
-  __shared__ float term[kMost];
+  __shared__ __align__(16) int col[kMost];
+  __shared__ __align__(16) float term[kMost];
   const int64_t r = p.row0 + blockIdx.x / (uint32_t)p.parts;
   const Part<T> part(p, r, blockIdx.x % (uint32_t)p.parts);
   const Entries e = entries_of(p, r);
@@ -1136,7 +1147,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(VocabRows p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int k = threadIdx.x + 64 * i;
-      if (k < p.K) col[k] = e.id[i] < p.V ? (int)e.id[i] : -1, term[k] = -g * e.q[i];
+      col[k] = k < p.K && e.id[i] < p.V ? (int)e.id[i] : -1, term[k] = -g * e.q[i];
     }
   }
   write_grad<T, NT, false, FAR>(p, r, part, d, col, term);
