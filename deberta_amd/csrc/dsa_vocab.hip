@@ -126,7 +126,7 @@ int check_distill(const dsa_distill_args* a, bool bwd) {
   return a->dlogits_stride < a->V && a->N > 1 ? fail("%s: dlogits' rows overlap", what) : 0;
 }
 
-constexpr int kThreads = 512;   // of a block that has a row
+constexpr int kThreads = 512, kThreadsNarrow = 256;  // of a block that has a row (by_width)
 constexpr int kPart = 64 * voc::kPartWaves;  // of one that has a part of a row
 constexpr int kPartMost = 2048, kPartLeast = 256;  // 16-byte vectors of a part
 constexpr int kBack = 512;
@@ -147,6 +147,17 @@ template <typename F>
 void by_bool(bool b, F f) {
   if (b) f(std::true_type{});
   else f(std::false_type{});
+}
+// f(threads of a block that has a row).  Many narrow rows are bound by each row's chain of
+// steps, so more of them at once: 4096 x 1001 bf16 19.8 us by 512 threads and 11.4 by
+// 256, with the 16 largest 51.9 and 28.4, 4096 x 16000 40.2 and 31.1, 2223 x 40155 43.8
+// and 37.4; of 160 KB a row and few rows alike (2223 x 40155 fp32 58.8 and 59.5, 512 x
+// 16000 bf16 9.5 and 9.0, 256 rows 7.9 and 7.9, with the 128 largest 12.9 and 15.3); wide
+// rows the other way (2048 x 128100 bf16 92.5 and 95.2, fp32 159.8 and 171.1).
+template <typename F>
+void by_width(int64_t N, int64_t row_bytes, F f) {
+  if (N >= 512 && row_bytes <= 128 << 10) f(std::integral_constant<int, kThreadsNarrow>{});
+  else f(std::integral_constant<int, kThreads>{});
 }
 double bytes_of(int64_t N, int64_t V, size_t elem) { return (double)N * (double)V * (double)elem; }
 
@@ -212,7 +223,10 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
     return by_rows(N, 1, "logprobs_fwd_kernel", [&](int64_t r, unsigned rows) {
       p.row0 = r;
       by_bool(far, [&](auto f) {
-        hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, kThreads, TOP, decltype(f)::value>), dim3(rows), dim3(kThreads), lds, st, p);
+        by_width(N, (int64_t)p.V * sizeof(T), [&](auto n) {
+          constexpr int NT = decltype(n)::value;
+          hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, NT, TOP, decltype(f)::value>), dim3(rows), dim3(NT), lds, st, p);
+        });
       });
     });
   const size_t part_lds = TOP ? (size_t)p.per * 16 / sizeof(T) / voc::kSeg * 4 : 0;
@@ -251,7 +265,10 @@ int distill_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
     return by_rows(N, 1, "distill_fwd_kernel", [&](int64_t r, unsigned rows) {
       p.row0 = r;
       by_bool(far, [&](auto f) {
-        hipLaunchKernelGGL((voc::distill_fwd_kernel<T, kThreads, decltype(f)::value>), dim3(rows), dim3(kThreads), 0, st, p);
+        by_width(N, (int64_t)p.V * sizeof(T), [&](auto n) {
+          constexpr int NT = decltype(n)::value;
+          hipLaunchKernelGGL((voc::distill_fwd_kernel<T, NT, decltype(f)::value>), dim3(rows), dim3(NT), 0, st, p);
+        });
       });
     });
   return by_rows(N, p.parts, "distill_part_kernel", [&](int64_t r, unsigned rows) {

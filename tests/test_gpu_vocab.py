@@ -355,6 +355,21 @@ def test_many_rows(gpu):
         _check_logprobs(x, _ints(-1, V, N, seed=19).masked_fill_(_ints(0, 5, N, seed=20) == 0, -100).clamp(min=-100), 2, grads="nll")
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+@pytest.mark.parametrize("N", [511, 512, 700])
+def test_many_narrow_rows(N, dtype, gpu):
+    """The blocks that such rows go to (fewer threads from 512 rows on), with ties in
+    their hundreds, rows left out and the largest in every number."""
+    for V, k, grads in ((130, 128, "all"), (1001, 5, "all"), (1001, 64, "nll"), (3001, 20, "nll")):
+        _say("narrow", N, V, k, dtype)
+        x = _rand(N, V, seed=V + k, dtype=dtype)
+        x[::7] = x[::7].round()
+        x[3::50] = 1.5
+        ids = _ints(0, V, N, seed=V).masked_fill_(_ints(0, 6, N, seed=k) == 0, -100)
+        _check_logprobs(x.to(gpu), ids, k, 1.5, grads=grads)
+    _check_distill(_rand(N, 777, seed=3, dtype=dtype).to(gpu), _ints(-1, 777, N, 33, seed=4), _rand(N, 33, seed=5, std=3.0), 2.0)
+
+
 def test_offsets_past_32_bits(gpu):
     """Rows that begin past 2^31 elements, and past 2^32 bytes; the rows between
     are left out.  Against the same rows by themselves, whose sums may go in
