@@ -322,12 +322,14 @@ def _cpu_distillation(
         raise IndexError(f"{what}: a teacher's id is outside the vocabulary of {V}")
     wide = _wide_dtype(logits.dtype)
     given = ids >= 0
-    t = (teacher_logits.to(wide) / temperature).masked_fill(~given, -math.inf)
+    t = teacher_logits.to(wide).masked_fill(~given, -math.inf)
     if teacher_lse is not None:
-        log_q = t - teacher_lse.to(wide).unsqueeze(-1)
+        log_q = t / temperature - teacher_lse.to(wide).unsqueeze(-1)
     else:
-        some = ~(t == -math.inf).all(-1, keepdim=True)
-        log_q = torch.log_softmax(torch.where(some, t, 0.0), -1).masked_fill(~some, -math.inf)
+        # the largest off first, as from the student's: the type's lowest value would overflow
+        most = t.amax(-1, keepdim=True)
+        some = most != -math.inf
+        log_q = torch.log_softmax(torch.where(some, (t - most) / temperature, 0.0), -1).masked_fill(~some, -math.inf)
     log_q = log_q.masked_fill(~given, -math.inf)
     q = log_q.exp()
     z, _ = _cpu_scaled(logits, ~given.any(-1), temperature)

@@ -517,6 +517,25 @@ def test_distill_masks(dtype, gpu):
     assert (d[1] == 0).all() and d[0].abs().sum() > 0
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+def test_distill_teachers_that_leave_float32(dtype, gpu):
+    """A teacher whose logits / T leave float32: its largest is taken off first, so
+    that a row of the type's lowest value is uniform."""
+    x, ids, lowest = _rand(4, 333, seed=3, dtype=dtype).to(gpu), _ints(0, 333, 4, 3, seed=4), torch.finfo(FP).min
+    teacher = _rand(4, 3, seed=5)
+    teacher[0], teacher[2, 1] = lowest, lowest
+    teacher[1] = 3e38 + 1e37 * torch.arange(3)
+    _say("distill far teachers", dtype)
+    for T in (0.5, 0.25):
+        _check_distill(x, ids, teacher, T)
+    _check_distill(x, ids, torch.full((4, 3), torch.finfo(BF).min, dtype=BF), 0.5)
+    T, far = 2.0**-100, torch.tensor([[1e9, 1e9 - 64.0]]).repeat(4, 1).to(gpu)  # q = (1, 0): T (max - x), as in the test above of such temperatures
+    c = x.cpu().double()
+    loss = da.fused_distillation_loss(x, torch.stack((x.argmin(-1), x.argmax(-1)), -1), far, T).cpu().double()
+    want = T * (c.amax(-1) - c.amin(-1))
+    assert ((loss - want).abs() <= 8 * U * want).all()
+
+
 def test_distill_strides(gpu):
     wide = _rand(6, 1111, seed=6, dtype=BF).to(gpu)
     ids, teacher = _ints(0, 1001, 6, 9, seed=7), _rand(6, 9, seed=8)

@@ -157,6 +157,27 @@ def test_cpu_distillation_at_extreme_temperatures():
         assert (da.fused_distillation_loss(x[:, :1], zero[:, :1].long(), zero, T) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_cpu_distillation_takes_the_teachers_largest_off_before_its_scaling(dtype):
+    """A teacher whose logits / T leave float32: rows of the type's lowest value are
+    uniform, as they are on the device, and differences decide, not the values."""
+    x, ids = _rand(4, 50, dtype=dtype), torch.randint(0, 50, (4, 3), generator=torch.Generator().manual_seed(2))
+    teacher = _rand(4, 3, seed=3)
+    teacher[0] = torch.finfo(torch.float32).min
+    teacher[1] = 3e38 + 1e37 * torch.arange(3)
+    teacher[2, 1] = torch.finfo(torch.float32).min  # probability 0
+    for T in (0.5, 0.25):
+        q, log_q = ov.teacher_probs(ids, teacher, T)
+        assert (q[0] - 1 / 3).abs().max() < 1e-15 and q[1].tolist() == [0, 0, 1] and q[2, 1] == 0
+        _near(da.fused_distillation_loss(x, ids, teacher, T), ov.distillation(ov.log_probs(x, T), ids, q, log_q, T))
+    # q = (1, 0), so T^2 (-log p) = T (max - x): a product with 1 / T, two with T and a difference
+    T, far = 2.0**-100, torch.tensor([[1e9, 1e9 - 64.0]]).expand(4, 2)
+    ids = torch.stack((x.argmin(-1), x.argmax(-1)), -1)
+    want = T * (x.double().amax(-1) - x.double().amin(-1))
+    got = da.fused_distillation_loss(x, ids, far, T).double()
+    assert ((got - want).abs() <= 8 * 2.0**-24 * want).all()
+
+
 @pytest.mark.parametrize("shape", [(0, 9), (2, 0, 9)], ids=str)
 def test_cpu_no_rows(shape):
     x = torch.zeros(shape)
