@@ -318,9 +318,13 @@ def _cpu_distillation(
     for name, t, shape in (("teacher_logits", teacher_logits, tuple(ids.shape)), ("teacher_lse", teacher_lse, rows)):
         if t is not None and (tuple(t.shape) != shape or t.device != logits.device):
             raise ValueError(f"{what}: {name} must have shape {shape} and be on {logits.device}, got {tuple(t.shape)} on {t.device}")
+    wide = _wide_dtype(logits.dtype)  # float64 beside a student in float64 alone
+    if teacher_logits.dtype not in (torch.float32, torch.bfloat16, wide):
+        raise TypeError(f"{what} teacher_logits: dtype must be float32 or bfloat16, got {teacher_logits.dtype}")
+    if teacher_lse is not None and teacher_lse.dtype not in (torch.float32, wide):
+        raise TypeError(f"{what}: teacher_lse must be float32, got {teacher_lse.dtype}")
     if (ids >= V).any():
         raise IndexError(f"{what}: a teacher's id is outside the vocabulary of {V}")
-    wide = _wide_dtype(logits.dtype)
     given = ids >= 0
     t = teacher_logits.to(wide).masked_fill(~given, -math.inf)
     if teacher_lse is not None:

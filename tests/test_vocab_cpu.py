@@ -228,6 +228,28 @@ def test_refusals():
         d(x, t_ids, teacher)
 
 
+def test_a_teachers_types_are_the_devices():
+    """float32 or bfloat16 logits and a float32 logsumexp, as on the GPU; float64
+    beside a student in float64, which is computed so."""
+    x, ids, teacher, lse = _rand(3, 8), torch.tensor([[1], [2], [3]]), torch.zeros(3, 1), torch.zeros(3)
+    d = da.fused_distillation_loss
+    for student in (x, x.bfloat16(), x.double()):
+        for t in (torch.float16, torch.int64, torch.int32, torch.bool, torch.complex64):
+            with pytest.raises(TypeError, match="teacher_logits: dtype must be float32 or bfloat16"):
+                d(student, ids, teacher.to(t))
+        for t in (torch.float16, torch.bfloat16, torch.int64):
+            with pytest.raises(TypeError, match="teacher_lse must be float32"):
+                d(student, ids, teacher, 1.0, lse.to(t))
+        for t in (torch.float32, torch.bfloat16):
+            assert d(student, ids, teacher.to(t), 1.0, lse).isfinite().all()
+    for student in (x, x.bfloat16()):
+        with pytest.raises(TypeError, match="teacher_logits: dtype must be float32 or bfloat16"):
+            d(student, ids, teacher.double())
+        with pytest.raises(TypeError, match="teacher_lse must be float32"):
+            d(student, ids, teacher, 1.0, lse.double())
+    assert d(x.double(), ids, teacher.double(), 1.0, lse.double()).dtype == torch.float64
+
+
 # ---------------------------------------------------------------------------
 # calls on device tensors, seen without one (see test_hidden_calls_cpu.py)
 
