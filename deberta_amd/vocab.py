@@ -352,13 +352,21 @@ def fused_distillation_loss(
     logits, float32 ``(...)``, with ``p = softmax(logits / T)`` over the whole
     vocabulary and the teacher's entries ``teacher_ids`` (int64 or int32) and
     ``teacher_logits`` (float32 or bfloat16), both ``(..., K)`` with K at most 128,
-    in any order: for example the top ids of :func:`fused_token_logprobs` with
-    their log probabilities (a constant of the row does not matter).
+    in any order.
 
-    ``q = softmax(teacher_logits / T)`` over the row's entries; with
-    ``teacher_lse`` (float32 ``(...)``), the logsumexp of the teacher's whole
+    ``q = softmax(teacher_logits / T)`` over the row's entries, to which a constant
+    of the row does not matter: for example the ``top_ids`` and ``top_logprobs`` of
+    :func:`fused_token_logprobs` at temperature 1, or at any temperature t
+    ``t * top_logprobs`` (its results are of ``logits / t``, and this function divides
+    by T whatever it is given).
+
+    With ``teacher_lse`` (float32 ``(...)``), the logsumexp of the teacher's whole
     ``logits / T``, ``q = exp(teacher_logits / T - teacher_lse)``, whose sum is
-    below one: what the teacher gives to other tokens is then left out.
+    below one: what the teacher gives to other tokens is then left out.  The two
+    have to be of the same logits, and a constant of one alone does matter: of a
+    teacher's pass at the temperature T itself ``T * top_logprobs`` with a
+    ``teacher_lse`` of zeros (its ``logsumexp`` goes with the raw logits, not with
+    its log probabilities).
 
     A negative id is no entry, and one of probability 0 adds nothing whatever
     the student's is; a row without entries is not read, its loss and gradient are

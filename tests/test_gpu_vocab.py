@@ -536,6 +536,22 @@ def test_distill_teachers_that_leave_float32(dtype, gpu):
     assert ((loss - want).abs() <= 8 * U * want).all()
 
 
+def test_distill_from_a_teachers_pass(gpu):
+    """What a pass at T stores, times T, are logits with a logsumexp of 0: the
+    teacher's own probabilities at T."""
+    T, K = 2.0, 40
+    for dtype in (BF, FP):
+        c = _rand(6, 1001, seed=31, dtype=dtype)
+        t = da.fused_token_logprobs(c.to(gpu), top_k=K, temperature=T)
+        lse = torch.zeros(6)
+        _check_distill(_rand(6, 1001, seed=32, dtype=dtype).to(gpu), t.top_ids.cpu(), T * t.top_logprobs.cpu(), T, lse)
+        loss = da.fused_distillation_loss(c.to(gpu), t.top_ids, T * t.top_logprobs, T, lse.to(gpu)).cpu().double()
+        # of a student that is the teacher nothing: q = p to the pass' (200 + 4 |lp|) u, a product's and the loss' own
+        lp = torch.log_softmax(c.double() / T, -1).gather(-1, t.top_ids.cpu())
+        q, l = lp.exp(), lp.abs()
+        assert (loss.abs() <= T * T * U * (q * ((6 * l + 40) * 2 * l + 2 * (220 + 8 * l))).sum(-1)).all()
+
+
 def test_distill_strides(gpu):
     wide = _rand(6, 1111, seed=6, dtype=BF).to(gpu)
     ids, teacher = _ints(0, 1001, 6, 9, seed=7), _rand(6, 9, seed=8)

@@ -228,6 +228,25 @@ def test_refusals():
         d(x, t_ids, teacher)
 
 
+@pytest.mark.parametrize("t", [1.0, 2.0, 0.7])
+def test_what_a_teachers_pass_stores_gives_its_probabilities(t):
+    """The documented ways from a pass at t to the loss at T: of a student that is the
+    teacher, with q over the entries the loss of those alone, with the teacher's own
+    probabilities nothing.  In float64, to far more than the roundings of 50 terms."""
+    x, T, K = _rand(5, 50, dtype=torch.float64), 2.0, 12
+    p = da.fused_token_logprobs(x, top_k=K, temperature=t)
+    logp = torch.log_softmax(x / T, -1).gather(-1, p.top_ids)
+    log_q = torch.log_softmax(x.gather(-1, p.top_ids) / T, -1)
+    got = da.fused_distillation_loss(x, p.top_ids, t * p.top_logprobs, T)
+    assert (got - T * T * (log_q.exp() * (log_q - logp)).sum(-1)).abs().max() < 1e-12
+    if t == 1.0:
+        assert torch.equal(got, da.fused_distillation_loss(x, p.top_ids, p.top_logprobs, T))
+    if t == T:
+        zeros = torch.zeros_like(p.entropy)
+        assert da.fused_distillation_loss(x, p.top_ids, T * p.top_logprobs, T, zeros).abs().max() < 1e-12
+        assert da.fused_distillation_loss(x, p.top_ids, x.gather(-1, p.top_ids), T, p.logsumexp).abs().max() < 1e-12
+
+
 def test_a_teachers_types_are_the_devices():
     """float32 or bfloat16 logits and a float32 logsumexp, as on the GPU; float64
     beside a student in float64, which is computed so."""
