@@ -257,6 +257,87 @@ def test_rows_by_the_hundred_megabytes(gpu):
             assert ((e[r].double() - want).abs() <= tol).all()
 
 
+def _logprobs_agree(o, x, ids, T):
+    """Every result against float64, in pieces of up to 9M values on the GPU."""
+    N, V = x.shape
+    k = 0 if o.top_ids is None else o.top_ids.shape[-1]
+    step = max(1, (9 << 20) // V)
+    for lo in range(0, N, step):
+        r = slice(lo, lo + step)
+        logp = torch.log_softmax(x[r].double() / T, -1)
+        out = ids[r] == -100
+        lp = logp.gather(-1, ids[r].clamp(min=0).unsqueeze(-1)).squeeze(-1).masked_fill(out, 0.0)
+        assert ((o.logprobs[r].double() - lp).abs() <= U * (200 + 4 * lp.abs())).all()
+        H, M2 = ov.moments(logp)
+        assert ((o.entropy[r].double() - H.masked_fill(out, 0.0)).abs() <= U * (200 + 200 * H + 6 * M2)).all()
+        z = x[r].double() / T
+        lse, m = torch.logsumexp(z, -1).masked_fill(out, 0.0), z.amax(-1).abs()
+        assert ((o.logsumexp[r].double() - lse).abs() <= U * (200 + 3 * m + lse.abs())).all()
+        if k:
+            top = torch.sort(x[r].float(), dim=-1, descending=True, stable=True).indices[:, :k]
+            assert torch.equal(o.top_ids[r], top.masked_fill(out.unsqueeze(-1), -1))
+            tl = logp.gather(-1, top).masked_fill(out.unsqueeze(-1), 0.0)
+            assert ((o.top_logprobs[r].double() - tl).abs() <= U * (200 + 4 * tl.abs())).all()
+
+
+def _distillation_agrees(loss, x, t_ids, teacher, T):
+    N, V = x.shape
+    step = max(1, (9 << 20) // V)
+    for lo in range(0, N, step):
+        r = slice(lo, lo + step)
+        logp = torch.log_softmax(x[r].double() / T, -1)
+        q, lq = ov.teacher_probs(t_ids[r], teacher[r], T)
+        at = t_ids[r].clamp(min=0)
+        lqa, la = lq.nan_to_num(0, 0, 0).abs(), logp.gather(-1, at).abs()
+        tol = T * T * U * (q * ((3 * lqa + 40) * (lqa + la) + 220 + 4 * la + 3 * lqa)).sum(-1)
+        assert ((loss[r].double() - ov.distillation(logp, at, q, lq, T)).abs() <= tol).all()
+
+
+def _entries(N, V, K, gpu):
+    t_ids = torch.randint(0, V, (N, K), generator=torch.Generator().manual_seed(3))
+    t_ids[3::5, K // 2 :] = -1
+    t_ids[2::9] = -1
+    return t_ids.to(gpu), _rand(N, K, seed=4, std=3.0).to(gpu)
+
+
+@pytest.mark.parametrize(
+    "N,V,dtype,k",
+    [
+        (1100, 128100, BF, 5), (560, 128100, FP, 5),  # whole rows by 512 threads
+        (2100, 65001, BF, 64), (2100, 32501, FP, 64),  # by 256
+        (1100, 128100, BF, 0), (560, 128100, FP, 0),  # in parts
+        (8400, 16001, BF, 0), (8400, 8001, FP, 0),  # as many bytes in rows of one part
+    ],
+)
+def test_logits_past_the_caches(N, V, dtype, k, gpu):
+    """Forwards that autograd does not record, from 256 MiB on: their loads go past
+    the caches.  A seventh of the rows is left out."""
+    _say("past the caches", N, V, dtype, k)
+    x = _on_gpu(N, V, seed=N + V, gpu=gpu, dtype=dtype)
+    assert x.numel() * x.element_size() >= 256 << 20
+    ids = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(2)).to(gpu)
+    ids[5::7] = -100
+    _logprobs_agree(da.fused_token_logprobs(x, ids, top_k=k, temperature=1.3), x, ids, 1.3)
+
+
+@pytest.mark.parametrize(
+    "N,V,dtype,grad",
+    [
+        (1100, 128100, BF, False), (560, 128100, FP, False), (8400, 16001, BF, False), (8400, 8001, FP, False),
+        (2100, 128100, BF, True), (1100, 128100, FP, True),
+    ],
+)
+def test_distillations_past_the_caches(N, V, dtype, grad, gpu):
+    """From 256 MiB on where no backward reads the logits again, from 512 MiB on
+    where one does."""
+    _say("distillation past the caches", N, V, dtype, grad)
+    x = _on_gpu(N, V, seed=N + V, gpu=gpu, dtype=dtype)
+    assert x.numel() * x.element_size() >= (512 if grad else 256) << 20
+    t_ids, teacher = _entries(N, V, 40, gpu)
+    loss = da.fused_distillation_loss(x.requires_grad_(grad), t_ids, teacher, 1.3).detach()
+    _distillation_agrees(loss, x.detach(), t_ids, teacher, 1.3)
+
+
 def test_more_rows_than_a_launch_takes(gpu):
     """2^22 blocks a launch: rows of two columns, where log p is -log1p(exp(-d)) of
     their difference, to the tolerances above."""
