@@ -749,3 +749,54 @@ def test_training_step_of_teacher_and_student(gpu):
         assert (a.cpu().double() - b).norm() <= 1e-4 * b.norm()
     best = head.predict(hidden, weight, top_k=4)
     assert torch.equal(best.top_ids[:, 0], head(hidden, weight).argmax(-1))
+
+
+@pytest.mark.parametrize("autocast", [False, True], ids=["bf16", "autocast"])
+def test_training_step_in_bf16(autocast, gpu):
+    """The same step with a head in bf16, and with one in float32 under bf16 autocast:
+    bf16 logits go into the operators, gradients have their leaves' types.  Against
+    float64 from the same values: the dense product, its bias, GELU, LayerNorm, the
+    vocabulary's product and its bias round to bf16 forward, at most as many products and
+    sums backward, and a logit's error of six half steps of the largest logit (here below
+    5) moves p by 6 * 5 half steps.  All one way, with a factor of two for the GELU's
+    slope: logits off by 12 half steps of the largest, a gradient by (12 + 12 + 30) 2^-8 of
+    its norm."""
+    torch.manual_seed(0)
+    C, V, N, T = 64, 1500, 160, 1.5
+    config = SimpleNamespace(hidden_size=C, vocab_size=V, layer_norm_eps=1e-7)
+    kept = FP if autocast else BF
+    head, weight = da.FusedMLMHead(config).to(gpu, kept), torch.nn.Parameter(_rand(V, C, seed=1, std=0.1, dtype=kept).to(gpu))
+    with torch.no_grad():
+        head.bias.copy_(_rand(V, seed=6, std=0.1).to(gpu))
+        head.dense.bias.copy_(_rand(C, seed=7, std=0.1).to(gpu))
+    hidden = _rand(N, C, seed=2, std=1.0, dtype=kept).to(gpu).requires_grad_()
+    labels = _ints(0, V, N, seed=4).masked_fill_(_ints(0, 3, N, seed=5) == 0, -100).to(gpu)
+    teacher = da.fused_token_logprobs(_rand(N, V, seed=3, dtype=BF).to(gpu), top_k=32)
+    with torch.autocast("cuda", dtype=BF, enabled=autocast):
+        logits = head(hidden, weight)
+        mlm, rows = head.forward_loss(hidden, weight, labels)
+        distil = head.forward_distillation(hidden, weight, teacher.top_ids, teacher.top_logprobs, T)
+        best = head.predict(hidden, weight, top_k=4)
+    assert logits.dtype == BF and mlm.dtype == distil.dtype == rows.entropy.dtype == FP
+    # the operators read these logits
+    _check_logprobs(logits.detach(), labels.cpu(), 4)
+    assert torch.equal(best.top_ids, da.fused_token_logprobs(logits.detach(), top_k=4).top_ids)
+    leaves = [hidden, weight, *head.parameters()]
+    got = torch.autograd.grad(mlm + distil, leaves)
+
+    F = torch.nn.functional
+    copies = [t.detach().cpu().double().requires_grad_() for t in leaves]
+    named = dict(zip([n for n, _ in head.named_parameters()], copies[2:]))
+    z = F.layer_norm(F.gelu(F.linear(copies[0], named["dense.weight"], named["dense.bias"])), (C,), named["LayerNorm.weight"], named["LayerNorm.bias"], 1e-7)
+    z = F.linear(z, copies[1], named["bias"])
+    h, most = 2.0**-8, z.abs().max().item()
+    assert most < 5
+    assert (logits.detach().cpu().double() - z.detach()).abs().max() <= 12 * h * most
+    logp = ov.log_probs(z, T)
+    q, log_q = ov.teacher_probs(teacher.top_ids.cpu(), teacher.top_logprobs.cpu(), T)
+    want = [F.cross_entropy(z, labels.cpu()), ov.distillation(logp, teacher.top_ids.cpu(), q, log_q, T).mean()]
+    # a log probability moves by twice what the logits are off by (over T, times T^2)
+    assert abs(mlm.item() - want[0].item()) <= 24 * h * most and abs(distil.item() - want[1].item()) <= 24 * h * most * T
+    for leaf, a, b in zip(leaves, got, torch.autograd.grad(sum(want), copies)):
+        assert a.dtype == leaf.dtype
+        assert (a.cpu().double() - b).norm() <= 54 * h * b.norm(), leaf.shape
