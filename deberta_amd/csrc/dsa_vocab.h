@@ -948,18 +948,20 @@ __global__ __launch_bounds__(NT) void distill_part_kernel(VocabRows p) {
   write_part<T, NT, false, false, FAR>(p, r, blockIdx.x % (uint32_t)p.parts, nullptr);
 }
 
-// A wave a row.  (4096 rows of 128 entries 14 us, each entry's logit a line of its
+// (4096 rows of 128 entries 14 us by a wave each, each entry's logit a line of its
 // own from memory; handed on by the parts, which had them in the caches, 6 and 5
 // more in the parts.)
-template <typename T>
-__global__ __launch_bounds__(64) void distill_join_kernel(VocabRows p) {
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_join_kernel(VocabRows p) {
+  __shared__ float red[3 * (NT / 64)];
   const int64_t r = p.row0 + blockIdx.x;
-  const Entries e = entries_of(p, r);
+  const Entries e = entries_of(p, r);  // by every wave
   if (!e.any) {
     write_no_loss(p, r);
     return;
   }
-  write_loss<T>(p, r, e, wave_run<false>(join_parts<64, false>(p, r, part_of(p, r)), p.c));
+  const Run all = block_run<NT, false>(join_parts<NT, false>(p, r, part_of(p, r)), p.c, red);
+  if (threadIdx.x < 64) write_loss<T>(p, r, e, all);
 }
 
 // ---------------------------------------------------------------------------

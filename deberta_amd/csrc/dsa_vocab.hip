@@ -159,6 +159,16 @@ void by_width(int64_t N, int64_t row_bytes, F f) {
   if (N >= 512 && row_bytes <= 128 << 10) f(std::integral_constant<int, kThreadsNarrow>{});
   else f(std::integral_constant<int, kThreads>{});
 }
+// f(threads of a block that joins a row's parts).  The join by 64 threads of a row in 63
+// parts 3.4 us, in 513 10.5, in 2442 45, by 1024 2.5, 2.8 and 5.8; a pass of 24 rows in 257
+// parts 36.9 and 33.3, of 100 rows in 17 parts 15.3 and 15.8.
+constexpr int kPartsOfAWave = 32;
+template <bool TOP, typename F>
+void by_parts(int parts, F f) {
+  if constexpr (TOP) f(std::integral_constant<int, 256>{});  // of 2^19 columns at most
+  else if (parts <= kPartsOfAWave) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 1024>{});
+}
 double bytes_of(int64_t N, int64_t V, size_t elem) { return (double)N * (double)V * (double)elem; }
 
 // How a forward cuts its rows.
@@ -167,18 +177,36 @@ struct Cut {
   size_t part_bytes, bytes;
 };
 
-// Whether rows go in parts, joined by a second launch.  Few long rows leave most
-// of the card idle by themselves: 1 x 128100 bf16 11.0 us whole, 9.6 in parts (the
-// host's share), 128 rows 12.2 and 11.3, 192 rows 13.1 and 13.6; with the 10 largest
-// 16.2 and 10.4, 128 rows 17.2 and 15.6, 192 rows 18.1 and 18.6; 64000 columns are as
-// fast whole (7.2 and 9.4, 10.9 and 10.5).  And many bytes are read faster where
+// Whether rows go in parts, joined by a second launch.  A block's time goes by its
+// row's columns, bf16 and fp32 alike (a lane's chain of loads and sums), that of parts
+// by all bytes, behind a launch more.  us of a pass whole and in parts, by rows:
+//   128100 bf16    8: 11.6 10.7    96: 12.1 10.7   160: 12.9 12.7   192: 13.3 13.9
+//   128100 fp32    8: 12.1 10.7    64: 12.3 11.3    96: 13.1 14.3
+//   262144 bf16    8: 19.9 11.2   128: 21.7 17.3   192: 21.8 21.7   224: 22.2 24.1
+//   262144 fp32    8: 21.4 10.9    48: 21.4 13.7    96: 22.0 19.8   128: 22.2 24.0
+//   524288 fp32    8: 38.4 10.6    96: 40.6 33.3   128: 48.3 43.9
+//   2^20   fp32    8: 73.7 11.0    64: 87.0 44.3
+//   82000  bf16    8:  9.6 11.7    96:  9.9 10.8
+// and with the largest, whose search is one block's either way (5, 20 or 64 of them):
+//   128100 bf16    8: 16.7 11.9   128: 17.5 16.2   160: 17.7 17.5   192: 18.0 19.0
+//   128100 fp32    8: 19.1 12.0    64: 19.3 14.5    96: 19.8 17.0   128: 19.4 19.5
+//   262144 fp32    8: 32.5 13.1    96: 32.9 25.8   128: 33.2 30.0   192: 34.8 38.8
+//   64000  fp32    8: 15.0 14.4    64: 15.2 15.2   100: 15.2 16.8 (64)
+//   50021  fp32    8: 12.4 11.9   100: 12.4 12.9 (20)
+//   48000  bf16    8: 10.2 12.1 (20)
+// So rows go in parts while their bytes are below a line over the columns: none below
+// 70000 (46000) columns, 41 (37) MB at 128100, all of 262144 and more without the
+// largest (by the next rule), up to 215 MB of 524288 with them.  A lane of a whole row
+// adds up 32 batches at most then, 64 with the largest.
+//
+// And many bytes are read faster where
 // neighbouring blocks read neighbouring lines: the loss of 1229 x 128100 with its
 // gradient 161.6 and 152.2, of 777 x 50021 fp32 80.1 and 76.9 (in between, 512 x
 // 128100 23.9 and 26.5), but not with the largest to find, whose search then has
 // nothing to hide behind: 64 of 2048 rows 93 and 115.
-bool in_parts(int64_t N, int64_t row_bytes, int top) {
-  const double bytes = bytes_of(N, row_bytes, 1);
-  if (row_bytes >= 160 << 10 && bytes < 36 << 20) return true;
+bool in_parts(int64_t N, int64_t V, int elem, int top) {
+  const double bytes = bytes_of(N, V, elem);
+  if (bytes < (top ? 450. * (double)(V - 46000) : 700. * (double)(V - 70000))) return true;
   return !top && bytes >= 128 << 20;
 }
 
@@ -187,7 +215,7 @@ Cut cut_of(int64_t N, int64_t V, int dt, int top) {
   const int64_t most = V / (dt == DSA_BF16 ? 8 : 4) + 9;  // vectors, wherever a row begins
   c.segs = (int)(V / voc::kSeg) + 2;
   c.parts = 1, c.per = kPartMost;
-  if (!in_parts(N, V * elem_bytes(dt), top)) return c;
+  if (!in_parts(N, V, elem_bytes(dt), top)) return c;
   // 128100 bf16 in 63 parts 4.2 us, in 8 parts 5.0
   while (c.per > kPartLeast && N * cdiv(most, c.per) < 512) c.per /= 2;
   c.parts = (int)cdiv(most, c.per);
@@ -239,8 +267,10 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
          }) ||
          by_rows(N, 1, "logprobs_join_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
-           constexpr int NT = TOP ? 256 : 64;
-           hipLaunchKernelGGL((voc::logprobs_join_kernel<T, NT, TOP>), dim3(rows), dim3(NT), lds, st, p);
+           by_parts<TOP>(p.parts, [&](auto n) {
+             constexpr int NT = decltype(n)::value;
+             hipLaunchKernelGGL((voc::logprobs_join_kernel<T, NT, TOP>), dim3(rows), dim3(NT), lds, st, p);
+           });
          });
 }
 
@@ -279,7 +309,10 @@ int distill_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
          }) ||
          by_rows(N, 1, "distill_join_kernel", [&](int64_t r, unsigned rows) {
            p.row0 = r;
-           hipLaunchKernelGGL((voc::distill_join_kernel<T>), dim3(rows), dim3(64), 0, st, p);
+           by_parts<false>(p.parts, [&](auto n) {
+             constexpr int NT = decltype(n)::value;
+             hipLaunchKernelGGL((voc::distill_join_kernel<T, NT>), dim3(rows), dim3(NT), 0, st, p);
+           });
          });
 }
 

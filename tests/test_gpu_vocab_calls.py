@@ -338,6 +338,75 @@ def test_distillations_past_the_caches(N, V, dtype, grad, gpu):
     _distillation_agrees(loss, x.detach(), t_ids, teacher, 1.3)
 
 
+@pytest.mark.parametrize(
+    "N,V,dtype,k",
+    [
+        (100, 128100, FP, 0), (70, 128100, FP, 20), (60, 262144, FP, 0), (36, 262145, BF, 64), (20, 1 << 19, FP, 5),
+        (110, 1 << 19, FP, 5),  # whole
+        (24, (1 << 21) + 1, FP, 0), (1, 5_000_001, BF, 0), (1, 20_000_000, FP, 0), (1, 1 << 25, BF, 0),
+    ],
+)
+def test_few_long_rows(N, V, dtype, k, gpu):
+    """Rows in up to 2442 parts, and the longest that a block reads by itself.  The sum's
+    share is 400 u: of a whole row 16 + 64 + 10 additions and as many scalings of 3 u by a
+    larger maximum, of one in parts 16 + 2 + 10 and 10 in the join; 3 ln V <= 52."""
+    _say("long rows", N, V, dtype, k)
+    x = _on_gpu(N, V, seed=N, gpu=gpu, dtype=dtype)
+    ids = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(2)).to(gpu)
+    ids[2::7] = -100
+    t_ids, teacher = _entries(N, V, 40, gpu)
+    o = da.fused_token_logprobs(x, ids, top_k=k, temperature=1.3)
+    loss = da.fused_distillation_loss(x, t_ids, teacher, 1.3)
+    for r in range(N):
+        z = x[r].double() / 1.3
+        lse = torch.logsumexp(z, -1)
+        if ids[r] == -100:
+            assert o.logprobs[r] == 0 and o.entropy[r] == 0 and o.logsumexp[r] == 0
+        else:
+            lp = z[ids[r]] - lse
+            assert abs(o.logprobs[r].double() - lp) <= U * (400 + 4 * lp.abs())
+            assert abs(o.logsumexp[r].double() - lse) <= U * (400 + 3 * z.amax().abs() + lse.abs())
+            H, M2 = ov.moments(z - lse)
+            assert abs(o.entropy[r].double() - H) <= U * (400 + 400 * H + 6 * M2)
+            if k:
+                top = torch.sort(x[r].float(), descending=True, stable=True).indices[:k]
+                assert torch.equal(o.top_ids[r], top)
+                assert ((o.top_logprobs[r].double() - (z[top] - lse)).abs() <= U * (400 + 4 * (z[top] - lse).abs())).all()
+        q, lq = ov.teacher_probs(t_ids[r], teacher[r], 1.3)
+        at = t_ids[r].clamp(min=0)
+        lqa, la = lq.nan_to_num(0, 0, 0).abs(), (z[at] - lse).abs()
+        want = 1.3**2 * torch.where(q == 0, 0.0, q * (lq - (z[at] - lse))).sum()
+        assert abs(loss[r].double() - want) <= 1.3**2 * U * (q * ((3 * lqa + 40) * (lqa + la) + 420 + 4 * la + 3 * lqa)).sum()
+
+
+def test_the_longest_row(gpu):
+    """2^31 - 128 columns, forward and backward, in pieces against float64.  A lane of the
+    join adds up 512 parts' sums: 540 additions and as many scalings of 3 u, 3 ln V <= 65:
+    2300 u."""
+    V, T = (1 << 31) - 128, 1.3
+    _say("the longest row")
+    x = torch.empty(1, V, dtype=BF, device=gpu).normal_(generator=torch.Generator(device=gpu).manual_seed(1)).requires_grad_()
+    for token in (0, V - 1):
+        ids = torch.tensor([token], device=gpu)
+        o = da.fused_token_logprobs(x, ids, temperature=T)
+        pieces = x.detach().view(-1).split(1 << 27)
+        lse = torch.logsumexp(torch.stack([torch.logsumexp(c.double() / T, -1) for c in pieces]), -1)
+        lp = x.detach()[0, token].double() / T - lse
+        assert abs(o.logprobs.double() - lp) <= U * (2300 + 4 * lp.abs())
+        assert abs(o.logsumexp.double() - lse) <= U * (2300 + 24 + lse)
+    (d,) = torch.autograd.grad(o.logprobs.sum(), x)
+    at = 0
+    for c, e in zip(pieces, d.view(-1).split(1 << 27)):
+        logp = c.double() / T - lse
+        want = -logp.exp() / T
+        tol = U * -want * (3 * logp.abs() + 2300) + 2.0**-8 * want.abs()
+        at += c.numel()
+        if at == V:
+            want[-1] += 1 / T
+            tol[-1] += 4 * U + 2.0**-8
+        assert ((e.double() - want).abs() <= tol).all()
+
+
 def test_more_rows_than_a_launch_takes(gpu):
     """2^22 blocks a launch: rows of two columns, where log p is -log1p(exp(-d)) of
     their difference, to the tolerances above."""
