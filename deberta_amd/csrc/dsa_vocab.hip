@@ -253,7 +253,8 @@ int logprobs_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
       by_bool(far, [&](auto f) {
         by_width(N, (int64_t)p.V * sizeof(T), [&](auto n) {
           constexpr int NT = decltype(n)::value;
-          hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, NT, TOP, decltype(f)::value>), dim3(rows), dim3(NT), lds, st, p);
+          constexpr bool FAR = decltype(f)::value && (TOP || NT == kThreadsNarrow);  // so many bytes of wide rows are in parts
+          hipLaunchKernelGGL((voc::logprobs_fwd_kernel<T, NT, TOP, FAR>), dim3(rows), dim3(NT), lds, st, p);
         });
       });
     });
@@ -297,7 +298,8 @@ int distill_fwd(voc::VocabRows p, int64_t N, hipStream_t st) {
       by_bool(far, [&](auto f) {
         by_width(N, (int64_t)p.V * sizeof(T), [&](auto n) {
           constexpr int NT = decltype(n)::value;
-          hipLaunchKernelGGL((voc::distill_fwd_kernel<T, NT, decltype(f)::value>), dim3(rows), dim3(NT), 0, st, p);
+          constexpr bool FAR = decltype(f)::value && NT == kThreadsNarrow;
+          hipLaunchKernelGGL((voc::distill_fwd_kernel<T, NT, FAR>), dim3(rows), dim3(NT), 0, st, p);
         });
       });
     });
