@@ -13,11 +13,12 @@ with.
 
 One pass over the logits forward and one backward; they are float32 or bfloat16
 of any width, row stride and element alignment, arithmetic and results are
-float32, and equal inputs give equal bits (the order of a row's sums goes by the
-shape and by where the row begins between two 128-byte borders).  With z = logits / temperature and
-lse = log(sum(exp(z))), a logit of -inf has probability 0 and adds nothing; a
-row with a NaN or +inf, or without a finite logit, has NaN results (lse -inf
-where all are -inf).
+float32, and equal calls give equal bits (the order of a row's sums goes by the
+shape and type, by whether top alternatives are asked for and by where the row
+begins between two 128-byte borders: any of these may change the last bits).  With
+z = logits / temperature and lse = log(sum(exp(z))), a logit of -inf has
+probability 0 and adds nothing; a row with a NaN or +inf, or without a finite
+logit, has NaN results (lse -inf where all are -inf).
 
 In plain eager mode the functions go through the package's extension
 (csrc/vocab_ext.h); CPU tensors run the same in torch operations (float64 ones

@@ -13,9 +13,10 @@
  * Rows (2^36 at most) hold V contiguous values; the logits' and the gradient's
  * row strides are given, every other tensor is contiguous, and what a call writes
  * overlaps nothing else that it takes.  Logits are DSA_F32 or DSA_BF16;
- * arithmetic, sums and results are float32.  Equal inputs give equal bits (no
- * float atomics); the order of a row's sums goes by where it begins between two
- * 128-byte borders and by N and V.
+ * arithmetic, sums and results are float32.  Equal calls give equal bits (no
+ * float atomics).  The order of a row's sums goes by where it begins between two
+ * 128-byte borders, by N, V and dtype and by whether top_k is 0: other rows beside
+ * it, or the largest asked for, may change the last bits of its results.
  *
  * A logit of -inf has probability 0 and adds nothing to sums, entropy or
  * gradients.  A row with a NaN or +inf among its logits, or without a finite
