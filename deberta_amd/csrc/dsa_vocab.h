@@ -22,10 +22,15 @@
 // by k values at least, so the k largest lie in the segments that reach it and
 // are among their values that do: about as many lines of the row as there are
 // values to find are read again, and the ranks of what reaches the bound are counted
-// (write_top).  Where thousands of values are equal the k segments whose maxima
-// are largest (equal ones: the first) are selected exactly, and of their values the
-// k largest (top_of_segments): a value outside of them, at most its own segment's
-// maximum, has k larger ones before it.
+// (write_top).  Where more than 512 segments or values reach the number, the k segments
+// whose maxima are largest (equal ones: the first) are selected exactly, and of their
+// values the k largest (top_of_segments): a value outside of them, at most its own
+// segment's maximum, has k larger ones before it.  The number is one of 16 bits, so that
+// is a row with thousands of values near its largest that are equal in their upper 16
+// bits: equal ones in bf16, ones of the same 2^-7 of their value in fp32.  (512 x 128100
+// fp32 normals of deviation 2, and the same plus 1000, us: 20 largest 45 and 54, 64 48
+// and 69, 128 52 and 90; in bf16, of which 1000 leaves every fourth whole number, 29 and
+// 33, 31 and 34, 33 and 69.)
 //
 // HBM bounds it where there are many rows; of 128100 bf16 columns, us and TB/s of
 // what has to move (a read reaches 6.3 here, a fill 6.9, a copy 5.0):
@@ -555,7 +560,7 @@ DSA_DEV void put_top(const VocabRows& p, int64_t r, int rank, int j, uint32_t ke
 
 // The row's largest, from its segments' maxima in sh.keys: those of the k
 // segments whose maxima are largest (read again at every step: this is for rows
-// with thousands of equal values).
+// with thousands of values that are equal in their upper 16 bits).
 template <typename T, int NT>
 DSA_DEV void top_of_segments(const Line<T>& l, const VocabRows& p, int64_t r, const Shared& sh) {
   const int tid = threadIdx.x, k = p.top;

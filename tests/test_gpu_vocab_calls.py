@@ -407,6 +407,22 @@ def test_the_longest_row(gpu):
         assert ((e.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("N,V", [(3, 128100), (200, 128100), (3, 20011), (600, 20011)])
+def test_the_largest_of_moved_rows(N, V, gpu):
+    """Thousands of values that are equal in their upper 16 bits and differ below them:
+    more than compete in the fast search.  In parts, and by 512 and 256 threads."""
+    for dtype in (FP, BF):
+        x = (_on_gpu(N, V, seed=V, gpu=gpu, dtype=FP) + 1000.0).to(dtype)
+        x[1] = 1000.0 - (x[1] - 1000.0).abs()  # the largest side by side at one value
+        want = torch.sort(x.float(), dim=-1, descending=True, stable=True).indices
+        for k in (1, 20, 64, 128):
+            _say("moved", N, V, dtype, k)
+            o = da.fused_token_logprobs(x, top_k=k)
+            assert torch.equal(o.top_ids, want[:, :k])
+            tl = torch.log_softmax(x.double(), -1).gather(-1, want[:, :k])
+            assert ((o.top_logprobs.double() - tl).abs() <= U * (200 + 4 * tl.abs())).all()
+
+
 def test_more_rows_than_a_launch_takes(gpu):
     """2^22 blocks a launch: rows of two columns, where log p is -log1p(exp(-d)) of
     their difference, to the tolerances above."""
