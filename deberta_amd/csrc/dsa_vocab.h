@@ -33,13 +33,14 @@
 // 33, 31 and 34, 33 and 69.)
 //
 // HBM bounds it where there are many rows; of 128100 bf16 columns, us and TB/s of
-// what has to move (a read reaches 6.3 here, a fill 6.9, a copy 5.0):
+// what has to move (kernels that only read reach 6.4 to 7.0 so, that copy 6.1):
 //   forward   1229 rows in parts 55 + 5 to join (315 MB, 5.3), 4096 rows of a
-//             distillation 152 + 17 (1.05 GB, 6.2); 64 largest of 2048 rows, whole, 107 in a
-//             trace and 93 to 96 a pass (525 MB, 5.5)
-//   backward  1229 rows 94 (630 MB, 6.7, in part from the last-level cache), 4096 rows
+//             distillation 152 + 17 (1.05 GB, 6.9 the parts by themselves); 64 largest of
+//             2048 rows, whole, 95 to 96 a pass of a settled card (525 MB, 5.5), 102 to
+//             133 in the first hundred behind an idle one
+//   backward  1229 rows 95 (630 MB, 6.6, in part from the last-level cache), 4096 rows
 //             of a distillation 379 (2.10 GB, 5.5), of a loss with 85% of the rows left
-//             out 197 (1.21 GB, 6.1)
+//             out 198 (1.21 GB, 6.1)
 // With few rows it is the chain of a launch, a part's batch, a join and its reads: one
 // row 3.8 + 5.1 us with its 5 largest, 16 by one block (and its host side 8.7).
 #pragma once
