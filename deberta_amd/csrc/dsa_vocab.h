@@ -36,7 +36,7 @@
 // what has to move (kernels that only read reach 6.4 to 7.0 so, that copy 6.1):
 //   forward   1229 rows in parts 55 + 5 to join (315 MB, 5.3), 4096 rows of a
 //             distillation 152 + 17 (1.05 GB, 6.9 the parts by themselves); 64 largest of
-//             2048 rows, whole, 95 to 96 a pass of a settled card (525 MB, 5.5), 102 to
+//             2048 rows, whole, 95 to 98 a pass of a settled card (525 MB, 5.5), 102 to
 //             133 in the first hundred behind an idle one
 //   backward  1229 rows 95 (630 MB, 6.6, in part from the last-level cache), 4096 rows
 //             of a distillation 379 (2.10 GB, 5.5), of a loss with 85% of the rows left

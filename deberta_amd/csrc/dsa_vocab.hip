@@ -180,24 +180,28 @@ struct Cut {
 // Whether rows go in parts, joined by a second launch.  A block's time goes by its
 // row's columns, bf16 and fp32 alike (a lane's chain of loads and sums), that of parts
 // by all bytes, behind a launch more.  us of a pass whole and in parts, by rows:
+//   82000  bf16    8:  9.6 11.7    96:  9.9 10.8
 //   128100 bf16    8: 11.6 10.7    96: 12.1 10.7   160: 12.9 12.7   192: 13.3 13.9
 //   128100 fp32    8: 12.1 10.7    64: 12.3 11.3    96: 13.1 14.3
-//   262144 bf16    8: 19.9 11.2   128: 21.7 17.3   192: 21.8 21.7   224: 22.2 24.1
+//   262144 bf16    8: 19.9 11.2   128: 21.7 17.3   192: 21.8 21.7   250: 22.3 25.2
 //   262144 fp32    8: 21.4 10.9    48: 21.4 13.7    96: 22.0 19.8   128: 22.2 24.0
 //   524288 fp32    8: 38.4 10.6    96: 40.6 33.3   128: 48.3 43.9
 //   2^20   fp32    8: 73.7 11.0    64: 87.0 44.3
-//   82000  bf16    8:  9.6 11.7    96:  9.9 10.8
 // and with the largest, whose search is one block's either way (5, 20 or 64 of them):
-//   128100 bf16    8: 16.7 11.9   128: 17.5 16.2   160: 17.7 17.5   192: 18.0 19.0
-//   128100 fp32    8: 19.1 12.0    64: 19.3 14.5    96: 19.8 17.0   128: 19.4 19.5
-//   262144 fp32    8: 32.5 13.1    96: 32.9 25.8   128: 33.2 30.0   192: 34.8 38.8
-//   64000  fp32    8: 15.0 14.4    64: 15.2 15.2   100: 15.2 16.8 (64)
-//   50021  fp32    8: 12.4 11.9   100: 12.4 12.9 (20)
 //   48000  bf16    8: 10.2 12.1 (20)
-// So rows go in parts while their bytes are below a line over the columns: none below
-// 70000 (46000) columns, 41 (37) MB at 128100, all of 262144 and more without the
-// largest (by the next rule), up to 215 MB of 524288 with them.  A lane of a whole row
-// adds up 32 batches at most then, 64 with the largest.
+//   64000  bf16    8: 13.2 13.2    64: 13.6 13.9   100: 13.6 14.6 (64)
+//   82000  bf16    8: 14.1 12.3    96: 14.2 13.9   160: 14.1 15.2 (5)
+//   50021  fp32    8: 12.4 11.9   100: 12.4 12.9 (20)
+//   64000  fp32    8: 15.0 14.4    64: 15.2 15.2   100: 15.2 16.8 (64)
+//   128100 bf16    8: 16.7 11.9   128: 17.5 16.2   160: 17.7 17.5   192: 18.0 19.0 (5)
+//   128100 fp32    8: 19.1 12.0    64: 19.3 14.5    96: 19.8 17.0   128: 19.4 19.5 (5)
+//   262144 bf16    8: 29.9 16.4   128: 30.7 27.1   192: 31.5 31.7 (64)
+//   262144 fp32    8: 34.9 16.9    96: 35.7 30.1   128: 35.8 34.2   160: 35.9 38.9 (64)
+// So rows go in parts while their bytes are below lines over the columns.  Without the
+// largest none below 70000 columns, 41 MB of 128100, 102 of 262144, and all of 333000 and
+// more (by the next rule).  With them none below 51000 in bf16, 46000 in fp32, whose search
+// is the longer, 38 MB of 128100 and 53, and none of so many bytes that whole rows are read
+// past the caches.  A lane of a whole row adds up 41 batches at most then, 64 with the largest.
 //
 // And many bytes are read faster where
 // neighbouring blocks read neighbouring lines: the loss of 1229 x 128100 with its
@@ -205,9 +209,9 @@ struct Cut {
 // 128100 23.9 and 26.5), but not with the largest to find, whose search then has
 // nothing to hide behind: 64 of 2048 rows 93 and 115.
 bool in_parts(int64_t N, int64_t V, int elem, int top) {
-  const double bytes = bytes_of(N, V, elem);
-  if (bytes < (top ? 450. * (double)(V - 46000) : 700. * (double)(V - 70000))) return true;
-  return !top && bytes >= 128 << 20;
+  const double bytes = bytes_of(N, V, elem), cols = (double)V;
+  if (top) return bytes < std::min(elem == 2 ? std::min(650. * (cols - 51000.), 460. * (cols - 45000.)) : 640. * (cols - 46000.), kFarLogits);
+  return bytes < std::min(700. * (cols - 70000.), 455. * (cols - 38000.)) || bytes >= 128 << 20;
 }
 
 Cut cut_of(int64_t N, int64_t V, int dt, int top) {

@@ -341,8 +341,8 @@ def test_distillations_past_the_caches(N, V, dtype, grad, gpu):
 @pytest.mark.parametrize(
     "N,V,dtype,k",
     [
-        (100, 128100, FP, 0), (70, 128100, FP, 20), (60, 262144, FP, 0), (36, 262145, BF, 64), (20, 1 << 19, FP, 5),
-        (110, 1 << 19, FP, 5),  # whole
+        (100, 128100, FP, 0), (70, 128100, FP, 20), (100, 128100, FP, 5), (60, 262144, FP, 0), (36, 262145, BF, 64), (20, 1 << 19, FP, 5),
+        (130, 1 << 19, FP, 5), (120, 128100, FP, 5),  # whole
         (24, (1 << 21) + 1, FP, 0), (1, 5_000_001, BF, 0), (1, 20_000_000, FP, 0), (1, 1 << 25, BF, 0),
     ],
 )

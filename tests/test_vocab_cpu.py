@@ -434,15 +434,15 @@ def test_long_rows_go_in_parts():
     bytes_of = _lib.load().dsa_vocab_workspace_bytes
     f32, bf16 = _lib.DSA_F32, _lib.DSA_BF16
     for N, V, dt, k in ((1, 10_000_000, f32, 0), (1, 20_000_000, f32, 0), (1, 1 << 25, bf16, 0), (36, 262144, f32, 0), (36, 262144, f32, 5),
-                        (72, 262144, bf16, 5), (90, 262144, f32, 64), (20, 524288, f32, 5), (100, 524288, f32, 128), (100, 1 << 20, f32, 0)):
+                        (72, 262144, bf16, 5), (90, 262144, f32, 64), (20, 524288, f32, 5), (100, 524288, f32, 128), (100, 1 << 20, f32, 0), (100, 128100, f32, 5)):
         assert bytes_of(N, V, dt, k) > 0, (N, V, dt, k)
     # of more columns than this every row is, where no largest are asked for: a lane's chain
-    # is 32 batches at most
+    # is 41 batches at most
     for N in (1, 10, 50, 100, 1000, 100_000):
-        for V in (270_000, 1 << 20, 1 << 27):
+        for V in (340_000, 1 << 20, 1 << 27):
             assert bytes_of(N, V, f32, 0) > 0 and bytes_of(N, V, bf16, 0) > 0, (N, V)
     # short rows are not, nor so many that whole ones fill the card
-    for N, V, dt, k in ((1, 50021, f32, 0), (32, 64000, bf16, 0), (100, 128100, f32, 0), (200, 128100, bf16, 0), (8, 41000, f32, 5),
+    for N, V, dt, k in ((1, 50021, f32, 0), (32, 64000, bf16, 0), (250, 262144, bf16, 0), (100, 128100, f32, 0), (200, 128100, bf16, 0), (8, 41000, f32, 5),
                         (200, 128100, bf16, 20), (256, 262144, f32, 64)):
         assert bytes_of(N, V, dt, k) == 0, (N, V, dt, k)
 
